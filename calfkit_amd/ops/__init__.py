@@ -23,7 +23,14 @@ __all__ = [
     "rope_qk",
     "rope_qkv_write",
     "kv_write",
+    "kv_write_fp8",
+    "kv_read_fp8",
+    "rope_qkv_write_fp8",
+    "rope_qkv_write_slab_fp8",
     "attn_decode",
+    "attn_decode_fp8",
+    "attn_decode_shared",
+    "build_prefix_groups",
     "attn_prefill",
     "attn_prefill_varlen",
     "build_prefill_blocks",
@@ -178,6 +185,211 @@ def kv_write(kcache: torch.Tensor, vcache: torch.Tensor, k: torch.Tensor,
         vcache[p, :, off] = v[t]
 
 
+# ----------------------------------------------------------- e4m3 kv cache
+#
+# Codes float8_e4m3fn [P, Hkv, 64, 128] and scale bytes uint8 [P, Hkv, 64]: one
+# scale 2^(byte - 127) for each (token, KV head), the least power of two that
+# brings the row's largest finite value to 448 (e4m3fn's largest) or less.
+# NaN and infinities are stored as NaN.
+
+def _require(ok: bool, what: str) -> None:
+    if not ok:  # the extension's checks raise the same type
+        raise RuntimeError(what)
+
+
+def _check_fp8_cache(kcache, vcache, kscale, vscale) -> None:
+    for c in (kcache, vcache):
+        _require(c.dtype == torch.float8_e4m3fn,
+                 "the cache must be float8_e4m3fn")
+        _require(c.dim() == 4 and c.shape[2:] == (64, 128) and c.shape[1] > 0
+                 and c.is_contiguous() and c.shape == kcache.shape,
+                 "the caches must be contiguous [P, Hkv, 64, 128]")
+    for c in (kscale, vscale):
+        _require(c.dtype == torch.uint8, "the scales must be uint8")
+        _require(c.shape == kcache.shape[:3] and c.is_contiguous(),
+                 "the scales must be contiguous [P, Hkv, 64]")
+
+
+def _check_rows(t, name: str, rows: int, hkv: int) -> None:
+    _require(t.dtype == torch.bfloat16, f"{name} must be bf16")
+    _require(t.shape == (rows, hkv, 128), f"{name} must be [T, Hkv, 128]")
+    _require(rows == 0 or (t.stride(2) == 1
+                           and (hkv == 1 or t.stride(1) == 128)),
+             f"{name} heads must be contiguous")
+    _require(rows <= 1 or t.stride(0) % 8 == 0,
+             f"{name} rows must start on 16 bytes")
+
+
+def _check_index(t, name: str, rows: int) -> None:
+    _require(t.dtype == torch.int32, f"{name} must be int32")
+    _require(t.shape == (rows,) and t.is_contiguous(),
+             f"{name} must be a contiguous [T]")
+
+
+def _times_pow2(x: torch.Tensor, e: torch.Tensor) -> torch.Tensor:
+    """x * 2^e with 2^e put together from its bits, in two factors that stay
+    normal numbers."""
+    half = torch.div(e, 2, rounding_mode="floor")
+    for part in (half, e - half):
+        x = x * ((part.int() + 127) << 23).view(torch.float32).unsqueeze(-1)
+    return x
+
+
+def _quantise_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    x = x.float()
+    finite = torch.isfinite(x)
+    a = torch.where(finite, x.abs(), 0.0).amax(-1)
+    m, e = torch.frexp(a)
+    e = torch.where(m > 0.875, e - 8, e - 9)  # 448 = 0.875 * 2^9
+    e = torch.where(a > 0, e, 0).clamp_min(-127)
+    y = torch.where(finite, _times_pow2(x, -e), float("nan"))
+    return y.to(torch.float8_e4m3fn), (e + 127).to(torch.uint8)
+
+
+def _dequantise(codes: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+    return _times_pow2(codes.float(), scale.int() - 127)
+
+
+def kv_write_fp8(kcache: torch.Tensor, vcache: torch.Tensor,
+                 kscale: torch.Tensor, vscale: torch.Tensor, k: torch.Tensor,
+                 v: torch.Tensor, slots: torch.Tensor) -> None:
+    """Quantise [T,Hkv,128] bf16 rows into the e4m3 cache at flat slots.
+
+    Rows with a slot outside the cache (negative: padding) are not written.
+    Where one slot is named twice, what it holds afterwards is not defined.
+    """
+    if _native(k):
+        _K.kv_write_fp8(kcache, vcache, kscale, vscale, k, v, slots)
+        return
+    _check_fp8_cache(kcache, vcache, kscale, vscale)
+    T, hkv = k.shape[0], kcache.shape[1]
+    _check_rows(k, "k", T, hkv)
+    _check_rows(v, "v", T, hkv)
+    _check_index(slots, "slots", T)
+    keep = (slots >= 0) & (slots < kcache.shape[0] * 64)
+    s = slots[keep].long()
+    for cache, scale, x in ((kcache, kscale, k), (vcache, vscale, v)):
+        codes, e = _quantise_rows(x[keep])
+        cache.view(torch.uint8)[s // 64, :, s % 64] = codes.view(torch.uint8)
+        scale[s // 64, :, s % 64] = e
+
+
+def kv_read_fp8(k: torch.Tensor, v: torch.Tensor, kcache: torch.Tensor,
+                vcache: torch.Tensor, kscale: torch.Tensor,
+                vscale: torch.Tensor, slots: torch.Tensor) -> None:
+    """Read the e4m3 cache's rows at flat slots back into bf16 [T,Hkv,128].
+
+    Exact: a code has 4 significant bits.  Rows with a slot outside the cache
+    stay as they were.
+    """
+    if _native(k):
+        _K.kv_read_fp8(k, v, kcache, vcache, kscale, vscale, slots)
+        return
+    _check_fp8_cache(kcache, vcache, kscale, vscale)
+    T, hkv = slots.shape[0], kcache.shape[1]
+    _check_rows(k, "k", T, hkv)
+    _check_rows(v, "v", T, hkv)
+    _check_index(slots, "slots", T)
+    keep = (slots >= 0) & (slots < kcache.shape[0] * 64)
+    s = slots[keep].long()
+    for cache, scale, x in ((kcache, kscale, k), (vcache, vscale, v)):
+        codes = cache.view(torch.uint8)[s // 64, :, s % 64]
+        x[keep] = _dequantise(codes.view(torch.float8_e4m3fn),
+                              scale[s // 64, :, s % 64]).to(x.dtype)
+
+
+def _check_rope(qkv, cos_sin, positions, slots, hq: int, hkv: int, kcache,
+                q_out) -> None:
+    T = qkv.shape[0]
+    _require(hq > 0 and hkv == kcache.shape[1],
+             "hkv does not match the cache")
+    _require(qkv.dtype == torch.bfloat16 and qkv.dim() == 2
+             and qkv.is_contiguous() and qkv.shape[1] == (hq + 2 * hkv) * 128,
+             "qkv must be a contiguous bf16 [T, (hq + 2 hkv) * 128]")
+    _require(cos_sin.dtype == torch.float32 and cos_sin.dim() == 2
+             and cos_sin.shape[1] == 128 and cos_sin.shape[0] > 0
+             and cos_sin.is_contiguous(),
+             "cos_sin must be a contiguous f32 [max_pos, 128]")
+    _check_index(positions, "positions", T)
+    _check_index(slots, "slots", T)
+    _require(q_out is None or (
+        q_out.dtype == torch.bfloat16 and q_out.shape == (T, hq, 128)
+        and q_out.is_contiguous()),
+        "q_out must be a contiguous bf16 [T, hq, 128]")
+
+
+def _rotate(x: torch.Tensor, cos_sin: torch.Tensor,
+            positions: torch.Tensor) -> torch.Tensor:
+    """f32 [T, heads, 128] rotated by each row's position."""
+    at = positions.long().clamp(0, cos_sin.shape[0] - 1)
+    cos, sin = cos_sin[at].unsqueeze(1).split(64, dim=-1)
+    lo, hi = x.split(64, dim=-1)
+    return torch.cat([lo * cos - hi * sin, hi * cos + lo * sin], dim=-1)
+
+
+def rope_qkv_write_fp8(qkv: torch.Tensor, kcache: torch.Tensor,
+                       vcache: torch.Tensor, kscale: torch.Tensor,
+                       vscale: torch.Tensor, cos_sin: torch.Tensor,
+                       positions: torch.Tensor, slots: torch.Tensor,
+                       hq: int, hkv: int,
+                       q_out: torch.Tensor | None = None) -> None:
+    """``rope_qkv_write`` into the e4m3 cache (one launch).
+
+    Rotates the Q and K heads in place inside the packed
+    [T, (hq+2*hkv)*128] rows; with ``q_out`` [T, hq, 128] the rotated queries
+    go there and qkv stays as it was.  What is quantised are the rotated
+    values as bf16 holds them, so the cache and the packed rows say the same.
+    Positions are taken into the table's range; slots as in
+    ``kv_write_fp8``.
+    """
+    if _native(qkv):
+        _K.rope_qkv_write_fp8(qkv, kcache, vcache, kscale, vscale, cos_sin,
+                              positions, slots, hq, hkv, q_out)
+        return
+    _check_fp8_cache(kcache, vcache, kscale, vscale)
+    _check_rope(qkv, cos_sin, positions, slots, hq, hkv, kcache, q_out)
+    T = qkv.shape[0]
+    rows = qkv.view(T, hq + 2 * hkv, 128)
+    turned = _rotate(rows[:, :hq + hkv].float(), cos_sin,
+                     positions).to(qkv.dtype)
+    kv_write_fp8(kcache, vcache, kscale, vscale, turned[:, hq:],
+                 rows[:, hq + hkv:], slots)
+    if q_out is not None:
+        q_out.copy_(turned[:, :hq])
+    else:
+        rows[:, :hq + hkv] = turned
+
+
+def rope_qkv_write_slab_fp8(qkv: torch.Tensor, work: torch.Tensor,
+                            kcache: torch.Tensor, vcache: torch.Tensor,
+                            kscale: torch.Tensor, vscale: torch.Tensor,
+                            cos_sin: torch.Tensor, positions: torch.Tensor,
+                            slots: torch.Tensor, hq: int, hkv: int,
+                            Mp: int, splitk: int) -> None:
+    """``rope_qkv_write_slab`` into the e4m3 cache: the rows are the sums of
+    the split-K slabs, rotated before they are rounded to bf16."""
+    if _native(qkv):
+        _K.rope_qkv_write_slab_fp8(qkv, work, kcache, vcache, kscale, vscale,
+                                   cos_sin, positions, slots, hq, hkv, Mp,
+                                   splitk)
+        return
+    _check_fp8_cache(kcache, vcache, kscale, vscale)
+    _check_rope(qkv, cos_sin, positions, slots, hq, hkv, kcache, None)
+    T, W = qkv.shape
+    _require(work.dtype == torch.float32 and work.is_contiguous(),
+             "work must be contiguous f32")
+    _require(splitk >= 1 and Mp >= T and work.numel() >= splitk * Mp * W,
+             "work is too small for its slabs")
+    x = work.view(-1)[: splitk * Mp * W].view(splitk, Mp, W)[:, :T].sum(0)
+    x = x.view(T, hq + 2 * hkv, 128)
+    rows = qkv.view(T, hq + 2 * hkv, 128)
+    rows[:, :hq + hkv] = _rotate(x[:, :hq + hkv], cos_sin,
+                                 positions).to(qkv.dtype)
+    rows[:, hq + hkv:] = x[:, hq + hkv:].to(qkv.dtype)
+    kv_write_fp8(kcache, vcache, kscale, vscale, rows[:, hq:hq + hkv],
+                 rows[:, hq + hkv:], slots)
+
+
 # ---------------------------------------------------------------- attention
 
 def attn_decode(out: torch.Tensor, q: torch.Tensor, kcache: torch.Tensor,
@@ -202,6 +414,179 @@ def attn_decode(out: torch.Tensor, q: torch.Tensor, kcache: torch.Tensor,
             s = (kk[:, kvh] @ (q[b, h].float() * scale)) # [n]
             p = torch.softmax(s, dim=-1)
             out[b, h] = (p @ vv[:, kvh]).to(out.dtype)
+
+
+def _check_paged(out, q, kcache, page_table, seq_lens) -> None:
+    _require(q.dtype == torch.bfloat16 and q.dim() == 3 and q.shape[2] == 128,
+             "q must be bf16 [B, hq, 128]")
+    B, hq, hkv = q.shape[0], q.shape[1], kcache.shape[1]
+    _require(B == 0 or (q.stride(2) == 1 and (hq == 1 or q.stride(1) == 128)),
+             "q heads must be contiguous")
+    _require(B <= 1 or q.stride(0) % 8 == 0, "q rows must start on 16 bytes")
+    _require(out.dtype == torch.bfloat16 and out.shape == q.shape
+             and out.is_contiguous(),
+             "out must be contiguous bf16 of q's shape")
+    _require(hq % hkv == 0 and hq // hkv <= 16,
+             "hq must be a multiple of hkv, up to 16 times it")
+    _require(page_table.dtype == torch.int32 and page_table.dim() == 2
+             and page_table.shape[0] == B and page_table.is_contiguous(),
+             "page_table must be a contiguous int32 [B, max_pages]")
+    _require(seq_lens.dtype == torch.int32 and seq_lens.shape == (B,)
+             and seq_lens.is_contiguous(),
+             "seq_lens must be a contiguous int32 [B]")
+
+
+def _attend_rows(out, q, pages_of, seq_lens, max_pages, hkv, num_pages,
+                 scale: float) -> None:
+    """The paged attention of both cache types, row by row in f32."""
+    B, hq, dh = q.shape
+    for b in range(B):
+        n = min(max(int(seq_lens[b]), 0), max_pages * 64)
+        out[b] = 0
+        if n == 0:
+            continue
+        pages, k, v = pages_of(b, (n + 63) // 64)
+        k, v = (x.permute(1, 0, 2, 3).reshape(hkv, -1, dh)[:, :n]
+                for x in (k, v))
+        there = ((pages >= 0) & (pages < num_pages)).repeat_interleave(64)[:n]
+        if not bool(there.any()):
+            continue
+        k, v = k[:, there], v[:, there]
+        s = (q[b].float().view(hkv, hq // hkv, dh) @ k.transpose(1, 2)) * scale
+        out[b] = (torch.softmax(s, -1) @ v).reshape(hq, dh).to(out.dtype)
+
+
+def attn_decode_fp8(out: torch.Tensor, q: torch.Tensor, kcache: torch.Tensor,
+                    vcache: torch.Tensor, kscale: torch.Tensor,
+                    vscale: torch.Tensor, page_table: torch.Tensor,
+                    seq_lens: torch.Tensor, scale: float) -> None:
+    """``attn_decode`` over the e4m3 cache. q/out: [B,Hq,128].
+
+    Long sequences are split over the card and joined.  A row of length 0
+    gives zeros; lengths are taken up to the table's width; a page id outside
+    the cache counts as a page without tokens.
+    """
+    if _native(q):
+        _K.attn_decode_fp8(out, q, kcache, vcache, kscale, vscale, page_table,
+                           seq_lens, scale)
+        return
+    _check_fp8_cache(kcache, vcache, kscale, vscale)
+    _check_paged(out, q, kcache, page_table, seq_lens)
+    P = kcache.shape[0]
+
+    def pages_of(b: int, count: int):
+        pages = page_table[b, :count].long()
+        at = pages.clamp(0, P - 1)
+        return (pages, _dequantise(kcache[at], kscale[at]),
+                _dequantise(vcache[at], vscale[at]))
+
+    _attend_rows(out, q, pages_of, seq_lens, page_table.shape[1],
+                 kcache.shape[1], P, scale)
+
+
+def attn_decode_shared(out: torch.Tensor, q: torch.Tensor,
+                       kcache: torch.Tensor, vcache: torch.Tensor,
+                       page_table: torch.Tensor, seq_lens: torch.Tensor,
+                       group: torch.Tensor, group_lens: torch.Tensor,
+                       scale: float, kscale: torch.Tensor | None = None,
+                       vscale: torch.Tensor | None = None) -> None:
+    """Paged GQA decode attention for a batch whose rows share prefixes.
+
+    ``group`` [B] i32 names each row's prefix group (< 0: none) and
+    ``group_lens`` [groups <= 64] i32 the tokens its rows have in common, in
+    the same pages: each prefix is attended once for all its rows, the rest
+    row by row, and the two are joined.  ``build_prefix_groups`` finds the
+    groups.  The result is that of ``attn_decode`` (or, with the scales of
+    an e4m3 cache, ``attn_decode_fp8``) up to the order of its sums, whatever
+    the grouping.
+    """
+    if _native(q):
+        _K.attn_decode_shared(out, q, kcache, vcache, page_table, seq_lens,
+                              group, group_lens, scale, kscale, vscale)
+        return
+    _require((kscale is None) == (vscale is None),
+             "kscale and vscale come together")
+    if kscale is not None:
+        _check_fp8_cache(kcache, vcache, kscale, vscale)
+    else:
+        for c in (kcache, vcache):
+            _require(c.dtype == torch.bfloat16,
+                     "a cache without scales must be bf16")
+            _require(c.dim() == 4 and c.shape[2:] == (64, 128)
+                     and c.shape[1] > 0 and c.is_contiguous()
+                     and c.shape == kcache.shape,
+                     "the caches must be contiguous [P, Hkv, 64, 128]")
+    _check_paged(out, q, kcache, page_table, seq_lens)
+    B, P = q.shape[0], kcache.shape[0]
+    _require(group.dtype == torch.int32 and group.shape == (B,)
+             and group.is_contiguous(),
+             "group must be a contiguous int32 [B]")
+    _require(group_lens.dtype == torch.int32 and group_lens.dim() == 1
+             and group_lens.is_contiguous(),
+             "group_lens must be a contiguous int32 [groups]")
+    _require(group_lens.shape[0] <= 64, "at most 64 prefix groups")
+    first: dict[int, int] = {}  # group -> the row whose pages stand for it
+    for b, g in enumerate(group.tolist()):
+        if 0 <= g < group_lens.shape[0]:
+            first.setdefault(g, b)
+
+    def pages_of(b: int, count: int):
+        pages = page_table[b, :count].long()
+        g = int(group[b])
+        if g in first:
+            upto = min(max(int(group_lens[g]), 0), count * 64)
+            pages = pages.clone()
+            # a prefix's last page may be its rows' own beyond the prefix:
+            # the common tokens of it lie in the first row's page
+            pages[:upto // 64] = page_table[first[g], :upto // 64].long()
+        at = pages.clamp(0, P - 1)
+        if kscale is None:
+            return pages, kcache[at].float(), vcache[at].float()
+        return (pages, _dequantise(kcache[at], kscale[at]),
+                _dequantise(vcache[at], vscale[at]))
+
+    _attend_rows(out, q, pages_of, seq_lens, page_table.shape[1],
+                 kcache.shape[1], P, scale)
+
+
+def build_prefix_groups(page_table: "np.ndarray", lengths: "np.ndarray",
+                        max_groups: int = 64, min_rows: int = 2,
+                        min_pages: int = 1) -> tuple["np.ndarray",
+                                                     "np.ndarray"]:
+    """Host-side prefix groups of a batch for ``attn_decode_shared``.
+
+    page_table [B, max_pages] and lengths [B] as numpy arrays.  Rows with the
+    same first page form a group; its prefix is the run of whole pages that
+    all of them have in common.  Groups of fewer rows or pages than the
+    minimum are left out, and of more than ``max_groups`` those that save the
+    least reading.  Returns (group [B] i32, group_lens [max_groups] i32).
+    """
+    import numpy as np
+
+    B = page_table.shape[0]
+    group = np.full(B, -1, dtype=np.int32)
+    lens = np.zeros(max_groups, dtype=np.int32)
+    whole = np.minimum(np.asarray(lengths) // 64, page_table.shape[1])
+    rows = np.flatnonzero(whole >= max(1, min_pages))
+    if rows.size == 0:
+        return group, lens
+    found = []
+    heads, where = np.unique(page_table[rows, 0], return_inverse=True)
+    for h in range(heads.size):
+        members = rows[where == h]
+        if members.size < max(2, min_rows):
+            continue
+        most = int(whole[members].min())
+        same = (page_table[members, :most]
+                == page_table[members[0], :most]).all(0)
+        pages = most if same.all() else int(np.argmin(same))
+        if pages >= max(1, min_pages):
+            found.append(((members.size - 1) * pages, pages, members))
+    found.sort(key=lambda f: -f[0])
+    for g, (_, pages, members) in enumerate(found[:max_groups]):
+        group[members] = g
+        lens[g] = pages * 64
+    return group, lens
 
 
 def attn_prefill(out: torch.Tensor, q: torch.Tensor, k: torch.Tensor,

@@ -1,0 +1,787 @@
+// Single-token GQA attention on MFMA over a paged cache, bf16 or e4m3, with
+// the work split over long sequences and prefixes that many rows share
+// computed once for all of them (MI355X, gfx950).
+//
+//   out[b, h] = sum_j softmax_j(scale * q[b, h] . K_j) V_j,   j < seq_lens[b]
+//
+// A softmax over a union of token ranges joins from each range's
+// (m = max s, l = sum exp(s - m), o = sum exp(s - m) V): with M = max m,
+// out = sum exp(m - M) o / sum exp(m - M) l.  m, l, o are held in fp32 and s
+// in units of log2, so that the exponential is one v_exp_f32.
+//
+// Everything is computed transposed, so that softmax stays inside a lane:
+//   S^T = K Q^T  (A = K rows as they lie in the cache, B = Q rows),
+//   O^T = V^T P^T (A = V^T through the LDS transposing read, B = P).
+// C of the first product holds, for ONE query row per lane, the tokens
+// g*4 + reg of each tile (g = the lane's group of 16, or of 32); B of the
+// second wants 8 tokens a lane.  A sum over tokens may take them in any order,
+// so B's slots m = 0..7 are read as {4 tokens of one half, 4 of the other}
+// and V^T is read in the same order: P never leaves its registers.
+//
+// P is rounded to bf16 for the matrix instruction (2^-9 of each weight, with
+// independent signs: the same size as the rounding of the output itself);
+// its sum l is taken before that rounding.
+//
+// e4m3 rows become bf16 on the way in (scale times code is exact in bf16), so
+// both caches share one arithmetic.
+
+#include "common.h"
+#include "fp8.h"
+
+#define HD 128
+#define KVPAGE 64
+#define MAXG 16        // query heads of one KV head: one MFMA column block
+#define MAXGROUPS 64   // prefix groups of one call: one wave finds a tile's
+
+using f32x4 = __attribute__((ext_vector_type(4))) float;
+using f32x16 = __attribute__((ext_vector_type(16))) float;
+using bf16x8v = __attribute__((ext_vector_type(8))) __bf16;
+using s16x4 = __attribute__((ext_vector_type(4))) short;
+using s16x8 = __attribute__((ext_vector_type(8))) short;
+using u32x4 = __attribute__((ext_vector_type(4))) unsigned;
+
+#define MFMA16(a, b, c) __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0)
+#define MFMA32(a, b, c) __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0)
+
+// Row pitch of V in LDS, in halfwords: 288 B = 72 banks, so that the 4-token
+// blocks of a transposing read fall on banks 8 apart.
+#define V_PITCH 144
+// Row pitch of K: 272 B, 16 B reads of 16 rows cover all banks.
+#define K_PITCH 136
+
+namespace {
+
+// 4 tokens x 16 dims of 16 lanes, transposed: lane i gets dim i's 4 tokens.
+__device__ __forceinline__ s16x4 read_tr(const __hip_bfloat16* p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (__attribute__((address_space(3))) s16x4*)(p));
+}
+
+__device__ __forceinline__ bf16x8v join(s16x4 a, s16x4 b) {
+  const s16x8 r = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+  return __builtin_bit_cast(bf16x8v, r);
+}
+
+// 16 codes of one row -> two vectors of 8 bf16.
+__device__ __forceinline__ void widen(const u32x4 c, const float s, u32x4& lo,
+                                      u32x4& hi) {
+  lo = (u32x4){e4m3_to_bf16x2<false>(c[0], s), e4m3_to_bf16x2<true>(c[0], s),
+               e4m3_to_bf16x2<false>(c[1], s), e4m3_to_bf16x2<true>(c[1], s)};
+  hi = (u32x4){e4m3_to_bf16x2<false>(c[2], s), e4m3_to_bf16x2<true>(c[2], s),
+               e4m3_to_bf16x2<false>(c[3], s), e4m3_to_bf16x2<true>(c[3], s)};
+}
+
+__device__ __forceinline__ float exp2_fast(const float x) {
+  return __builtin_amdgcn_exp2f(x);
+}
+
+struct Paged {
+  const void* kcache;        // [P, hkv, 64, 128] bf16 or e4m3
+  const void* vcache;
+  const uint8_t* kscale;     // [P, hkv, 64] or null
+  const uint8_t* vscale;
+  const __hip_bfloat16* q;   // [B, hq, 128], rows q_stride apart
+  const int32_t* page_table;  // [B, max_pages]
+  const int32_t* seq_lens;    // [B]
+  const int32_t* group;       // [B] or null: prefix group, < 0 for none
+  const int32_t* group_lens;  // [ngroups] tokens of each group's prefix
+  float* part_o;              // [B * hq, slots, 128]
+  float* part_ml;             // [B * hq, slots, 2]
+  int64_t q_stride;
+  int B, hq, hkv, G, max_pages, num_pages, ngroups;
+  int nshared, nsplit;  // partial slots of the prefix and of the rest
+  float scale_log2;     // scale * log2(e)
+};
+
+__device__ __forceinline__ int row_len(const Paged& a, const int b) {
+  return min(max(a.seq_lens[b], 0), a.max_pages * KVPAGE);
+}
+
+// Tokens of row b that its group's shared pass covers.
+__device__ __forceinline__ int prefix_len(const Paged& a, const int b,
+                                          const int n) {
+  if (a.group == nullptr) return 0;
+  const int g = a.group[b];
+  return (g >= 0 && g < a.ngroups) ? min(max(a.group_lens[g], 0), n) : 0;
+}
+
+}  // namespace
+
+// ------------------------------------------------------------ each row's own
+//
+// One block = (row, KV head, split): NW waves take the split's pages in turn.
+// A wave reads K straight into A fragments (a lane's 16 B of one token; the
+// Q fragments take the dims in the same order) and turns V in its own LDS
+// page, so that the page loop has no block barrier.  Bound: the bytes of the
+// cache; the matrix instructions run mostly empty (G of 16 columns) and still
+// take a tenth of the vector instructions that dot products would.
+template <bool FP8, int NW>
+__global__ __launch_bounds__(NW* WAVE, 2) void paged_decode_kernel(
+    const Paged a, __hip_bfloat16* __restrict__ out) {
+  __shared__ __attribute__((aligned(16)))
+  __hip_bfloat16 v_lds[NW][KVPAGE * V_PITCH];
+  __shared__ float ml_lds[NW][MAXG][2];
+
+  const int b = blockIdx.x, kvh = blockIdx.y, split = blockIdx.z;
+  const int wid = threadIdx.x / WAVE, lane = threadIdx.x % WAVE;
+  const int l16 = lane & 15, g4 = lane >> 4;
+  const int n = row_len(a, b);
+  const int first = prefix_len(a, b, n);
+  const int page0 = first / KVPAGE;
+  const int npages = (n + KVPAGE - 1) / KVPAGE - page0;
+  const int each = (max(npages, 0) + a.nsplit - 1) / a.nsplit;
+  const int pbegin = page0 + split * each;
+  const int pend = page0 + min(npages, (split + 1) * each);
+
+  // fragment c of lane group g4 holds dims 32c + 8*g4 .. of a bf16 row, or of
+  // an e4m3 row (whose 16 B are 16 dims) 64*(c/2) + 16*g4 + 8*(c%2) ..
+  bf16x8v qf[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const int d = FP8 ? (c / 2) * 64 + g4 * 16 + (c % 2) * 8 : c * 32 + g4 * 8;
+    u32x4 v = {0, 0, 0, 0};
+    if (l16 < a.G)
+      v = *reinterpret_cast<const u32x4*>(
+          a.q + b * a.q_stride + (kvh * a.G + l16) * HD + d);
+    qf[c] = __builtin_bit_cast(bf16x8v, v);
+  }
+
+  float m = -INFINITY, l = 0.f;
+  f32x4 o[8];
+#pragma unroll
+  for (int d = 0; d < 8; ++d) o[d] = (f32x4){0.f, 0.f, 0.f, 0.f};
+
+  __hip_bfloat16* vt = v_lds[wid];
+  const __hip_bfloat16* vt_read =
+      vt + (g4 * 4 + (l16 >> 2)) * V_PITCH + (l16 & 3) * 4;
+  const int32_t* table = a.page_table + (int64_t)b * a.max_pages;
+
+  for (int pi = pbegin + wid; pi < pend; pi += NW) {
+    const int page = table[pi];
+    if (page < 0 || page >= a.num_pages) continue;  // no such page: no tokens
+    const int64_t panel = ((int64_t)page * a.hkv + kvh) * KVPAGE;
+    const int tok0 = pi * KVPAGE;
+    const bool whole = tok0 >= first && tok0 + KVPAGE <= n;
+
+    constexpr int KLD = FP8 ? 2 : 4;    // 16 B loads of a lane, a 16-token tile
+    constexpr int VLD = FP8 ? 8 : 16;   // 16 B loads of a lane, a page of V
+    constexpr int VROW = FP8 ? 8 : 16;  // lanes of one row of V
+    u32x4 kr[4][KLD], vr[VLD];
+    unsigned char ks[4], vs[VLD];
+    const char* kp = (const char*)a.kcache + panel * (FP8 ? HD : 2 * HD);
+    const char* vp = (const char*)a.vcache + panel * (FP8 ? HD : 2 * HD);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+#pragma unroll
+      for (int c = 0; c < KLD; ++c)
+        kr[t][c] = *reinterpret_cast<const u32x4*>(
+            kp + (t * 16 + l16) * (FP8 ? HD : 2 * HD) + c * 64 + g4 * 16);
+      if (FP8) ks[t] = a.kscale[panel + t * 16 + l16];
+    }
+#pragma unroll
+    for (int i = 0; i < VLD; ++i) {
+      vr[i] = *reinterpret_cast<const u32x4*>(vp + (i * WAVE + lane) * 16);
+      if (FP8) vs[i] = a.vscale[panel + (i * WAVE + lane) / VROW];
+    }
+
+    f32x4 s[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      u32x4 kf[4];
+      if constexpr (FP8) {
+        const float sc = e8m0_scale(ks[t]);
+        widen(kr[t][0], sc, kf[0], kf[1]);
+        widen(kr[t][1], sc, kf[2], kf[3]);
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) kf[c] = kr[t][c];
+      }
+      s[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        s[t] = MFMA16(__builtin_bit_cast(bf16x8v, kf[c]), qf[c], s[t]);
+    }
+
+    float mt = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        s[t][r] *= a.scale_log2;
+        if (!whole) {
+          const int tok = tok0 + t * 16 + g4 * 4 + r;
+          if (tok < first || tok >= n) s[t][r] = -INFINITY;
+        }
+        mt = fmaxf(mt, s[t][r]);
+      }
+    mt = fmaxf(mt, __shfl_xor(mt, 16, WAVE));
+    mt = fmaxf(mt, __shfl_xor(mt, 32, WAVE));
+    const float mn = fmaxf(m, mt);
+    const float mu = (mn == -INFINITY) ? 0.f : mn;  // nothing seen yet
+    const float keep = exp2_fast(m - mu);
+    m = mn;
+    l *= keep;
+#pragma unroll
+    for (int d = 0; d < 8; ++d) o[d] *= keep;
+
+    bf16x8v pf[2];
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float p = exp2_fast(s[t][r] - mu);
+        l += p;
+        pf[t >> 1][(t & 1) * 4 + r] = (__bf16)p;
+      }
+
+    // V to LDS as bf16; rows outside the sequence as zeros (weight 0 times
+    // whatever a recycled page holds may be NaN)
+#pragma unroll
+    for (int i = 0; i < VLD; ++i) {
+      const int row = (i * WAVE + lane) / VROW;
+      const int tok = tok0 + row;
+      const bool gone = !whole && (tok < first || tok >= n);
+      __hip_bfloat16* dst = vt + row * V_PITCH;
+      if constexpr (FP8) {
+        u32x4 lo, hi;
+        widen(vr[i], e8m0_scale(vs[i]), lo, hi);
+        if (gone) lo = hi = (u32x4){0, 0, 0, 0};
+        dst += (lane % VROW) * 16;
+        reinterpret_cast<u32x4*>(dst)[0] = lo;
+        reinterpret_cast<u32x4*>(dst)[1] = hi;
+      } else {
+        if (gone) vr[i] = (u32x4){0, 0, 0, 0};
+        reinterpret_cast<u32x4*>(dst + (lane % VROW) * 8)[0] = vr[i];
+      }
+    }
+    // one wave's LDS operations run in order: only the compiler has to be told
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int d = 0; d < 8; ++d) {
+        const __hip_bfloat16* p = vt_read + u * 32 * V_PITCH + d * 16;
+        o[d] = MFMA16(join(read_tr(p), read_tr(p + 16 * V_PITCH)), pf[u], o[d]);
+      }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+
+  l += __shfl_xor(l, 16, WAVE);
+  l += __shfl_xor(l, 32, WAVE);
+
+  // ---- join the waves: O rows over the V pages, now free
+  __syncthreads();
+  float* o_lds = reinterpret_cast<float*>(&v_lds[0][0]);  // [NW][16][128]
+  if (l16 < a.G) {
+#pragma unroll
+    for (int d = 0; d < 8; ++d)
+      *reinterpret_cast<f32x4*>(
+          &o_lds[(wid * MAXG + l16) * HD + d * 16 + g4 * 4]) = o[d];
+    if (g4 == 0) {
+      ml_lds[wid][l16][0] = m;
+      ml_lds[wid][l16][1] = l;
+    }
+  }
+  __syncthreads();
+  const int slots = a.nshared + a.nsplit;
+  for (int i = threadIdx.x; i < a.G * HD; i += NW * WAVE) {
+    const int g = i / HD, d = i % HD;
+    const int64_t row = (int64_t)b * a.hq + kvh * a.G + g;
+    const float* pml = a.part_ml + row * slots * 2;
+    const int joined = (a.nsplit == 1 && first > 0) ? a.nshared : 0;
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) M = fmaxf(M, ml_lds[w][g][0]);
+    for (int k = 0; k < joined; ++k) M = fmaxf(M, pml[k * 2]);
+    const float mu = (M == -INFINITY) ? 0.f : M;
+    float L = 0.f, acc = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float c = exp2_fast(ml_lds[w][g][0] - mu);
+      L = fmaf(c, ml_lds[w][g][1], L);
+      acc = fmaf(c, o_lds[(w * MAXG + g) * HD + d], acc);
+    }
+    for (int k = 0; k < joined; ++k) {
+      const float lk = pml[k * 2 + 1];
+      if (lk == 0.f) continue;  // an empty range: its o is not written
+      const float c = exp2_fast(pml[k * 2] - mu);
+      L = fmaf(c, lk, L);
+      acc = fmaf(c, a.part_o[(row * slots + k) * HD + d], acc);
+    }
+    if (a.nsplit == 1) {
+      // no weight at all (an empty row): zeros
+      out[row * HD + d] = f2bf(L == 0.f ? 0.f : acc / L);
+    } else {
+      const int64_t slot = row * slots + a.nshared + split;
+      a.part_o[slot * HD + d] = acc;
+      if (d == 0) {
+        a.part_ml[slot * 2] = M;
+        a.part_ml[slot * 2 + 1] = L;
+      }
+    }
+  }
+}
+
+// Joins the partial slots of one (row, head): a wave each, 2 dims a lane.
+__global__ __launch_bounds__(4 * WAVE) void paged_join_kernel(
+    const Paged a, __hip_bfloat16* __restrict__ out) {
+  const int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / WAVE;
+  if (row >= (int64_t)a.B * a.hq) return;
+  const int lane = threadIdx.x % WAVE;
+  const int b = (int)(row / a.hq);
+  const int slots = a.nshared + a.nsplit;
+  const bool has_prefix = prefix_len(a, b, row_len(a, b)) > 0;
+  const int from = has_prefix ? 0 : a.nshared;
+  const float* ml = a.part_ml + row * slots * 2;
+  float M = -INFINITY;
+  for (int k = from; k < slots; ++k) M = fmaxf(M, ml[k * 2]);
+  const float mu = (M == -INFINITY) ? 0.f : M;
+  float L = 0.f, o0 = 0.f, o1 = 0.f;
+  for (int k = from; k < slots; ++k) {
+    const float lk = ml[k * 2 + 1];
+    if (lk == 0.f) continue;
+    const float c = exp2_fast(ml[k * 2] - mu);
+    const float2 o =
+        reinterpret_cast<const float2*>(a.part_o + (row * slots + k) * HD)[lane];
+    L = fmaf(c, lk, L);
+    o0 = fmaf(c, o.x, o0);
+    o1 = fmaf(c, o.y, o1);
+  }
+  const float inv = (L == 0.f) ? 0.f : 1.f / L;
+  __hip_bfloat16* dst = out + row * HD + lane * 2;
+  dst[0] = f2bf(L == 0.f ? 0.f : o0 * inv);
+  dst[1] = f2bf(L == 0.f ? 0.f : o1 * inv);
+}
+
+// -------------------------------------------------------- the shared prefix
+//
+// One block = (KV head, split of the prefix, tile of up to 128 query rows of
+// one group): rows (b, g) of the group's members in batch order.  4 waves own
+// 32 rows each; pages of K and V pass through LDS, double-buffered, the next
+// page's loads in flight under this page's products.  Bound: the matrix
+// instructions and, at 32 rows a wave, LDS reads at the same rate (each 1 KB
+// fragment feeds one 32x32x16 product of 32 cycles, four SIMDs to 128 B a
+// cycle).  blockIdx.x is the KV head, so that with 8 of them each XCD's L2
+// holds one head's prefix for every tile and split.
+template <bool FP8>
+__global__ __launch_bounds__(4 * WAVE, 2) void paged_shared_kernel(
+    const Paged a) {
+  __shared__ __attribute__((aligned(16)))
+  __hip_bfloat16 k_lds[2][KVPAGE * K_PITCH];
+  __shared__ __attribute__((aligned(16)))
+  __hip_bfloat16 v_lds[2][KVPAGE * V_PITCH];
+  __shared__ int counts[MAXGROUPS];
+  __shared__ int tile_rows[128];
+  __shared__ int tile_of[4];  // group, its tile, rows in it, longest row
+
+  const int kvh = blockIdx.x, split = blockIdx.y, tile = blockIdx.z;
+  const int tid = threadIdx.x;
+  const int wid = tid / WAVE, lane = tid % WAVE;
+  const int per_tile = 128 / a.G;
+
+  // ---- which group's which rows: count members, walk the tiles, then the
+  // members in batch order (a few hundred loads from L2)
+  if (tid < MAXGROUPS) counts[tid] = 0;
+  __syncthreads();
+  for (int b = tid; b < a.B; b += 4 * WAVE) {
+    const int g = a.group[b];
+    if (g >= 0 && g < a.ngroups) atomicAdd(&counts[g], 1);
+  }
+  __syncthreads();
+  if (wid == 0) {
+    const int tiles = (counts[lane] + per_tile - 1) / per_tile;
+    int upto = tiles;
+#pragma unroll
+    for (int off = 1; off < WAVE; off <<= 1) {
+      const int x = __shfl_up(upto, off, WAVE);
+      if (lane >= off) upto += x;
+    }
+    const bool mine = tile >= upto - tiles && tile < upto;
+    if (lane == 0) tile_of[0] = -1;
+    __builtin_amdgcn_wave_barrier();
+    if (mine) {
+      tile_of[0] = lane;
+      tile_of[1] = tile - (upto - tiles);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const int g = tile_of[0];
+    if (g >= 0) {
+      const int skip = tile_of[1] * per_tile;
+      int seen = 0, longest = 0;
+      for (int b0 = 0; b0 < a.B && seen < skip + per_tile; b0 += WAVE) {
+        const int b = b0 + lane;
+        const bool in = b < a.B && a.group[b] == g;
+        const unsigned long long bal = __ballot(in);
+        const int rank = seen + __popcll(bal & ((1ull << lane) - 1)) - skip;
+        if (in && rank >= 0 && rank < per_tile) {
+          tile_rows[rank] = b;
+          longest = max(longest, row_len(a, b));
+        }
+        seen += __popcll(bal);
+      }
+#pragma unroll
+      for (int off = 32; off > 0; off >>= 1)
+        longest = max(longest, __shfl_xor(longest, off, WAVE));
+      if (lane == 0) {
+        tile_of[2] = min(seen - skip, per_tile);
+        tile_of[3] = longest;
+      }
+    }
+  }
+  __syncthreads();
+  const int grp = tile_of[0];
+  if (grp < 0) return;  // fewer tiles than blocks
+  const int nrows = tile_of[2] * a.G;
+
+  // no token past the longest row: what lies there may be anything
+  const int glen = min(max(a.group_lens[grp], 0), tile_of[3]);
+  const int npages = (glen + KVPAGE - 1) / KVPAGE;
+  const int each = (npages + a.nshared - 1) / a.nshared;
+  const int pbegin = split * each;
+  const int pend = min(npages, pbegin + each);
+  const int32_t* table = a.page_table + (int64_t)tile_rows[0] * a.max_pages;
+
+  // ---- this wave's 32 query rows: one a lane, halves h of the MFMA's K
+  const int r32 = lane & 31, h = lane >> 5;
+  const int i = wid * 32 + r32;
+  const bool live = i < nrows;
+  const int b = tile_rows[live ? i / a.G : 0];
+  const int head = kvh * a.G + (live ? i % a.G : 0);
+  // a lane without a row computes row 0 again and writes nothing
+  const int limit = live ? min(row_len(a, b), glen) : glen;
+  const bool wave_live = wid * 32 < nrows;
+  bf16x8v qf[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    qf[k] = *reinterpret_cast<const bf16x8v*>(
+        a.q + b * a.q_stride + head * HD + k * 16 + h * 8);
+
+  float m = -INFINITY, l = 0.f;
+  f32x16 o[4];
+#pragma unroll
+  for (int d = 0; d < 4; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+
+  constexpr int LD = FP8 ? 2 : 4;     // 16 B loads of a thread, a page
+  constexpr int ROW = FP8 ? 8 : 16;   // threads of one row
+  u32x4 kr[LD], vr[LD];
+  unsigned char ks[LD], vs[LD];
+  const int trow = tid / ROW, tcol = tid % ROW;
+
+  auto fetch = [&](int pi) {
+    const int page = table[pi];
+    const bool ok = page >= 0 && page < a.num_pages;
+    const int64_t panel = ((int64_t)(ok ? page : 0) * a.hkv + kvh) * KVPAGE;
+    const char* kp = (const char*)a.kcache + panel * (FP8 ? HD : 2 * HD);
+    const char* vp = (const char*)a.vcache + panel * (FP8 ? HD : 2 * HD);
+#pragma unroll
+    for (int j = 0; j < LD; ++j) {
+      kr[j] = *reinterpret_cast<const u32x4*>(kp + (j * 4 * WAVE + tid) * 16);
+      vr[j] = *reinterpret_cast<const u32x4*>(vp + (j * 4 * WAVE + tid) * 16);
+      if (FP8) {
+        const int64_t at = panel + j * (4 * WAVE / ROW) + trow;
+        ks[j] = a.kscale[at];
+        vs[j] = a.vscale[at];
+      }
+    }
+    return ok;
+  };
+  auto stage = [&](int buf, int pi) {
+#pragma unroll
+    for (int j = 0; j < LD; ++j) {
+      const int row = j * (4 * WAVE / ROW) + trow;
+      const bool gone = pi * KVPAGE + row >= glen;  // NaN there times weight 0
+      __hip_bfloat16* kd = &k_lds[buf][row * K_PITCH];
+      __hip_bfloat16* vd = &v_lds[buf][row * V_PITCH];
+      if constexpr (FP8) {
+        u32x4 lo, hi;
+        widen(kr[j], e8m0_scale(ks[j]), lo, hi);
+        reinterpret_cast<u32x4*>(kd + tcol * 16)[0] = lo;
+        reinterpret_cast<u32x4*>(kd + tcol * 16)[1] = hi;
+        widen(vr[j], e8m0_scale(vs[j]), lo, hi);
+        if (gone) lo = hi = (u32x4){0, 0, 0, 0};
+        reinterpret_cast<u32x4*>(vd + tcol * 16)[0] = lo;
+        reinterpret_cast<u32x4*>(vd + tcol * 16)[1] = hi;
+      } else {
+        if (gone) vr[j] = (u32x4){0, 0, 0, 0};
+        reinterpret_cast<u32x4*>(kd + tcol * 8)[0] = kr[j];
+        reinterpret_cast<u32x4*>(vd + tcol * 8)[0] = vr[j];
+      }
+    }
+  };
+
+  bool ok = false;
+  if (pbegin < pend) {
+    ok = fetch(pbegin);
+    stage(0, pbegin);
+  }
+  for (int pi = pbegin; pi < pend; ++pi) {
+    __syncthreads();  // this page is staged; the other buffer is free
+    const int buf = (pi - pbegin) & 1;
+    const bool cur = ok;
+    if (pi + 1 < pend) ok = fetch(pi + 1);
+    if (wave_live && cur) {
+      const __hip_bfloat16* kt = &k_lds[buf][r32 * K_PITCH + h * 8];
+      const __hip_bfloat16* vt =
+          &v_lds[buf][(4 * h + ((lane & 15) >> 2)) * V_PITCH +
+                      ((lane >> 4) & 1) * 16 + (lane & 3) * 4];
+      f32x16 s[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[t][r] = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          s[t] = MFMA32(*reinterpret_cast<const bf16x8v*>(
+                            kt + t * 32 * K_PITCH + k * 16),
+                        qf[k], s[t]);
+      }
+      const int left = limit - pi * KVPAGE;  // this row's tokens of the page
+      float mt = -INFINITY;
+      if (__any(left < KVPAGE)) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (t * 32 + 8 * (r / 4) + 4 * h + r % 4 >= left)
+              s[t][r] = -INFINITY;
+            else
+              s[t][r] *= a.scale_log2;
+      } else {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) s[t] *= a.scale_log2;
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[t][r]);
+      mt = fmaxf(mt, __shfl_xor(mt, 32, WAVE));
+      const float mn = fmaxf(m, mt);
+      const float mu = (mn == -INFINITY) ? 0.f : mn;
+      if (__any(mn > m)) {  // a factor of 1 otherwise
+        const float keep = exp2_fast(m - mu);
+        l *= keep;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) o[d] *= keep;
+      }
+      m = mn;
+      bf16x8v pf[4];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float p = exp2_fast(s[t][r] - mu);
+          l += p;
+          pf[t * 2 + r / 8][r % 8] = (__bf16)p;
+        }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          const __hip_bfloat16* p = vt + u * 16 * V_PITCH + d * 32;
+          o[d] = MFMA32(join(read_tr(p), read_tr(p + 8 * V_PITCH)), pf[u], o[d]);
+        }
+    }
+    if (pi + 1 < pend) stage(buf ^ 1, pi + 1);
+  }
+
+  l += __shfl_xor(l, 32, WAVE);
+  if (!live) return;
+  const int64_t slot =
+      ((int64_t)b * a.hq + head) * (a.nshared + a.nsplit) + split;
+  if (h == 0) {
+    a.part_ml[slot * 2] = m;
+    a.part_ml[slot * 2 + 1] = l;
+  }
+#pragma unroll
+  for (int d = 0; d < 4; ++d)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      *reinterpret_cast<f32x4*>(
+          &a.part_o[slot * HD + d * 32 + r * 8 + h * 4]) =
+          (f32x4){o[d][r * 4], o[d][r * 4 + 1], o[d][r * 4 + 2],
+                  o[d][r * 4 + 3]};
+}
+
+#include <torch/extension.h>
+#include <ATen/hip/HIPContext.h>
+#include <c10/core/DeviceGuard.h>
+
+namespace {
+
+// Fills the arguments both entry points share, after checking them.
+Paged paged_args(const torch::Tensor& out, const torch::Tensor& q,
+                 const torch::Tensor& kcache, const torch::Tensor& vcache,
+                 const torch::Tensor& page_table,
+                 const torch::Tensor& seq_lens, double scale) {
+  const auto dev = q.device();
+  TORCH_CHECK(q.scalar_type() == torch::kBFloat16 && q.dim() == 3 &&
+                  q.size(2) == HD,
+              "q must be bf16 [B, hq, 128]");
+  const int64_t B = q.size(0), hq = q.size(1), hkv = kcache.size(1);
+  TORCH_CHECK(B == 0 || (q.stride(2) == 1 && (hq == 1 || q.stride(1) == HD)),
+              "q heads must be contiguous");
+  TORCH_CHECK((B <= 1 || q.stride(0) % 8 == 0) &&
+                  reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0,
+              "q rows must start on 16 bytes");
+  TORCH_CHECK(out.device() == dev && out.scalar_type() == torch::kBFloat16 &&
+                  out.sizes() == q.sizes() && out.is_contiguous(),
+              "out must be contiguous bf16 of q's shape");
+  TORCH_CHECK(hq % hkv == 0 && hq / hkv <= MAXG,
+              "hq must be a multiple of hkv, up to 16 times it");
+  TORCH_CHECK(page_table.device() == dev &&
+                  page_table.scalar_type() == torch::kInt32 &&
+                  page_table.dim() == 2 && page_table.size(0) == B &&
+                  page_table.is_contiguous(),
+              "page_table must be a contiguous int32 [B, max_pages]");
+  TORCH_CHECK(page_table.size(1) <= (1 << 24), "page_table is too wide");
+  TORCH_CHECK(seq_lens.device() == dev &&
+                  seq_lens.scalar_type() == torch::kInt32 &&
+                  seq_lens.dim() == 1 && seq_lens.size(0) == B &&
+                  seq_lens.is_contiguous(),
+              "seq_lens must be a contiguous int32 [B]");
+  TORCH_CHECK(hkv <= 65535, "too many KV heads");
+  Paged a{};
+  a.kcache = kcache.data_ptr();
+  a.vcache = vcache.data_ptr();
+  a.q = (const __hip_bfloat16*)q.data_ptr();
+  a.page_table = (const int32_t*)page_table.data_ptr();
+  a.seq_lens = (const int32_t*)seq_lens.data_ptr();
+  a.q_stride = B > 1 ? q.stride(0) : 0;
+  a.B = (int)B;
+  a.hq = (int)hq;
+  a.hkv = (int)hkv;
+  a.G = (int)(hq / hkv);
+  a.max_pages = (int)page_table.size(1);
+  a.num_pages = (int)kcache.size(0);
+  a.scale_log2 = (float)(scale * 1.4426950408889634);
+  return a;
+}
+
+// Blocks that fill the card's 256 CUs twice; a split has at least `least`
+// pages of the widest table row (the lengths themselves are on the device).
+int splits_for(int64_t blocks, int pages, int least) {
+  const int64_t want = (512 + blocks - 1) / std::max<int64_t>(blocks, 1);
+  return (int)std::max<int64_t>(
+      1, std::min<int64_t>({want, (pages + least - 1) / least, 128}));
+}
+
+template <bool FP8>
+void launch_decode(const Paged& a, torch::Tensor& out, hipStream_t s) {
+  const dim3 grid(a.B, a.hkv, a.nsplit);
+  hipLaunchKernelGGL((paged_decode_kernel<FP8, 4>), grid, dim3(4 * WAVE), 0, s,
+                     a, (__hip_bfloat16*)out.data_ptr());
+  if (a.nsplit > 1)
+    hipLaunchKernelGGL(paged_join_kernel,
+                       dim3((unsigned)(((int64_t)a.B * a.hq + 3) / 4)),
+                       dim3(4 * WAVE), 0, s, a,
+                       (__hip_bfloat16*)out.data_ptr());
+}
+
+// The partial slots: of this call alone (the allocator orders its reuse on
+// the stream, and a captured graph keeps its own).
+torch::Tensor partials(Paged& a, const torch::Tensor& q) {
+  const int64_t slots = a.nshared + a.nsplit;
+  if (slots == 1) return torch::Tensor();
+  const int64_t rows = (int64_t)a.B * a.hq * slots;
+  auto work = torch::empty({rows * (HD + 2)},
+                           q.options().dtype(torch::kFloat32));
+  a.part_o = (float*)work.data_ptr();
+  a.part_ml = a.part_o + rows * HD;
+  return work;
+}
+
+}  // namespace
+
+void attn_decode_fp8(torch::Tensor out, torch::Tensor q, torch::Tensor kcache,
+                     torch::Tensor vcache, torch::Tensor kscale,
+                     torch::Tensor vscale, torch::Tensor page_table,
+                     torch::Tensor seq_lens, double scale) {
+  const auto dev = q.device();
+  check_fp8_cache(kcache, vcache, kscale, vscale, dev);
+  Paged a = paged_args(out, q, kcache, vcache, page_table, seq_lens, scale);
+  if (a.B == 0) return;
+  a.kscale = (const uint8_t*)kscale.data_ptr();
+  a.vscale = (const uint8_t*)vscale.data_ptr();
+  c10::DeviceGuard guard(dev);
+  a.nsplit = splits_for((int64_t)a.B * a.hkv, a.max_pages, 4);
+  const auto work = partials(a, q);
+  launch_decode<true>(a, out, at::hip::getCurrentHIPStream().stream());
+  HIP_CHECK_LAST();
+}
+
+void attn_decode_shared(torch::Tensor out, torch::Tensor q,
+                        torch::Tensor kcache, torch::Tensor vcache,
+                        torch::Tensor page_table, torch::Tensor seq_lens,
+                        torch::Tensor group, torch::Tensor group_lens,
+                        double scale, c10::optional<torch::Tensor> kscale,
+                        c10::optional<torch::Tensor> vscale) {
+  const auto dev = q.device();
+  TORCH_CHECK(kscale.has_value() == vscale.has_value(),
+              "kscale and vscale come together");
+  const bool fp8 = kscale.has_value();
+  if (fp8) {
+    check_fp8_cache(kcache, vcache, *kscale, *vscale, dev);
+  } else {
+    for (const auto* c : {&kcache, &vcache}) {
+      TORCH_CHECK(c->device() == dev, "the cache is on another device");
+      TORCH_CHECK(c->scalar_type() == torch::kBFloat16,
+                  "a cache without scales must be bf16");
+      TORCH_CHECK(c->dim() == 4 && c->size(2) == KVPAGE && c->size(3) == HD &&
+                      c->size(1) > 0 && c->is_contiguous() &&
+                      c->sizes() == kcache.sizes(),
+                  "the caches must be contiguous [P, Hkv, 64, 128]");
+    }
+  }
+  Paged a = paged_args(out, q, kcache, vcache, page_table, seq_lens, scale);
+  TORCH_CHECK(group.device() == dev && group.scalar_type() == torch::kInt32 &&
+                  group.dim() == 1 && group.size(0) == a.B &&
+                  group.is_contiguous(),
+              "group must be a contiguous int32 [B]");
+  TORCH_CHECK(group_lens.device() == dev &&
+                  group_lens.scalar_type() == torch::kInt32 &&
+                  group_lens.dim() == 1 && group_lens.is_contiguous(),
+              "group_lens must be a contiguous int32 [groups]");
+  TORCH_CHECK(group_lens.size(0) <= MAXGROUPS, "at most 64 prefix groups");
+  if (a.B == 0) return;
+  if (fp8) {
+    a.kscale = (const uint8_t*)kscale->data_ptr();
+    a.vscale = (const uint8_t*)vscale->data_ptr();
+  }
+  a.ngroups = (int)group_lens.size(0);
+  c10::DeviceGuard guard(dev);
+  hipStream_t s = at::hip::getCurrentHIPStream().stream();
+  a.nsplit = splits_for((int64_t)a.B * a.hkv, a.max_pages, 4);
+  if (a.ngroups > 0) {
+    a.group = (const int32_t*)group.data_ptr();
+    a.group_lens = (const int32_t*)group_lens.data_ptr();
+    const int per_tile = 128 / a.G;
+    const int full = (a.B + per_tile - 1) / per_tile;
+    a.nshared = splits_for((int64_t)full * a.hkv, a.max_pages, 2);
+    const auto work = partials(a, q);
+    // each group may leave one tile part full; no more tiles than rows
+    const dim3 grid(a.hkv, a.nshared,
+                    std::min<int>(a.B, full + a.ngroups));
+    if (fp8)
+      hipLaunchKernelGGL((paged_shared_kernel<true>), grid, dim3(4 * WAVE), 0,
+                         s, a);
+    else
+      hipLaunchKernelGGL((paged_shared_kernel<false>), grid, dim3(4 * WAVE), 0,
+                         s, a);
+    if (fp8)
+      launch_decode<true>(a, out, s);
+    else
+      launch_decode<false>(a, out, s);
+  } else {
+    const auto work = partials(a, q);
+    if (fp8)
+      launch_decode<true>(a, out, s);
+    else
+      launch_decode<false>(a, out, s);
+  }
+  HIP_CHECK_LAST();
+}

@@ -33,6 +33,34 @@ void attn_prefill_varlen(torch::Tensor out, torch::Tensor q, torch::Tensor k,
                          torch::Tensor v, torch::Tensor block_map,
                          torch::Tensor q_starts, torch::Tensor kv_starts,
                          torch::Tensor past_lens, double scale);
+void rope_qkv_write_fp8(torch::Tensor qkv, torch::Tensor kcache,
+                        torch::Tensor vcache, torch::Tensor kscale,
+                        torch::Tensor vscale, torch::Tensor cos_sin,
+                        torch::Tensor positions, torch::Tensor slots,
+                        int64_t hq, int64_t hkv,
+                        c10::optional<torch::Tensor> q_out);
+void rope_qkv_write_slab_fp8(torch::Tensor qkv, torch::Tensor work,
+                             torch::Tensor kcache, torch::Tensor vcache,
+                             torch::Tensor kscale, torch::Tensor vscale,
+                             torch::Tensor cos_sin, torch::Tensor positions,
+                             torch::Tensor slots, int64_t hq, int64_t hkv,
+                             int64_t Mp, int64_t splitk);
+void kv_write_fp8(torch::Tensor kcache, torch::Tensor vcache,
+                  torch::Tensor kscale, torch::Tensor vscale, torch::Tensor k,
+                  torch::Tensor v, torch::Tensor slots);
+void kv_read_fp8(torch::Tensor k, torch::Tensor v, torch::Tensor kcache,
+                 torch::Tensor vcache, torch::Tensor kscale,
+                 torch::Tensor vscale, torch::Tensor slots);
+void attn_decode_fp8(torch::Tensor out, torch::Tensor q, torch::Tensor kcache,
+                     torch::Tensor vcache, torch::Tensor kscale,
+                     torch::Tensor vscale, torch::Tensor page_table,
+                     torch::Tensor seq_lens, double scale);
+void attn_decode_shared(torch::Tensor out, torch::Tensor q,
+                        torch::Tensor kcache, torch::Tensor vcache,
+                        torch::Tensor page_table, torch::Tensor seq_lens,
+                        torch::Tensor group, torch::Tensor group_lens,
+                        double scale, c10::optional<torch::Tensor> kscale,
+                        c10::optional<torch::Tensor> vscale);
 void sample(torch::Tensor out, torch::Tensor logits, torch::Tensor temperature,
             torch::Tensor seed_step, torch::Tensor topk, torch::Tensor cand,
             torch::Tensor row_seeds);
@@ -83,6 +111,18 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("attn_prefill", &attn_prefill, "causal GQA prefill attention (MFMA)");
   m.def("attn_prefill_varlen", &attn_prefill_varlen,
         "packed varlen causal GQA prefill attention (MFMA)");
+  m.def("rope_qkv_write_fp8", &rope_qkv_write_fp8,
+        "fused QKV epilogue: RoPE + e4m3 quantised paged-cache write");
+  m.def("rope_qkv_write_slab_fp8", &rope_qkv_write_slab_fp8,
+        "split-K reduce + RoPE + e4m3 quantised cache write in one launch");
+  m.def("kv_write_fp8", &kv_write_fp8,
+        "quantise K/V rows into the e4m3 paged cache");
+  m.def("kv_read_fp8", &kv_read_fp8,
+        "read rows of the e4m3 paged cache back as bf16");
+  m.def("attn_decode_fp8", &attn_decode_fp8,
+        "paged GQA decode attention over the e4m3 cache");
+  m.def("attn_decode_shared", &attn_decode_shared,
+        "paged GQA decode attention, shared prefixes computed once");
   m.def("sample", &sample, "Gumbel-max token sampling");
   m.def("skinny_gemm", &skinny_gemm,
         "decode projection GEMM: out = x @ w^T, w stored [N,K]");

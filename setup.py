@@ -22,6 +22,8 @@ sources = [
     os.path.join(CSRC, "elementwise.hip"),
     os.path.join(CSRC, "attn_decode.hip"),
     os.path.join(CSRC, "attn_prefill.hip"),
+    os.path.join(CSRC, "attn_paged.hip"),
+    os.path.join(CSRC, "kv_fp8.hip"),
     os.path.join(CSRC, "sampling.hip"),
     os.path.join(CSRC, "skinny_gemm.hip"),
     os.path.join(CSRC, "tile_gemm.hip"),

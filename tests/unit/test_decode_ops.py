@@ -1,0 +1,548 @@
+"""The quantised cache and the attention over it: kernels against 64-bit
+formulas, on the GPU and (the reference implementations) on the CPU.
+
+Tolerances are derived beside each check.  A rounding to bf16 is off by at
+most 2^-8 of the value, one to e4m3 by 2^-4, one to fp32 by 2^-24.
+"""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from calfkit_amd import ops
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+HD, PAGE = 128, 64
+
+
+def _two_to(e: torch.Tensor) -> torch.Tensor:
+    """2^e in 64 bits."""
+    return ((e.long() + 1023) << 52).view(torch.float64)
+
+
+def _quantised64(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """The values an e4m3 row with a power-of-two scale holds, and the scale
+    byte, from the format's definition in 64 bits (finite rows)."""
+    x = x.double().cpu()
+    a = x.abs().amax(-1, keepdim=True)
+    e = torch.full_like(a, -127)
+    for lift in (128, 64, 32, 16, 8, 4, 2, 1):
+        e = torch.where(a > 448.0 * _two_to(e + lift - 1), e + lift, e)
+    e = torch.where(a > 0, e, 0.0)
+    y = x * _two_to(-e)
+    octave = torch.frexp(y.abs().clamp_min(2.0 ** -6))[1] - 1
+    y = torch.round(y * _two_to(3 - octave)) * _two_to(octave - 3)
+    return y * _two_to(e), (e.squeeze(-1) + 127).to(torch.uint8)
+
+
+def _empty_cache(pages: int, hkv: int, device: str):
+    def codes():
+        return torch.zeros(pages, hkv, PAGE, HD, dtype=torch.uint8,
+                           device=device).view(torch.float8_e4m3fn)
+
+    def scales():
+        return torch.full((pages, hkv, PAGE), 7, dtype=torch.uint8,
+                          device=device)
+
+    return codes(), codes(), scales(), scales()
+
+
+def _values(cache: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+    """[P, hkv, PAGE, HD] in 64 bits, on the CPU."""
+    return (cache.cpu().float().double()
+            * _two_to(scale.cpu().int() - 127).unsqueeze(-1))
+
+
+# ------------------------------------------------------------- e4m3 cache
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("T,hkv", [(1, 1), (1, 8), (7, 2), (65, 8), (300, 3)])
+def test_kv_write_read_fp8(device, T, hkv):
+    """Every stored value is the definition's, and reads back as it is."""
+    g = torch.Generator().manual_seed(T * 31 + hkv)
+    spread = torch.exp2(torch.randint(-30, 30, (T, hkv, 1), generator=g).float())
+    rows = [(torch.randn(T, hkv, HD, generator=g) * spread).to(torch.bfloat16)
+            for _ in range(2)]
+    rows[0][0, 0] = 0.0                      # a row of zeros: scale 1
+    rows[1][0, 0] = 0.0
+    rows[1][0, 0, 5] = 448.0                 # the type's largest as it is
+    rows[1][-1, -1] = torch.linspace(-1, 1, HD) * 2.0 ** -120
+    if T > 2:
+        rows[0][1, 0, :4] = torch.tensor([464.0, 1.0, -0.0, 2.0 ** -12])
+        rows[0][2, 0] = 2.0 ** 119
+    # a strided k, as a view of the packed rows
+    packed = torch.zeros(T, 4 * hkv, HD, dtype=torch.bfloat16)
+    packed[:, hkv:2 * hkv] = rows[0]
+    k, v = packed.to(device)[:, hkv:2 * hkv], rows[1].to(device)
+    pages = T // PAGE + 2
+    kc, vc, ks, vs = _empty_cache(pages, hkv, device)
+    slots = torch.randperm(pages * PAGE, generator=g)[:T].to(torch.int32)
+    if T > 4:
+        slots[3] = -1                        # padding
+        slots[4] = pages * PAGE              # outside
+    ops.kv_write_fp8(kc, vc, ks, vs, k, v, slots.to(device))
+    keep = (slots >= 0) & (slots < pages * PAGE)
+    s = slots[keep].long()
+    for cache, scale, x in ((kc, ks, rows[0]), (vc, vs, rows[1])):
+        want, byte = _quantised64(x[keep])
+        assert torch.equal(scale.cpu()[s // PAGE, :, s % PAGE], byte)
+        assert torch.equal(_values(cache, scale)[s // PAGE, :, s % PAGE], want)
+        # what no slot names stays as it was
+        other = torch.ones(pages * PAGE, dtype=torch.bool)
+        other[s] = False
+        o = torch.nonzero(other).squeeze(1)
+        assert (scale.cpu()[o // PAGE, :, o % PAGE] == 7).all()
+        assert (cache.view(torch.uint8).cpu()[o // PAGE, :, o % PAGE] == 0).all()
+    back = [torch.full((T, hkv, HD), 3.0, dtype=torch.bfloat16, device=device)
+            for _ in range(2)]
+    ops.kv_read_fp8(*back, kc, vc, ks, vs, slots.to(device))
+    for x, b in zip(rows, back):
+        assert torch.equal(b.cpu().double()[keep], _quantised64(x[keep])[0])
+        assert (b.cpu()[~keep] == 3.0).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_kv_write_fp8_nonfinite(device):
+    """NaN and infinities become NaN and leave their row's scale alone."""
+    x = torch.randn(3, 1, HD).to(torch.bfloat16)
+    y = x.clone()
+    y[0, 0, 3], y[1, 0, 7], y[2, 0, 9] = math.nan, math.inf, -math.inf
+    for at in ((0, 3), (1, 7), (2, 9)):
+        x[at[0], 0, at[1]] = 0.0
+    kc, vc, ks, vs = _empty_cache(1, 1, device)
+    slots = torch.arange(3, dtype=torch.int32, device=device)
+    ops.kv_write_fp8(kc, vc, ks, vs, x.to(device), y.to(device), slots)
+    assert torch.equal(ks.cpu(), vs.cpu())
+    k, v = _values(kc, ks)[0, 0, :3], _values(vc, vs)[0, 0, :3]
+    bad = ~torch.isfinite(y[:, 0])
+    assert torch.isnan(v[bad]).all() and torch.equal(v[~bad], k[~bad])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("q_out", [False, True])
+@pytest.mark.parametrize("T,hq,hkv", [(1, 32, 8), (5, 2, 1), (130, 8, 2),
+                                      (33, 12, 3)])
+def test_rope_qkv_write_fp8(device, q_out, T, hq, hkv):
+    g = torch.Generator().manual_seed(T)
+    rows = torch.randn(T, (hq + 2 * hkv) * HD, generator=g).to(torch.bfloat16)
+    pos = torch.randint(0, 500, (T,), generator=g, dtype=torch.int32)
+    table = ops.build_rope_table(500, HD)
+    pages = T // PAGE + 1
+    slots = torch.randperm(pages * PAGE, generator=g)[:T].to(torch.int32)
+    if T > 1:
+        slots[1] = -1
+    kc, vc, ks, vs = _empty_cache(pages, hkv, device)
+    qkv = rows.clone().to(device)
+    q = torch.zeros(T, hq, HD, dtype=torch.bfloat16, device=device)
+    ops.rope_qkv_write_fp8(qkv, kc, vc, ks, vs, table.to(device),
+                           pos.to(device), slots.to(device), hq, hkv,
+                           q_out=q if q_out else None)
+    heads = rows.view(T, -1, HD).double()
+    cos, sin = table[pos.long()].double().unsqueeze(1).split(HD // 2, -1)
+    lo, hi = heads[:, :hq + hkv].split(HD // 2, -1)
+    want = torch.cat([lo * cos - hi * sin, hi * cos + lo * sin], -1)
+    # two products and their sum in fp32 (3 roundings of values up to
+    # |lo| + |hi|), one rounding to bf16
+    mag = torch.cat([lo.abs() + hi.abs()] * 2, -1)
+    tol = want.abs() * 2 ** -8 + mag * (3 * 2 ** -24)
+    got = qkv.cpu().view(T, -1, HD)
+    if q_out:
+        assert torch.equal(qkv.cpu(), rows)
+        turned_q = q.cpu()
+    else:
+        turned_q = got[:, :hq]
+        assert ((got[:, :hq + hkv].double() - want).abs() <= tol).all()
+        assert torch.equal(got[:, hq + hkv:], rows.view(T, -1, HD)[:, hq + hkv:])
+    assert ((turned_q.double() - want[:, :hq]).abs() <= tol[:, :hq]).all()
+    # the cache holds the packed row's own bf16 values, quantised
+    again = rows.clone().to(device)
+    ops.rope_qkv_write_fp8(again, *_empty_cache(pages, hkv, device),
+                           table.to(device), pos.to(device), slots.to(device),
+                           hq, hkv)
+    packed = again.cpu().view(T, -1, HD)
+    keep = slots >= 0
+    s = slots[keep].long()
+    for cache, scale, x in ((kc, ks, packed[:, hq:hq + hkv]),
+                            (vc, vs, packed[:, hq + hkv:])):
+        v, byte = _quantised64(x[keep])
+        assert torch.equal(_values(cache, scale)[s // PAGE, :, s % PAGE], v)
+        assert torch.equal(scale.cpu()[s // PAGE, :, s % PAGE], byte)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("splitk", [1, 4])
+def test_rope_qkv_write_slab_fp8(device, splitk):
+    T, Mp, hq, hkv = 19, 32, 8, 2
+    W = (hq + 2 * hkv) * HD
+    g = torch.Generator().manual_seed(splitk)
+    work = torch.randn(splitk * Mp * W, generator=g)
+    pos = torch.randint(0, 300, (T,), generator=g, dtype=torch.int32)
+    table = ops.build_rope_table(300, HD)
+    slots = torch.arange(T, dtype=torch.int32) * 3
+    slots[4] = -1
+    kc, vc, ks, vs = _empty_cache(1, hkv, device)
+    qkv = torch.full((T, W), 9.0, dtype=torch.bfloat16, device=device)
+    ops.rope_qkv_write_slab_fp8(qkv, work.to(device), kc, vc, ks, vs,
+                                table.to(device), pos.to(device),
+                                slots.to(device), hq, hkv, Mp, splitk)
+    slabs = work.view(splitk, Mp, -1, HD)[:, :T].double()
+    x, size = slabs.sum(0), slabs.abs().sum(0)
+    cos, sin = table[pos.long()].double().unsqueeze(1).split(HD // 2, -1)
+    lo, hi = x[:, :hq + hkv].split(HD // 2, -1)
+    want = x.clone()
+    want[:, :hq + hkv] = torch.cat([lo * cos - hi * sin, hi * cos + lo * sin], -1)
+    # splitk sums and 3 more roundings in fp32 of values up to size's pair,
+    # one rounding to bf16
+    pair = size[..., :64] + size[..., 64:]
+    tol = want.abs() * 2 ** -8 + torch.cat([pair, pair], -1) * (splitk + 3) * 2 ** -24
+    got = qkv.cpu().view(T, -1, HD)
+    assert ((got.double() - want).abs() <= tol).all()
+    keep = slots >= 0
+    s = slots[keep].long()
+    for cache, scale, part in ((kc, ks, got[:, hq:hq + hkv]),
+                               (vc, vs, got[:, hq + hkv:])):
+        assert torch.equal(_values(cache, scale)[0, :, s].transpose(0, 1),
+                           _quantised64(part[keep])[0])
+
+
+# -------------------------------------------------------------- attention
+
+def _batch(lens, hq, hkv, *, seed=0, fp8=True, pages=None, width=None):
+    """Caches, a shuffled page table and strided queries, on the CPU.  The
+    table's unused entries name no page; the cache beyond a row is NaN."""
+    g = torch.Generator().manual_seed(seed)
+    B = len(lens)
+    need = [(n + PAGE - 1) // PAGE for n in lens]
+    width = width or max(need + [1])
+    pages = pages or sum(need) + 2
+    order = torch.randperm(pages, generator=g).tolist()
+    table = torch.full((B, width), -1, dtype=torch.int32)
+    k = torch.randn(pages, hkv, PAGE, HD, generator=g)
+    v = torch.randn(pages, hkv, PAGE, HD, generator=g)
+    used = torch.zeros(pages, PAGE, dtype=torch.bool)
+    for b, n in enumerate(lens):
+        for i in range(need[b]):
+            p = order.pop()
+            table[b, i] = p
+            used[p, :min(PAGE, n - i * PAGE)] = True
+    k[~used.unsqueeze(1).expand(-1, hkv, -1)] = math.nan
+    v[~used.unsqueeze(1).expand(-1, hkv, -1)] = math.nan
+    k, v = k.to(torch.bfloat16), v.to(torch.bfloat16)
+    q = torch.randn(B, (hq + 2 * hkv) * HD, generator=g).to(torch.bfloat16)
+    q = q[:, :hq * HD].view(B, hq, HD)
+    s = dict(q=q, table=table, lens=torch.tensor(lens, dtype=torch.int32),
+             k=k, v=v, ks=None, vs=None)
+    if fp8:
+        s["k"], s["v"], s["ks"], s["vs"] = _empty_cache(pages, hkv, "cpu")
+        slots = torch.arange(pages * PAGE, dtype=torch.int32)
+        ops.kv_write_fp8(s["k"], s["v"], s["ks"], s["vs"],
+                         k.transpose(1, 2).reshape(-1, hkv, HD),
+                         v.transpose(1, 2).reshape(-1, hkv, HD), slots)
+    return s
+
+
+def _to(s, device):
+    out = {}
+    for name, t in s.items():
+        if t is None:
+            out[name] = None
+        elif name == "q":  # keep the packed rows' stride
+            B, hq, _ = t.shape
+            W = t.stride(0)
+            base = torch.zeros(B, W, dtype=t.dtype)
+            base[:, :hq * HD] = t.reshape(B, -1)
+            out[name] = base.to(device)[:, :hq * HD].view(B, hq, HD)
+        else:
+            out[name] = t.to(device)
+    return out
+
+
+def _expect(s, scale):
+    """out in 64 bits and how far a kernel may be from it.
+
+    Scores: 128 products in fp32, each sum's rounding at most 2^-24 of the
+    partial sums, so |ds| <= 2^-17 * scale * sum |q||k|, and the exponential
+    and the joins' factors 2^-20 more; a weight is off by twice that.  Weights
+    are rounded to bf16 (2^-8), sums of them and of their products in fp32.
+    The output is rounded once.
+    """
+    B, hq, _ = s["q"].shape
+    hkv = s["k"].shape[1]
+    if s["ks"] is None:
+        k, v = s["k"].double(), s["v"].double()
+    else:
+        k, v = _values(s["k"], s["ks"]), _values(s["v"], s["vs"])
+    out = torch.zeros(B, hq, HD, dtype=torch.float64)
+    tol = torch.zeros_like(out)
+    for b, n in enumerate(s["lens"].tolist()):
+        n = min(n, s["table"].shape[1] * PAGE)
+        if n <= 0:
+            continue
+        pages = s["table"][b, :(n + PAGE - 1) // PAGE].long()
+        kk, vv = (x[pages].permute(1, 0, 2, 3).reshape(hkv, -1, HD)[:, :n]
+                  for x in (k, v))
+        q = s["q"][b].double().view(hkv, -1, HD)
+        p = torch.softmax(q @ kk.transpose(1, 2) * scale, -1)
+        out[b] = (p @ vv).view(hq, HD)
+        ds = 2 ** -17 * abs(scale) * (q.abs() @ kk.abs().transpose(1, 2)).amax()
+        rel = 2 ** -8 + 2 * (ds + 2 ** -20) + n * 2 ** -24
+        tol[b] = 2 ** -8 * out[b].abs() + rel * (p @ vv.abs()).view(hq, HD)
+    return out, tol
+
+
+def _close(got, want, tol):
+    err = (got.cpu().double() - want).abs()
+    assert not torch.isnan(err).any()
+    assert (err <= tol).all(), float((err - tol).max())
+
+
+def _decode(s, scale=HD ** -0.5, device="cpu"):
+    d = _to(s, device)
+    out = torch.full(s["q"].shape, 5.0, dtype=torch.bfloat16, device=device)
+    ops.attn_decode_fp8(out, d["q"], d["k"], d["v"], d["ks"], d["vs"],
+                        d["table"], d["lens"], scale)
+    return out
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("hq,hkv", [(1, 1), (2, 1), (32, 8), (64, 8), (16, 1),
+                                    (9, 3)])
+@pytest.mark.parametrize("lens", [[1], [64], [65], [0, 1, 63, 128, 200]])
+def test_attn_decode_fp8(device, hq, hkv, lens):
+    s = _batch(lens, hq, hkv, seed=hq)
+    _close(_decode(s, device=device), *_expect(s, HD ** -0.5))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,n,hq,hkv", [(1, 5000, 32, 8), (3, 9001, 8, 8),
+                                        (40, 700, 32, 8), (300, 130, 8, 2)])
+def test_attn_decode_fp8_long_and_wide(B, n, hq, hkv):
+    """Split sequences, ragged lengths, a table wider than any row."""
+    rng = np.random.RandomState(B)
+    lens = [int(x) for x in rng.randint(0, n + 1, B)]
+    lens[0] = n
+    s = _batch(lens, hq, hkv, seed=B, width=n // PAGE + 9)
+    _close(_decode(s, device="cuda"), *_expect(s, HD ** -0.5))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_attn_decode_fp8_sharp_and_flat(device):
+    """Scores of hundreds (one weight is all) and a scale of 0 (all equal)."""
+    s = _batch([300, 77], 8, 2, seed=3)
+    s["q"] = s["q"] * 40
+    _close(_decode(s, 1.0, device=device), *_expect(s, 1.0))
+    _close(_decode(s, 0.0, device=device), *_expect(s, 0.0))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_attn_decode_fp8_lengths_and_pages_out_of_range(device):
+    """Lengths are taken to the table's width, negative ones are 0, and a page
+    id outside the cache counts as a page without tokens."""
+    s = _batch([128, 128, 100], 4, 2, seed=4)
+    want, tol = _expect(s, HD ** -0.5)
+    s["lens"] = torch.tensor([4000, 128, -3], dtype=torch.int32)
+    want[2], tol[2] = 0.0, 0.0
+    _close(_decode(s, device=device), want, tol)
+    full = dict(s, lens=torch.tensor([64, 128, 0], dtype=torch.int32))
+    want, tol = _expect(full, HD ** -0.5)
+    s["table"][0, 1] = s["k"].shape[0]
+    s["table"][1] = torch.tensor([-7, 1 << 30])
+    want[1], tol[1] = 0.0, 0.0
+    _close(_decode(s, device=device), want, tol)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_attn_decode_fp8_nan_row_stays_its_own(device):
+    """A NaN key inside a row shows in that row and head alone."""
+    s = _batch([70, 70], 4, 2, seed=5)
+    want, tol = _expect(s, HD ** -0.5)
+    page = int(s["table"][0, 1])
+    s["k"].view(torch.uint8)[page, 1, 2, 9] = 0x7F
+    got = _decode(s, device=device).cpu()
+    assert torch.isnan(got[0, 2:]).all()
+    got[0, 2:] = 0
+    want[0, 2:], tol[0, 2:] = 0, 0
+    _close(got, want, tol)
+
+
+# --------------------------------------------------------- shared prefixes
+
+def _shared_batch(groups, prefixes, tails, hq, hkv, *, seed=0, fp8=False):
+    """Rows of group g share their first prefixes[g] tokens' pages."""
+    B = len(groups)
+    lens = [(prefixes[g] if g >= 0 else 0) + t for g, t in zip(groups, tails)]
+    s = _batch(lens, hq, hkv, seed=seed, fp8=fp8)
+    first = {}
+    for b, g in enumerate(groups):
+        if g < 0:
+            continue
+        lead = first.setdefault(g, b)
+        # a row may be shorter than its prefix's last page: whole pages only
+        n = prefixes[g] // PAGE
+        s["table"][b, :n] = s["table"][lead, :n]
+    s["group"] = torch.tensor(groups, dtype=torch.int32)
+    s["glens"] = torch.tensor([p // PAGE * PAGE for p in prefixes],
+                              dtype=torch.int32)
+    return s
+
+
+def _shared(s, device="cpu", scale=HD ** -0.5):
+    d = _to(s, device)
+    out = torch.full(s["q"].shape, 5.0, dtype=torch.bfloat16, device=device)
+    ops.attn_decode_shared(out, d["q"], d["k"], d["v"], d["table"], d["lens"],
+                           d["group"], d["glens"], scale, kscale=d["ks"],
+                           vscale=d["vs"])
+    return out
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("hq,hkv", [(2, 1), (32, 8), (16, 1), (3, 3), (6, 2)])
+def test_attn_decode_shared(device, fp8, hq, hkv):
+    """Three interleaved groups, rows without one, tails of 0 and 1."""
+    groups = [0, 1, -1, 0, 2, 0, 1, -1, 2]
+    tails = [1, 70, 30, 0, 64, 63, 5, 0, 129]
+    s = _shared_batch(groups, [64, 192, 320], tails, hq, hkv, seed=hq, fp8=fp8)
+    _close(_shared(s, device), *_expect(s, HD ** -0.5))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("B,ngroups,pages,hq,hkv", [
+    (2, 1, 40, 32, 8), (100, 1, 9, 32, 8), (150, 64, 2, 8, 2),
+    (70, 3, 17, 64, 8), (300, 5, 3, 2, 1)])
+def test_attn_decode_shared_many(fp8, B, ngroups, pages, hq, hkv):
+    """Tiles part full, split prefixes, as many groups as a call takes."""
+    rng = np.random.RandomState(B)
+    groups = [int(x) for x in rng.randint(-1, ngroups, B)]
+    groups[0] = 0
+    prefixes = [int(x) * PAGE for x in rng.randint(0, pages + 1, ngroups)]
+    prefixes[0] = pages * PAGE
+    tails = [int(x) for x in rng.randint(0, 150, B)]
+    s = _shared_batch(groups, prefixes, tails, hq, hkv, seed=B, fp8=fp8)
+    _close(_shared(s, "cuda"), *_expect(s, HD ** -0.5))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("fp8", [False, True])
+def test_attn_decode_shared_any_prefix_length(device, fp8):
+    """A prefix that ends inside a page, a row shorter than its prefix, a group
+    id without a group, no groups at all: the result is the plain one."""
+    s = _shared_batch([0, 0, 0, 1], [192, 64], [9, 40, 77, 3], 8, 2, fp8=fp8)
+    s["lens"][1] = 150
+    want = _expect(s, HD ** -0.5)
+    for glens in ([100, 1], [192, 64], [0, 64], [191, -5], [1 << 30, 0]):
+        if glens[0] > 192:     # a prefix past the rows' own: not common pages
+            s["group"] = torch.tensor([0, -1, -1, -1], dtype=torch.int32)
+        s["glens"] = torch.tensor(glens, dtype=torch.int32)
+        _close(_shared(s, device), *want)
+    s["group"] = torch.tensor([2, 77, -9, 1 << 30], dtype=torch.int32)
+    _close(_shared(s, device), *want)
+    s["glens"] = torch.zeros(0, dtype=torch.int32)
+    _close(_shared(s, device), *want)
+
+
+def test_build_prefix_groups():
+    table = np.array([[3, 4, 5, 6], [3, 4, 9, 0], [8, 1, 2, 0], [3, 4, 5, 7],
+                      [8, 1, 2, 0], [11, 0, 0, 0], [3, 0, 0, 0]], np.int32)
+    lens = np.array([250, 190, 192, 256, 130, 64, 63])
+    group, glens = ops.build_prefix_groups(table, lens, max_groups=4)
+    # rows 0, 1, 3 share pages 3, 4; rows 2, 4 share 8, 1 (row 4 has but two
+    # whole pages); row 5 is alone and row 6 has no whole page
+    a, b = group[0], group[2]
+    assert a >= 0 and b >= 0 and a != b
+    assert group.tolist() == [a, a, b, a, b, -1, -1]
+    assert glens[a] == 128 and glens[b] == 128
+    one, lens1 = ops.build_prefix_groups(table, lens, max_groups=1)
+    assert one.tolist() == [0, 0, -1, 0, -1, -1, -1] and lens1.tolist() == [128]
+    none, _ = ops.build_prefix_groups(table, lens, min_rows=4)
+    assert (none == -1).all()
+    none, _ = ops.build_prefix_groups(table[:0], lens[:0])
+    assert none.shape == (0,)
+
+
+# --------------------------------------------------------------- refusals
+
+def _refusal_args(device):
+    s = _to(_batch([70, 5], 4, 2, seed=1), device)
+    qkv = torch.zeros(2, 8 * HD, dtype=torch.bfloat16, device=device)
+    i32 = torch.zeros(2, dtype=torch.int32, device=device)
+    rows = torch.zeros(2, 2, HD, dtype=torch.bfloat16, device=device)
+    table = ops.build_rope_table(8, HD, device=device)
+    cache = (s["k"], s["v"], s["ks"], s["vs"])
+    out = torch.zeros(2, 4, HD, dtype=torch.bfloat16, device=device)
+    return s, cache, qkv, i32, rows, table, out
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_refusals(device):
+    s, cache, qkv, i32, rows, table, out = _refusal_args(device)
+    kc, vc, ks, vs = cache
+
+    def refused(call, *args, **kw):
+        with pytest.raises(RuntimeError):
+            call(*args, **kw)
+
+    bf16 = torch.zeros(kc.shape, dtype=torch.bfloat16, device=device)
+    w, r = ops.kv_write_fp8, ops.kv_read_fp8
+    refused(w, bf16, vc, ks, vs, rows, rows, i32)
+    refused(w, kc[:, :1], vc, ks, vs, rows, rows, i32)
+    refused(w, kc, vc, ks[:1], vs, rows, rows, i32)
+    refused(w, kc, vc, ks.int(), vs, rows, rows, i32)
+    refused(w, kc, vc, ks, vs, rows.float(), rows, i32)
+    refused(w, kc, vc, ks, vs, rows[:, :1], rows, i32)
+    refused(w, kc, vc, ks, vs, rows, rows, i32.long())
+    refused(w, kc, vc, ks, vs, rows, rows, i32[:1])
+    refused(w, kc, vc, ks, vs, rows.transpose(1, 2).contiguous()
+            .transpose(1, 2), rows, i32)
+    refused(r, rows, rows, kc, vc, ks, vs, i32[:1])
+    refused(r, rows, rows[..., :64], kc, vc, ks, vs, i32)
+    rope = ops.rope_qkv_write_fp8
+    refused(rope, qkv, kc, vc, ks, vs, table, i32, i32, 5, 2)
+    refused(rope, qkv, kc, vc, ks, vs, table, i32, i32, 6, 1)
+    refused(rope, qkv.float(), kc, vc, ks, vs, table, i32, i32, 4, 2)
+    refused(rope, qkv, kc, vc, ks, vs, table[:, :64], i32, i32, 4, 2)
+    refused(rope, qkv, kc, vc, ks, vs, table, i32.long(), i32, 4, 2)
+    refused(rope, qkv, kc, vc, ks, vs, table, i32, i32, 4, 2, q_out=out.float())
+    refused(ops.rope_qkv_write_slab_fp8, qkv,
+            torch.zeros(8 * HD * 2, device=device), kc, vc, ks, vs, table,
+            i32, i32, 4, 2, 2, 2)
+    dec = ops.attn_decode_fp8
+    q, t, n = s["q"], s["table"], s["lens"]
+    refused(dec, out, q.float(), kc, vc, ks, vs, t, n, 1.0)
+    refused(dec, out[:1], q, kc, vc, ks, vs, t, n, 1.0)
+    refused(dec, out, q, bf16, bf16, ks, vs, t, n, 1.0)
+    refused(dec, out, q, kc, vc, ks, vs, t.long(), n, 1.0)
+    refused(dec, out, q, kc, vc, ks, vs, t[:1], n, 1.0)
+    refused(dec, out, q, kc, vc, ks, vs, t, n.long(), 1.0)
+    refused(dec, out[:, :3].contiguous(), q[:, :3], kc, vc, ks, vs, t, n, 1.0)
+    wide = torch.zeros(2, 34, HD, dtype=torch.bfloat16, device=device)
+    refused(dec, wide, wide, kc, vc, ks, vs, t, n, 1.0)
+    sh = ops.attn_decode_shared
+    g, gl = i32, i32[:1]
+    refused(sh, out, q, kc, vc, t, n, g, gl, 1.0)            # e4m3, no scales
+    refused(sh, out, q, bf16, bf16, t, n, g, gl, 1.0, kscale=ks)
+    refused(sh, out, q, bf16, bf16, t, n, g, gl, 1.0, kscale=ks, vscale=vs)
+    refused(sh, out, q, bf16, bf16, t, n, g[:1], gl, 1.0)
+    refused(sh, out, q, bf16, bf16, t, n, g, gl.long(), 1.0)
+    refused(sh, out, q, bf16, bf16, t, n, g,
+            torch.zeros(65, dtype=torch.int32, device=device), 1.0)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_empty_batches(device):
+    s, cache, qkv, i32, rows, table, out = _refusal_args(device)
+    kc, vc, ks, vs = cache
+    before = kc.view(torch.uint8).clone()
+    ops.kv_write_fp8(kc, vc, ks, vs, rows[:0], rows[:0], i32[:0])
+    ops.kv_read_fp8(rows[:0], rows[:0], kc, vc, ks, vs, i32[:0])
+    ops.rope_qkv_write_fp8(qkv[:0], kc, vc, ks, vs, table, i32[:0], i32[:0],
+                           4, 2)
+    assert torch.equal(kc.view(torch.uint8), before)
+    ops.attn_decode_fp8(out[:0], s["q"][:0], kc, vc, ks, vs, s["table"][:0],
+                        s["lens"][:0], 1.0)
+    ops.attn_decode_shared(out[:0], s["q"][:0], kc, vc, s["table"][:0],
+                           s["lens"][:0], i32[:0], i32[:1], 1.0, kscale=ks,
+                           vscale=vs)
