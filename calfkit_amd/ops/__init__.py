@@ -35,6 +35,7 @@ __all__ = [
     "attn_prefill_varlen",
     "build_prefill_blocks",
     "sample",
+    "sample_filtered",
     "skinny_gemm",
     "skinny_gemm_slabs",
     "tile_gemm",
@@ -696,6 +697,77 @@ def sample(out: torch.Tensor, logits: torch.Tensor, temperature: torch.Tensor,
             u = torch.rand(V, generator=gen).clamp_min(1e-12)
             g = -torch.log(-torch.log(u))
             out[b] = int((lg[b] / t + g).argmax())
+
+
+def sample_filtered(out: torch.Tensor, logits: torch.Tensor,
+                    temperature: torch.Tensor, top_k: torch.Tensor,
+                    top_p: torch.Tensor, min_p: torch.Tensor,
+                    uniform: torch.Tensor,
+                    kept: torch.Tensor | None = None) -> None:
+    """Draw tokens under temperature, top-k, top-p and min-p from one given
+    random number a row.  out [B] i32; logits [B, V] bf16 or f32, not changed.
+
+    The candidates (every entry but NaN and -inf) stand in order of falling
+    logit, ties by lowest index, each with weight exp((x - max) / T).  Kept is
+    the shortest of three prefixes of that order: the first ``top_k`` (0 or
+    less: all); those whose sum of weights before them is less than ``top_p``
+    of the first's whole sum (1 or more: all); those whose weight is at least
+    ``min_p`` (0 or less: all); never less than one.  The token is the first
+    whose sum up to and with it passes ``uniform`` (in [0, 1)) times the kept
+    sum.  Sums are taken in 64 bits, so the token is the formula's.
+
+    A temperature that is not above 0 takes the largest logit.  A row without
+    candidates gives token 0.  A row with a negative random number is not
+    drawn: its out and kept stay as they were.  ``kept`` [B] i32 receives the
+    number of candidates kept.
+    """
+    if _native(logits):
+        _K.sample_filtered(out, logits, temperature, top_k, top_p, min_p,
+                           uniform, kept)
+        return
+    _require(logits.dim() == 2 and logits.is_contiguous()
+             and logits.dtype in (torch.bfloat16, torch.float32),
+             "logits must be a contiguous bf16 or f32 [B, V]")
+    B, V = logits.shape
+    _require(1 <= V <= 1 << 20, "V must be from 1 to 2^20")
+    for t, name, dtype in ((out, "out", torch.int32),
+                           (temperature, "temperature", torch.float32),
+                           (top_k, "top_k", torch.int32),
+                           (top_p, "top_p", torch.float32),
+                           (min_p, "min_p", torch.float32),
+                           (uniform, "uniform", torch.float32),
+                           (kept, "kept", torch.int32)):
+        if t is None and name == "kept":
+            continue
+        _require(t.dtype == dtype and t.shape == (B,) and t.is_contiguous(),
+                 f"{name} must be a contiguous {dtype} [B]")
+    for b in range(B):
+        u = float(uniform[b])
+        if u < 0:
+            continue
+        x = logits[b].double() + 0.0
+        x = torch.where(torch.isnan(x), float("-inf"), x)
+        x, ids = torch.sort(x, descending=True, stable=True)
+        x = x[x > float("-inf")]
+        T = float(temperature[b])
+        if x.numel() == 0 or not T > 0:
+            out[b] = ids[0]
+            if kept is not None:
+                kept[b] = 1
+            continue
+        w = torch.where(x == x[0], 1.0, torch.exp((x - x[0]) / T))
+        cum = w.cumsum(0)
+        k = int(top_k[b])
+        n = min(k if 0 < k < V else V, x.numel())
+        if float(top_p[b]) < 1:
+            goal = float(top_p[b]) * float(cum[n - 1])
+            n = min(n, int(((cum - w) < goal).sum()))
+        n = min(n, int((w >= float(min_p[b])).sum()))
+        n = max(n, 1)
+        r = int((cum <= min(u, 1 - 2.0 ** -53) * float(cum[n - 1])).sum())
+        out[b] = ids[min(r, n - 1)]
+        if kept is not None:
+            kept[b] = n
 
 
 # ----------------------------------------------------- tool-call grammar

@@ -64,6 +64,11 @@ void attn_decode_shared(torch::Tensor out, torch::Tensor q,
 void sample(torch::Tensor out, torch::Tensor logits, torch::Tensor temperature,
             torch::Tensor seed_step, torch::Tensor topk, torch::Tensor cand,
             torch::Tensor row_seeds);
+void sample_filtered(torch::Tensor out, torch::Tensor logits,
+                     torch::Tensor temperature, torch::Tensor top_k,
+                     torch::Tensor top_p, torch::Tensor min_p,
+                     torch::Tensor uniform,
+                     c10::optional<torch::Tensor> kept);
 void skinny_gemm(torch::Tensor out, torch::Tensor x, torch::Tensor w,
                  torch::Tensor work, int64_t splitk);
 void skinny_gemm_silu(torch::Tensor out, torch::Tensor x, torch::Tensor w,
@@ -124,6 +129,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("attn_decode_shared", &attn_decode_shared,
         "paged GQA decode attention, shared prefixes computed once");
   m.def("sample", &sample, "Gumbel-max token sampling");
+  m.def("sample_filtered", &sample_filtered,
+        "temperature, top-k, top-p and min-p draw from given random numbers");
   m.def("skinny_gemm", &skinny_gemm,
         "decode projection GEMM: out = x @ w^T, w stored [N,K]");
   m.def("skinny_gemm_silu", &skinny_gemm_silu,

@@ -25,6 +25,7 @@ sources = [
     os.path.join(CSRC, "attn_paged.hip"),
     os.path.join(CSRC, "kv_fp8.hip"),
     os.path.join(CSRC, "sampling.hip"),
+    os.path.join(CSRC, "sample_filtered.hip"),
     os.path.join(CSRC, "skinny_gemm.hip"),
     os.path.join(CSRC, "tile_gemm.hip"),
     os.path.join(CSRC, "moe_gemm.hip"),
