@@ -131,7 +131,7 @@ class LlamaShard:
         self.rope = ops.build_rope_table(cfg.max_seq + MAX_RUN_OVERSHOOT,
                                          self.dh, cfg.rope_theta,
                                          device=self.device)
-        self._splitk_cache: dict[int, int] = {}
+        self._splitk_cache: dict[tuple, int] = {}
         #: comm stream for the TP-overlap decode pipeline (north star:
         #: "RCCL all-reduce over xGMI overlapped with the GEMMs")
         self._comm_stream = (torch.cuda.Stream(device=self.device)
@@ -202,7 +202,9 @@ class LlamaShard:
         return ops.small_plan(T, n_out, k_in)
 
     def _splitk_for(self, weight: torch.Tensor, m: int = 32) -> int:
-        key = (weight.shape[0], m > 64)
+        # both sizes: o and down share their rows but not their K, and a split
+        # that does not divide K reads past the rows' ends
+        key = (*weight.shape, m > 64)
         sk = self._splitk_cache.get(key)
         if sk is None:
             sk = ops.choose_splitk(weight.shape[0], weight.shape[1], m)

@@ -349,6 +349,14 @@ static int pad_m(int M) {
   return 256;
 }
 
+// Each wave's (M <= 64) or block's slice of K has to be whole k-steps: the
+// kernels read whole steps, past the rows' ends otherwise.
+static void check_split(int64_t K, int64_t splitk, int Mp) {
+  const int64_t part = Mp > 64 ? splitk * 64 : splitk * SGWAVES * 32;
+  TORCH_CHECK(splitk >= 1 && K % part == 0, "K must split evenly: K=", K,
+              " splitk=", splitk);
+}
+
 void skinny_gemm(torch::Tensor out, torch::Tensor x, torch::Tensor w,
                  torch::Tensor work, int64_t splitk) {
   // out[M,N] = x[M,K] @ w[N,K]^T ; work: fp32 scratch >= splitk*Mp*N
@@ -379,6 +387,7 @@ void skinny_gemm_slabs(torch::Tensor x, torch::Tensor w, torch::Tensor work,
   // slab-only launch: the consumer kernel fuses the split-K reduce
   const int M = x.size(0), N = w.size(0);
   const int Mp = pad_m(M);
+  check_split(x.size(1), splitk, Mp);
   TORCH_CHECK(work.numel() >= splitk * (int64_t)Mp * N, "workspace too small");
   hipStream_t s = at::hip::getCurrentHIPStream().stream();
   auto dummy_out = work;  // unused when direct=0
@@ -395,6 +404,7 @@ void skinny_gemm_silu(torch::Tensor out, torch::Tensor x, torch::Tensor w,
   const int M = x.size(0), K = x.size(1), N = w.size(0);
   const int F = N / 2;
   const int Mp = pad_m(M);
+  check_split(K, splitk, Mp);
   TORCH_CHECK(out.size(1) == F);
   TORCH_CHECK(work.numel() >= splitk * (int64_t)Mp * N, "workspace too small");
   hipStream_t s = at::hip::getCurrentHIPStream().stream();
