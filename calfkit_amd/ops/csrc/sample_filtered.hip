@@ -37,7 +37,7 @@ using u32x4 = __attribute__((ext_vector_type(4))) unsigned;
 
 constexpr int BLOCK = 1024;
 constexpr int NWAVES = BLOCK / WAVE;
-constexpr int MAXCHUNKS = 512;  // 16 B loads of a thread: up to 2^20 entries
+constexpr int MAXCHUNKS = 129;  // of 8192 bf16 entries: up to 2^20
 constexpr int MAXV = 1 << 20;
 
 // bf16: magnitudes [2^-41, 2^23) are 64 octaves of 128 values, each sign
@@ -49,6 +49,26 @@ constexpr int DISTINCT = 4096;
 constexpr int BINS32 = 8192;
 constexpr int MEMBERS = 2048;
 constexpr double FIXED = 8796093022208.0;  // 2^43: 2^20 entries sum below 2^63
+
+// 2^(j / 64), rounded to 64 bits.
+__constant__ const double POW2_64TH[64] = {
+    0x1.0000000000000p+0, 0x1.02c9a3e778061p+0, 0x1.059b0d3158574p+0, 0x1.0874518759bc8p+0,
+    0x1.0b5586cf9890fp+0, 0x1.0e3ec32d3d1a2p+0, 0x1.11301d0125b51p+0, 0x1.1429aaea92de0p+0,
+    0x1.172b83c7d517bp+0, 0x1.1a35beb6fcb75p+0, 0x1.1d4873168b9aap+0, 0x1.2063b88628cd6p+0,
+    0x1.2387a6e756238p+0, 0x1.26b4565e27cddp+0, 0x1.29e9df51fdee1p+0, 0x1.2d285a6e4030bp+0,
+    0x1.306fe0a31b715p+0, 0x1.33c08b26416ffp+0, 0x1.371a7373aa9cbp+0, 0x1.3a7db34e59ff7p+0,
+    0x1.3dea64c123422p+0, 0x1.4160a21f72e2ap+0, 0x1.44e086061892dp+0, 0x1.486a2b5c13cd0p+0,
+    0x1.4bfdad5362a27p+0, 0x1.4f9b2769d2ca7p+0, 0x1.5342b569d4f82p+0, 0x1.56f4736b527dap+0,
+    0x1.5ab07dd485429p+0, 0x1.5e76f15ad2148p+0, 0x1.6247eb03a5585p+0, 0x1.6623882552225p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.6dfb23c651a2fp+0, 0x1.71f75e8ec5f74p+0, 0x1.75feb564267c9p+0,
+    0x1.7a11473eb0187p+0, 0x1.7e2f336cf4e62p+0, 0x1.82589994cce13p+0, 0x1.868d99b4492edp+0,
+    0x1.8ace5422aa0dbp+0, 0x1.8f1ae99157736p+0, 0x1.93737b0cdc5e5p+0, 0x1.97d829fde4e50p+0,
+    0x1.9c49182a3f090p+0, 0x1.a0c667b5de565p+0, 0x1.a5503b23e255dp+0, 0x1.a9e6b5579fdbfp+0,
+    0x1.ae89f995ad3adp+0, 0x1.b33a2b84f15fbp+0, 0x1.b7f76f2fb5e47p+0, 0x1.bcc1e904bc1d2p+0,
+    0x1.c199bdd85529cp+0, 0x1.c67f12e57d14bp+0, 0x1.cb720dcef9069p+0, 0x1.d072d4a07897cp+0,
+    0x1.d5818dcfba487p+0, 0x1.da9e603db3285p+0, 0x1.dfc97337b9b5fp+0, 0x1.e502ee78b3ff6p+0,
+    0x1.ea4afa2a490dap+0, 0x1.efa1bee615a27p+0, 0x1.f50765b6e4540p+0, 0x1.fa7c1819e90d8p+0,
+};
 
 struct Args {
   int32_t* out;
@@ -65,11 +85,12 @@ struct Args {
 // What every path is asked: the row's filters.
 struct Row {
   float m;        // largest logit
-  double T;       // temperature > 0
+  double T, inv_T;  // temperature > 0
   int k;          // top_k or V
   double top_p;   // >= 1: off
   double min_p;
   double u;
+  const double* pow2;  // POW2_64TH in LDS
 };
 
 // The token: an index, or (token < 0) the nth of the entries of value x.
@@ -91,8 +112,27 @@ __device__ __forceinline__ bool candidate(const float x) {
   return x > -INFINITY;  // false for NaN
 }
 
+// exp(z) for z <= 0, to a few units of the last bit: z = n ln2 / 64 + y with
+// |y| <= ln2 / 128, exp(y) by its series up to y^5 (the next term is below
+// 2^-54), 2^(n / 64) from the table (in LDS).  A dozen operations and seven
+// constants; the general exp() keeps twice as many registers busy.
+__device__ __forceinline__ double exp_neg(double z, const double* pow2) {
+  z = fmax(z, -800.0);
+  const double n = rint(z * 0x1.71547652b82fep+6);
+  double y = fma(n, -0x1.62e42fc000000p-7, z);
+  y = fma(n, -0x1.7d1cf79abc9e4p-34, y);
+  double p = fma(y, 1.0 / 120.0, 1.0 / 24.0);
+  p = fma(y, p, 1.0 / 6.0);
+  p = fma(y, p, 0.5);
+  p = fma(y, p, 1.0);
+  p = fma(y, p, 1.0);
+  const int i = (int)n;
+  return ldexp(p * pow2[i & 63], i >> 6);
+}
+
 __device__ __forceinline__ double weight(const float x, const Row& r) {
-  return x == r.m ? 1.0 : exp(((double)x - (double)r.m) / r.T);
+  return x == r.m ? 1.0
+                  : exp_neg(((double)x - (double)r.m) * r.inv_T, r.pow2);
 }
 
 // ---- block-wide sums and scans; `lds` holds NWAVES + 1 values
@@ -108,12 +148,12 @@ __device__ __forceinline__ S block_scan(S x, S* lds, S* total) {
   __syncthreads();  // the last user of lds is done
   if (lane == WAVE - 1) lds[wid] = incl;
   __syncthreads();
-  S before = 0, all = 0;
+  S all = lds[lane % NWAVES];
+  S before = lane % NWAVES < wid ? all : (S)0;
 #pragma unroll
-  for (int w = 0; w < NWAVES; ++w) {
-    const S y = lds[w];
-    if (w < wid) before += y;
-    all += y;
+  for (int off = NWAVES / 2; off > 0; off >>= 1) {
+    all += __shfl_xor(all, off, WAVE);
+    before += __shfl_xor(before, off, WAVE);
   }
   *total = all;
   return before + incl - x;
@@ -127,9 +167,10 @@ __device__ __forceinline__ S block_total(S x, S* lds) {
   __syncthreads();
   if (lane == 0) lds[wid] = x;
   __syncthreads();
-  S all = 0;
+  S all = lds[lane % NWAVES];
 #pragma unroll
-  for (int w = 0; w < NWAVES; ++w) all += lds[w];
+  for (int off = NWAVES / 2; off > 0; off >>= 1)
+    all += __shfl_xor(all, off, WAVE);
   return all;
 }
 
@@ -139,21 +180,50 @@ __device__ __forceinline__ float block_largest(float x, float* lds) {
   __syncthreads();
   if (lane == 0) lds[wid] = x;
   __syncthreads();
+  x = lds[lane % NWAVES];
 #pragma unroll
-  for (int w = 0; w < NWAVES; ++w) x = fmaxf(x, lds[w]);
+  for (int off = NWAVES / 2; off > 0; off >>= 1)
+    x = fmaxf(x, __shfl_xor(x, off, WAVE));
   return x;
 }
 
-// One row in chunks of BLOCK x 16 B: chunk c of thread t is the entries from
-// (c * BLOCK + t) * PER - lead on, so that every load is aligned whatever the
-// row's start; the first NC chunks stay in registers.  Entries outside the
-// row read as NaN, which is no candidate.
-template <typename T, int NC>
-struct Entries {
-  static constexpr int PER = 16 / sizeof(T);
+// One entry a thread at a time, read (from L2) in every pass.
+template <typename T>
+struct Plain {
   const T* row;
+  int V;
+  __device__ __forceinline__ float at(const int i) const {
+    if constexpr (sizeof(T) == 4)
+      return row[i] + 0.f;
+    else
+      return bf2f(row[i]) + 0.f;
+  }
+  // f(index, value) of every candidate, AHEAD loads in flight
+  template <int AHEAD, typename F>
+  __device__ __forceinline__ void each(F f) const {
+#pragma unroll 1
+    for (int i = threadIdx.x; i < V; i += BLOCK * AHEAD) {
+      float x[AHEAD];
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j)
+        x[j] = i + j * BLOCK < V ? at(i + j * BLOCK) : -INFINITY;
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j)
+        if (candidate(x[j])) f(i + j * BLOCK, x[j]);
+    }
+  }
+};
+
+// A bf16 row in chunks of BLOCK x 16 B: chunk c of thread t is the 8 entries
+// from (c * BLOCK + t) * 8 - lead on, so that every load is aligned whatever
+// the row's start; the first NC chunks stay in registers.  Entries outside
+// the row read as NaN, which is no candidate.
+template <int NC>
+struct Entries {
+  static constexpr int PER = 8;
+  const __hip_bfloat16* row;
   int V, lead, chunks;
-  u32x4 held[NC > 0 ? NC : 1];
+  u32x4 held[NC];
 
   __device__ __forceinline__ int first_of(const int c) const {
     return (c * BLOCK + (int)threadIdx.x) * PER - lead;
@@ -162,26 +232,19 @@ struct Entries {
     const int i = first_of(c);
     if (i >= 0 && i + PER <= V)
       return *reinterpret_cast<const u32x4*>(row + i);
-    u32x4 v = {~0u, ~0u, ~0u, ~0u};  // NaN in either type
-    if constexpr (sizeof(T) == 4) {
-      const unsigned* src = reinterpret_cast<const unsigned*>(row);
+    u32x4 v = {~0u, ~0u, ~0u, ~0u};  // NaN
+    const unsigned short* src = reinterpret_cast<const unsigned short*>(row);
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (i + j >= 0 && i + j < V) v[j] = src[i + j];
-    } else {
-      const unsigned short* src = reinterpret_cast<const unsigned short*>(row);
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (i + j >= 0 && i + j < V)
-          v[j / 2] = (j & 1) ? (v[j / 2] & 0xffffu) | ((unsigned)src[i + j] << 16)
-                             : (v[j / 2] & 0xffff0000u) | src[i + j];
-    }
+    for (int j = 0; j < 8; ++j)
+      if (i + j >= 0 && i + j < V)
+        v[j / 2] = (j & 1) ? (v[j / 2] & 0xffffu) | ((unsigned)src[i + j] << 16)
+                           : (v[j / 2] & 0xffff0000u) | src[i + j];
     return v;
   }
-  __device__ __forceinline__ void open(const T* r, const int v) {
+  __device__ __forceinline__ void open(const __hip_bfloat16* r, const int v) {
     row = r;
     V = v;
-    lead = (int)((reinterpret_cast<uintptr_t>(r) % 16) / sizeof(T));
+    lead = (int)((reinterpret_cast<uintptr_t>(r) % 16) / 2);
     chunks = (V + lead + BLOCK * PER - 1) / (BLOCK * PER);
 #pragma unroll
     for (int c = 0; c < NC; ++c)
@@ -196,27 +259,13 @@ struct Entries {
     for (int c = NC; c < chunks; ++c) f(c, load(c));
   }
   static __device__ __forceinline__ float get(const u32x4 v, const int j) {
-    if constexpr (sizeof(T) == 4)
-      return __uint_as_float(v[j]);
-    else
-      return __uint_as_float((j & 1) ? (v[j / 2] & 0xffff0000u)
-                                     : (v[j / 2] << 16));
-  }
-  // f(index, value) of every candidate, -0 as +0
-  template <typename F>
-  __device__ __forceinline__ void each(F f) const {
-    each_chunk([&](const int c, const u32x4 v) {
-      const int i = first_of(c);
-#pragma unroll
-      for (int j = 0; j < PER; ++j) {
-        const float x = get(v, j) + 0.f;
-        if (candidate(x)) f(i + j, x);
-      }
-    });
+    return __uint_as_float((j & 1) ? (v[j / 2] & 0xffff0000u)
+                                   : (v[j / 2] << 16));
   }
 };
 
 struct Shared {
+  double pow2[64];
   double red_d[NWAVES + 1];
   unsigned long long red_u[NWAVES + 1];
   float red_f[NWAVES];
@@ -270,94 +319,109 @@ __device__ __forceinline__ int within(const double goal, const double before,
 
 // ------------------------------------------------- the general, slow search
 
-// Count and weight of the candidates with a key above (or from) t.
-template <typename E>
-__device__ __forceinline__ void above(const E& e, const Row& r, const unsigned t,
-                      const bool from, long long& n, double& w, Shared& s,
-                      const bool weigh) {
-  unsigned long long cnt = 0;
-  double sum = 0.0;
-  e.each([&](int, const float x) {
-    const unsigned key = key_of(x);
-    if (key > t || (from && key == t)) {
-      ++cnt;
-      if (weigh) sum += weight(x, r);
-    }
-  });
-  n = (long long)block_total<unsigned long long>(cnt, s.red_u);
-  w = weigh ? block_total<double>(sum, s.red_d) : 0.0;
-}
-
-// The largest key t with  count(key >= t) >= rank  or  weight(key >= t) > goal
-template <typename E>
-__device__ __forceinline__ unsigned bisect(const E& e, const Row& r, const bool by_count,
-                           const long long rank, const double goal,
-                           const bool reach, Shared& s) {
-  unsigned t = 0;
-  for (int bit = 31; bit >= 0; --bit) {
-    const unsigned up = t | (1u << bit);
-    long long n;
-    double w;
-    above(e, r, up, true, n, w, s, !by_count);
-    if (by_count ? n >= rank : (reach ? w >= goal : w > goal)) t = up;
-  }
-  return t;
-}
-
-template <typename E>
-__device__ __forceinline__ double sum_of_first(const E& e, const Row& r, const long long n,
-                               Shared& s) {
-  const unsigned t = bisect(e, r, true, n, 0.0, false, s);
-  long long cnt;
-  double w;
-  above(e, r, t, false, cnt, w, s, true);
-  return w + (double)(n - cnt) * weight(value_of(t), r);
-}
-
-// A call of its own: its registers are not the fast paths'.
+// Count and weight of the candidates with a key above (or from) t, and the
+// count of those that weigh min_p or more.
 template <typename T>
-__device__ __noinline__ Answer general(const T* row, const int V, const Row& r, Shared& s) {
-  Entries<T, 0> e;  // read again in every pass
-  e.open(row, V);
-  long long all;
-  double w_all;
-  above(e, r, 0u, true, all, w_all, s, true);
-  long long n = min((long long)r.k, all);
-  if (r.top_p < 1.0) {
-    const double goal =
-        r.top_p * (n == all ? w_all : sum_of_first(e, r, n, s));
-    long long np = 0;
-    if (goal > 0.0) {
-      // the key in which the sum reaches the goal (the last of all where
-      // rounding keeps it short): ranks above it lie before the goal
-      const unsigned t = bisect(e, r, false, 0, goal, true, s);
-      long long upto, cnt;
-      double w, before;
-      above(e, r, t, true, upto, w, s, false);
-      above(e, r, t, false, cnt, before, s, true);
-      np = cnt + within(goal, before, weight(value_of(t), r),
-                        (int)(upto - cnt), false);
+__device__ __forceinline__ void above(const Plain<T>& e, const Row& r,
+                                      const unsigned t, const bool from,
+                                      long long& n, double& w, long long& nm,
+                                      Shared& s) {
+  unsigned long long cnt = 0, cm = 0;
+  double sum = 0.0;
+#pragma unroll 1
+  for (int i = threadIdx.x; i < e.V; i += BLOCK) {
+    const float x = e.at(i);
+    const unsigned key = key_of(x);
+    if (candidate(x) && (key > t || (from && key == t))) {
+      const double wi = weight(x, r);
+      ++cnt;
+      cm += wi >= r.min_p;
+      sum += wi;
     }
-    n = min(n, np);
   }
-  unsigned long long cm = 0;
-  e.each([&](int, const float x) { cm += weight(x, r) >= r.min_p; });
-  n = min(n, (long long)block_total<unsigned long long>(cm, s.red_u));
-  n = max(n, 1ll);
-  const double goal = r.u * sum_of_first(e, r, n, s);
-  unsigned t = bisect(e, r, false, 0, goal, false, s);
-  long long upto, cnt;
-  double w, before;
-  above(e, r, t, false, cnt, before, s, true);
-  if (cnt >= n) {  // rounding kept every sum short: the last rank kept
-    t = bisect(e, r, true, n, 0.0, false, s);
-    above(e, r, t, false, cnt, before, s, true);
+  n = (long long)block_total<unsigned long long>(cnt, s.red_u);
+  nm = (long long)block_total<unsigned long long>(cm, s.red_u);
+  w = block_total<double>(sum, s.red_d);
+}
+
+// The four questions of a row, each by bisection for the largest key t with
+// count(key >= t) >= rank, weight(key >= t) >= goal, or > goal.  All passes
+// are one instance of the loop over the row: it keeps few registers.
+template <typename T>
+__device__ __forceinline__ Answer general(const Plain<T>& e, const Row& r,
+                                          Shared& s) {
+  long long all = 0, nm = 0, N = 0;
+  double Z = 0.0;
+  unsigned t = 0;
+  int nth = 0;
+  bool by_count = true;
+#pragma unroll 1
+  for (int step = -1; step < 4;) {
+    if (step == 2) N = max(1ll, min(N, nm));
+    if (step >= 0 && step < 2 && !(r.top_p < 1.0)) {
+      ++step;
+      continue;
+    }
+    const double goal = step == 1 ? r.top_p * Z : r.u * Z;
+    if (step == 1 && !(goal > 0.0)) {
+      N = 0;
+      ++step;
+      continue;
+    }
+    long long cnt = 0;
+    double before = 0.0;
+    int ties = 0;
+    t = 0;
+    // passes 0..31 bisect, 32 takes what lies above t, 33 that and t itself
+#pragma unroll 1
+    for (int pass = step < 0 ? 33 : 0; pass < 34; ++pass) {
+      const unsigned key = pass < 32 ? t | (1u << (31 - pass)) : t;
+      long long n, m;
+      double w;
+      above(e, r, key, pass != 32, n, w, m, s);
+      if (pass < 32) {
+        if (by_count ? n >= N : step == 1 ? w >= goal : w > goal) t = key;
+      } else if (pass == 32) {
+        cnt = n;
+        before = w;
+      } else {
+        ties = (int)(n - cnt);
+        all = n;
+        if (step < 0) nm = m;
+      }
+    }
+    const double wt = weight(value_of(t), r);
+    if (step < 0) {
+      N = min((long long)r.k, all);
+    } else if (step == 3 && !by_count && cnt >= N) {
+      // rounding keeps every sum short of the draw: the last rank kept
+      by_count = true;
+      continue;
+    } else if ((step & 1) == 0) {
+      Z = before + (double)(N - cnt) * wt;
+    } else if (step == 1) {
+      N = min(N, cnt + within(goal, before, wt, ties, false));
+    } else {
+      nth = (int)min((long long)within(goal, before, wt, ties - 1, true),
+                     N - 1 - cnt);
+    }
+    ++step;
+    by_count = (step & 1) == 0;
   }
-  above(e, r, t, true, upto, w, s, false);
-  int j = within(goal, before, weight(value_of(t), r), (int)(upto - cnt) - 1,
-                 true);
-  j = (int)min((long long)j, n - 1 - cnt);
-  return {nth_of_value(e, value_of(t), j, s), (int)n, 0, 0.f};
+  // the nth entry, in order of index, whose key is t
+  int left = nth, token = 0;
+#pragma unroll 1
+  for (int i0 = 0; i0 < e.V && left >= 0; i0 += BLOCK) {
+    const int i = i0 + threadIdx.x;
+    const bool is = i < e.V && candidate(e.at(i)) && key_of(e.at(i)) == t;
+    unsigned long long here;
+    const int rank = (int)block_scan<unsigned long long>(is, s.red_u, &here);
+    if (is && rank == left) s.at = i;
+    __syncthreads();
+    if (left < (int)here) token = s.at;
+    left -= (int)here;
+  }
+  return {token, (int)N, 0, 0.f};
 }
 
 // --------------------------------------------------- bf16: bins are values
@@ -388,7 +452,7 @@ __device__ __forceinline__ int last_entry(const int entries, Shared& s, F ok) {
 
 // Both row functions say false where the general search has to take the row.
 template <int NC>
-__device__ __forceinline__ bool bf16_row(const Entries<__hip_bfloat16, NC>& e,
+__device__ __forceinline__ bool bf16_row(const Entries<NC>& e,
                                         const Row& r, Lds16& L, Answer& ans) {
   Shared& s = L.s;
   const int tid = threadIdx.x;
@@ -558,9 +622,8 @@ struct Lds32 {
   Shared s;
 };
 
-template <int NC>
-__device__ __forceinline__ bool fp32_row(const Entries<float, NC>& e,
-                                        const Row& r, Lds32& L, Answer& ans) {
+__device__ __forceinline__ bool fp32_row(const Plain<float>& e, const Row& r,
+                                        Lds32& L, Answer& ans) {
   constexpr int PT = BINS32 / BLOCK;  // bins of a thread, in order
   Shared& s = L.s;
   const int tid = threadIdx.x;
@@ -573,7 +636,7 @@ __device__ __forceinline__ bool fp32_row(const Entries<float, NC>& e,
   // the bins cover the others
   const double reach = 746.0 * r.T;
   float low = r.m;
-  e.each([&](int, const float x) {
+  e.template each<8>([&](int, const float x) {
     if ((double)r.m - (double)x <= reach) low = fminf(low, x);
   });
   low = -block_largest(-low, s.red_f);
@@ -585,15 +648,14 @@ __device__ __forceinline__ bool fp32_row(const Entries<float, NC>& e,
   const auto bin_of = [&](const float x) __attribute__((always_inline)) {
     return min(BINS32 - 1, (int)((r.m - x) * by));
   };
-  const double inv = 1.0 / r.T;
   unsigned long long nm = 0, far = 0;
-  e.each([&](int, const float x) {
+  e.template each<2>([&](int, const float x) {
     if (x < low) {
       ++far;
       nm += 0.0 >= r.min_p;
       return;
     }
-    const double w = x == r.m ? 1.0 : exp(((double)x - (double)r.m) * inv);
+    const double w = weight(x, r);
     const int b = bin_of(x);
     atomicAdd(&L.w[b], (unsigned long long)(w * FIXED + 0.5));
     atomicAdd(&L.n[b], 1u);
@@ -615,188 +677,212 @@ __device__ __forceinline__ bool fp32_row(const Entries<float, NC>& e,
                                                                &listed);
   const double w_all = (double)w_fix * (1.0 / FIXED);
 
-  // ---- the bin with a rank or a sum, and its members in order
-  int bin = -1, members = 0, before_n = 0;
+  // ---- four questions, each to one bin: the sum of the first n_k, the rank
+  // of the top-p border, the sum of the first N, the rank of the draw
+  const long long all = (long long)(listed + far);
+  long long N = min((long long)r.k, all);
+  double Z = w_all;
+  int bin = -1, members = 0, before_n = 0, token = 0;
   double before_w = 0.0;
-  // (first bin whose count up to its end reaches `rank`, or whose sum does)
-  const auto open = [&](const bool by_count, const long long rank,
-                        const double goal, const bool pass) __attribute__((always_inline)) {
-    __syncthreads();
-    if (tid == 0) s.hit = -1;
-    __syncthreads();
-    unsigned long long cw = bw, cn = bn;
-#pragma unroll
-    for (int j = 0; j < PT; ++j) {
-      const int b = tid * PT + j;
-      const unsigned long long ew = cw + L.w[b], en = cn + L.n[b];
-      const double d0 = (double)cw * (1.0 / FIXED);
-      const double d1 = (double)ew * (1.0 / FIXED);
-      const bool here =
-          L.n[b] != 0 &&
-          (by_count ? ((long long)cn < rank && (long long)en >= rank)
-           : pass   ? (d0 <= goal && d1 > goal)
-                    : (d0 < goal && d1 >= goal));
-      if (here) {
-        s.hit = b;
-        s.at = (int)cn;
-        s.hit_before = d0;
-      }
-      cw = ew;
-      cn = en;
+#pragma unroll 1
+  for (int step = 0; step < 4; ++step) {
+    if (step == 2) N = max(1ll, min(N, (long long)nm));
+    if (step < 2 && !(r.top_p < 1.0)) continue;
+    bool by_count = (step & 1) == 0;
+    if (by_count && N >= (long long)listed) {
+      Z = w_all;
+      continue;
     }
-    __syncthreads();
-    if (s.hit < 0 || s.hit == bin) return s.hit >= 0;
-    bin = s.hit;
-    before_n = s.at;
-    before_w = s.hit_before;
-    members = (int)L.n[bin];
-    if (members > MEMBERS) return true;  // the caller looks
-    if (tid == 0) s.members = 0;
-    __syncthreads();
-    e.each([&](const int i, const float x) {
-      if (x >= low && bin_of(x) == bin) {
-        const unsigned p = atomicAdd(&s.members, 1u);
-        L.key[p] = key_of(x);
-        L.index[p] = i;
-      }
-    });
-    __syncthreads();
-    for (int p = tid; p < members; p += BLOCK) {
-      const unsigned key = L.key[p];
-      const int i = L.index[p];
-      int rank_in = 0;
-      for (int q = 0; q < members; ++q) {
-        const unsigned k2 = L.key[q];
-        rank_in += k2 > key || (k2 == key && L.index[q] < i);
-      }
-      L.sorted_key[rank_in] = key;
-      L.sorted_index[rank_in] = i;
+    const double goal = step == 1 ? r.top_p * Z : r.u * Z;
+    if (step == 1 && !(goal > 0.0)) {
+      N = 0;
+      continue;
     }
-    __syncthreads();
-    return true;
-  };
-  // walks the open bin: ranks in it whose sum before (or with) them does not
-  // pass the goal, at most `upto` ranks; the sum of those
-  const auto walk = [&](const int upto, const double goal, const bool with,
-                        double& sum) __attribute__((always_inline)) {
+    bool found = false;
+    const long long rank = min(N, (long long)listed);
+#pragma unroll 1
+    for (int again = 0; again < 2; ++again) {
+      __syncthreads();
+      if (tid == 0) s.hit = -1;
+      __syncthreads();
+      unsigned long long cw = bw, cn = bn;
+#pragma unroll 1
+      for (int b = tid * PT; b < tid * PT + PT; ++b) {
+        const unsigned n = L.n[b];
+        const unsigned long long ew = cw + L.w[b], en = cn + n;
+        const double d0 = (double)cw * (1.0 / FIXED);
+        const double d1 = (double)ew * (1.0 / FIXED);
+        if (n != 0 &&
+            (by_count    ? ((long long)cn < rank && (long long)en >= rank)
+             : step == 1 ? (d0 < goal && d1 >= goal)
+                         : (d0 <= goal && d1 > goal))) {
+          s.hit = b;
+          s.at = (int)cn;
+          s.hit_before = d0;
+        }
+        cw = ew;
+        cn = en;
+      }
+      __syncthreads();
+      found = s.hit >= 0;
+      // the draw's two sums agree to the last bits only: the last rank kept
+      // at most
+      if (step != 3 || by_count || (found && s.at < N)) break;
+      by_count = true;
+    }
+    if (!found) {  // (step 1: rounding keeps the whole sum short of the goal)
+      N = min(N, (long long)listed);
+      continue;
+    }
+    if (s.hit != bin) {
+      bin = s.hit;
+      before_n = s.at;
+      before_w = s.hit_before;
+      members = (int)L.n[bin];
+      if (members > MEMBERS) return false;
+      if (tid == 0) s.members = 0;
+      __syncthreads();
+      e.template each<8>([&](const int i, const float x) {
+        if (x >= low && bin_of(x) == bin) {
+          const unsigned p = atomicAdd(&s.members, 1u);
+          L.key[p] = key_of(x);
+          L.index[p] = i;
+        }
+      });
+      __syncthreads();
+      for (int p = tid; p < members; p += BLOCK) {
+        const unsigned key = L.key[p];
+        const int i = L.index[p];
+        int rank_in = 0;
+        for (int q = 0; q < members; ++q) {
+          const unsigned k2 = L.key[q];
+          rank_in += k2 > key || (k2 == key && L.index[q] < i);
+        }
+        L.sorted_key[rank_in] = key;
+        L.sorted_index[rank_in] = i;
+      }
+      __syncthreads();
+    }
+    // the bin's ranks that come before the goal, and their sum up to rank N
+    const int upto =
+        (step & 1) ? members : (int)min((long long)members, N - before_n);
+    double mine[MEMBERS / BLOCK], t = 0.0, sum;
     const int per = (members + BLOCK - 1) / BLOCK;
-    double mine[MEMBERS / BLOCK], t = 0.0, all;
 #pragma unroll
     for (int j = 0; j < MEMBERS / BLOCK; ++j) {
       const int p = tid * per + j;
-      mine[j] = 0.0;
-      if (j < per && p < members && p < upto)
-        mine[j] = weight(value_of(L.sorted_key[p]), r);
+      mine[j] = (j < per && p < upto) ? weight(value_of(L.sorted_key[p]), r)
+                                      : 0.0;
       t += mine[j];
     }
-    double b = before_w + block_scan<double>(t, s.red_d, &all);
+    double b = before_w + block_scan<double>(t, s.red_d, &sum);
     unsigned long long n = 0;
 #pragma unroll
     for (int j = 0; j < MEMBERS / BLOCK; ++j) {
-      const int p = tid * per + j;
-      if (j < per && p < members && p < upto)
-        n += with ? (b + mine[j] <= goal) : (b < goal);
+      if (j < per && tid * per + j < upto)
+        n += step == 1 ? b < goal : b + mine[j] <= goal;
       b += mine[j];
     }
-    sum = before_w + all;
-    return (int)block_total<unsigned long long>(n, s.red_u);
-  };
-  const auto sum_first = [&](const long long n, double& Z) __attribute__((always_inline)) {
-    if (n >= (long long)listed) {
-      Z = w_all;
-      return true;
-    }
-    open(true, n, 0.0, false);
-    if (members > MEMBERS) return false;
-    walk((int)(n - before_n), 0.0, false, Z);
-    return true;
-  };
-
-  const long long all = (long long)(listed + far);
-  long long N = min((long long)r.k, all);
-  double Z;
-  if (r.top_p < 1.0) {
-    if (!sum_first(N, Z)) return false;
-    const double goal = r.top_p * Z;
-    long long np = 0;
-    if (goal > 0.0) {
-      if (open(false, 0, goal, false)) {
-        if (members > MEMBERS) return false;
-        double sum;
-        np = before_n + walk(members, goal, false, sum);
-      } else {
-        np = (long long)listed;
-      }
-    }
-    N = min(N, np);
+    n = block_total<unsigned long long>(n, s.red_u);
+    if ((step & 1) == 0) Z = before_w + sum;
+    if (step == 1) N = min(N, before_n + (long long)n);
+    if (step == 3)
+      token = L.sorted_index[(int)min((long long)min((int)n, members - 1),
+                                      N - 1 - before_n)];
   }
-  N = max(1ll, min(N, (long long)nm));
-  if (!sum_first(N, Z)) return false;
-  const double goal = r.u * Z;
-  // (the two sums agree to the last bits only: the last rank kept at most)
-  if (!open(false, 0, goal, true) || before_n >= N) open(true, N, 0.0, false);
-  if (members > MEMBERS) return false;
-  double sum;
-  int j = walk(members, goal, true, sum);
-  j = (int)min((long long)min(j, members - 1), N - 1 - before_n);
-  ans = {L.sorted_index[j], (int)N, 0, 0.f};
+  ans = {token, (int)N, 0, 0.f};
   return true;
 }
 
-template <typename T>
-struct LdsOf;
-template <>
-struct LdsOf<__hip_bfloat16> {
-  using type = Lds16;
-};
-template <>
-struct LdsOf<float> {
-  using type = Lds32;
-};
-
-template <typename T, int NC>
-__global__ __launch_bounds__(BLOCK) void sample_filtered_kernel(const Args a) {
-  __shared__ __attribute__((aligned(16))) typename LdsOf<T>::type L;
-  const int b = blockIdx.x;
+// What is the row's filters' apart from its logits; false: not asked for.
+__device__ __forceinline__ bool open_row(const Args& a, const int b, Row& r,
+                                         Shared& s) {
   const float u = a.uniform[b];
-  if (u < 0.f) return;  // the row is not asked for: it stays as it was
-  Entries<T, NC> e;
-  e.open(reinterpret_cast<const T*>(a.logits) + (int64_t)b * a.V, a.V);
-  Row r;
-  float m = -INFINITY;
-  e.each([&](int, const float x) { m = fmaxf(m, x); });
-  r.m = block_largest(m, L.s.red_f);
-  const float T_ = a.temperature[b];
+  if (u < 0.f) return false;
   const int k = a.top_k[b];
-  r.T = (double)T_;
+  r.T = (double)a.temperature[b];
+  r.inv_T = 1.0 / r.T;
   r.k = (k > 0 && k < a.V) ? k : a.V;
   r.top_p = (double)a.top_p[b];
   r.min_p = (double)a.min_p[b];
   r.u = fmin((double)u, 1.0 - 0x1p-53);  // [0, 1); NaN too
-  Answer ans{0, 1, 0, 0.f};
-  bool done = true;  // the same in all threads
-  if (r.m == -INFINITY) {
-    // no candidate: token 0
-  } else if (!(T_ > 0.f)) {
-    ans = {-1, 1, 0, r.m};
-  } else {
-    if constexpr (sizeof(T) == 2)
-      done = bf16_row(e, r, L, ans);
-    else
-      done = fp32_row(e, r, L, ans);
+  r.pow2 = s.pow2;
+  if (threadIdx.x < 64) s.pow2[threadIdx.x] = POW2_64TH[threadIdx.x];
+  return true;
+}
+
+__device__ __forceinline__ void answer(const Args& a, const int b,
+                                       const int token, const int kept) {
+  if (threadIdx.x == 0) {
+    a.out[b] = token;
+    if (a.kept) a.kept[b] = kept;
   }
-  // (known to be uniform, the call keeps no register of the other branch)
+}
+
+template <int NC>
+__global__ __launch_bounds__(BLOCK) void sample_filtered_bf16_kernel(
+    const Args a) {
+  __shared__ __attribute__((aligned(16))) Lds16 L;
+  const int b = blockIdx.x;
+  Row r;
+  if (!open_row(a, b, r, L.s)) return;  // out and kept stay as they were
+  const __hip_bfloat16* row =
+      reinterpret_cast<const __hip_bfloat16*>(a.logits) + (int64_t)b * a.V;
+  Entries<NC> e;
+  e.open(row, a.V);
+  float m = -INFINITY;
+  e.each_chunk([&](int, const u32x4 v) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = fmaxf(m, e.get(v, j));  // not a NaN
+  });
+  r.m = block_largest(m, L.s.red_f) + 0.f;
+  Answer ans{0, 1, 0, 0.f};  // no candidate: token 0
+  bool done = true;          // the same in all threads
+  if (r.m > -INFINITY) {
+    ans = {-1, 1, 0, r.m};  // T <= 0: the first of the largest
+    if (r.T > 0.0) done = bf16_row(e, r, L, ans);
+  }
+  // (known to be uniform, neither branch keeps the other's registers)
   if (!__builtin_amdgcn_readfirstlane(done)) {
     __syncthreads();
-    ans = general(reinterpret_cast<const T*>(a.logits) + (int64_t)b * a.V, a.V,
-                  r, L.s);
+    ans = general(Plain<__hip_bfloat16>{row, a.V}, r, L.s);
   } else if (__builtin_amdgcn_readfirstlane(ans.token) < 0) {
     ans.token = nth_of_value(e, ans.x, ans.nth, L.s);
   }
-  if (threadIdx.x == 0) {
-    a.out[b] = ans.token;
-    if (a.kept) a.kept[b] = ans.kept;
+  answer(a, b, ans.token, ans.kept);
+}
+
+__global__ __launch_bounds__(BLOCK) void sample_filtered_fp32_kernel(
+    const Args a) {
+  __shared__ __attribute__((aligned(16))) Lds32 L;
+  const int b = blockIdx.x;
+  Row r;
+  if (!open_row(a, b, r, L.s)) return;
+  const Plain<float> e{
+      reinterpret_cast<const float*>(a.logits) + (int64_t)b * a.V, a.V};
+  float m = -INFINITY;
+  e.template each<8>([&](int, const float x) { m = fmaxf(m, x); });
+  r.m = block_largest(m, L.s.red_f);
+  Answer ans{0, 1, 0, 0.f};
+  bool done = true;
+  if (r.m > -INFINITY) {
+    if (r.T > 0.0) {
+      done = fp32_row(e, r, L, ans);
+    } else {
+      if (threadIdx.x == 0) L.s.at = a.V;
+      __syncthreads();
+      e.template each<8>([&](const int i, const float x) {
+        if (x == r.m) atomicMin(&L.s.at, i);
+      });
+      __syncthreads();
+      ans.token = L.s.at;
+    }
   }
+  if (!__builtin_amdgcn_readfirstlane(done)) {
+    __syncthreads();
+    ans = general(e, r, L.s);
+  }
+  answer(a, b, ans.token, ans.kept);
 }
 
 }  // namespace
@@ -843,17 +929,14 @@ void sample_filtered(torch::Tensor out, torch::Tensor logits,
                (const float*)min_p.data_ptr(),
                (const float*)uniform.data_ptr(),
                (int)V};
-#define LAUNCH(T, NC)                                                       \
-  hipLaunchKernelGGL((sample_filtered_kernel<T, NC>), dim3((unsigned)B),    \
-                     dim3(BLOCK), 0, s, a)
-  // bf16 rows of up to 64 KB or 256 KB stay in registers (beyond, the rest is
-  // read again); fp32 rows are read from L2 in every pass
+  // a bf16 row's first 64 KB or 256 KB stay in registers, the rest is read
+  // again; fp32 rows are read from L2 in every pass
+  const dim3 grid((unsigned)B), block(BLOCK);
   if (logits.scalar_type() == torch::kFloat32)
-    LAUNCH(float, 0);
+    hipLaunchKernelGGL(sample_filtered_fp32_kernel, grid, block, 0, s, a);
   else if (V * 2 <= 65536 - 16)
-    LAUNCH(__hip_bfloat16, 4);
+    hipLaunchKernelGGL((sample_filtered_bf16_kernel<4>), grid, block, 0, s, a);
   else
-    LAUNCH(__hip_bfloat16, 16);
-#undef LAUNCH
+    hipLaunchKernelGGL((sample_filtered_bf16_kernel<16>), grid, block, 0, s, a);
   HIP_CHECK_LAST();
 }
