@@ -23,6 +23,7 @@ from __future__ import annotations
 
 import logging
 import queue
+import struct
 import threading
 import time
 from concurrent.futures import Future
@@ -53,10 +54,23 @@ PREFILL_BUDGET = int(_os.environ.get("CALF_PREFILL_BUDGET", "12288"))
 #: enough to LOSE throughput end-to-end (233 -> 210 turns/s at 512)
 RUN_STEPS = (8, 4, 2, 1)
 
+#: prefix groups of one decode run (more share without being grouped)
+MAX_PREFIX_GROUPS = 16
+#: whole pages a group's rows have in common before it is worth a pass
+MIN_PREFIX_PAGES = 2
+
 #: lockstep op channel opcodes (tensor-coded: the
 #: pickled broadcast_object_list per visit becomes one fixed int64[2]
 #: header broadcast, plus one int64 payload broadcast only for prefills)
 OP_STOP, OP_DECODE, OP_PREFILL = 0, 1, 2
+
+
+def _float_bits(x: float) -> int:
+    return int.from_bytes(struct.pack("<d", x), "little", signed=True)
+
+
+def _bits_float(i: int) -> float:
+    return struct.unpack("<d", i.to_bytes(8, "little", signed=True))[0]
 
 
 def _encode_prefill(seqs) -> list[int]:
@@ -65,7 +79,8 @@ def _encode_prefill(seqs) -> list[int]:
         r = s.request
         names = r.tool_names or []
         vals += [s.seq_id, r.max_new_tokens, int(r.temperature * 1e6),
-                 r.top_k, r.seed, int(r.ignore_eos),
+                 r.top_k, _float_bits(r.top_p), _float_bits(r.min_p), r.seed,
+                 int(r.ignore_eos),
                  r.tool_trigger if r.tool_names else -1, r.tool_ncalls,
                  len(names)]
         vals += names
@@ -78,9 +93,9 @@ def _decode_prefill(vals: list[int]) -> list["GenRequest"]:
     reqs = []
     i = 1
     for _ in range(vals[0]):
-        (sid, mx, temp_i, topk, seed, ig_eos, trig, ncalls,
-         n_names) = vals[i:i + 9]
-        i += 9
+        (sid, mx, temp_i, topk, topp, minp, seed, ig_eos, trig, ncalls,
+         n_names) = vals[i:i + 11]
+        i += 11
         names = vals[i:i + n_names]
         i += n_names
         n_ids = vals[i]
@@ -88,7 +103,9 @@ def _decode_prefill(vals: list[int]) -> list["GenRequest"]:
         ids = vals[i:i + n_ids]
         i += n_ids
         req = GenRequest(prompt_ids=list(ids), max_new_tokens=mx,
-                         temperature=temp_i / 1e6, top_k=topk, seed=seed,
+                         temperature=temp_i / 1e6, top_k=topk,
+                         top_p=_bits_float(topp), min_p=_bits_float(minp),
+                         seed=seed,
                          ignore_eos=bool(ig_eos),
                          tool_names=list(names) if trig >= 0 else None,
                          tool_trigger=max(trig, 0), tool_ncalls=ncalls)
@@ -104,6 +121,19 @@ def _row_key(seed: int, pos: int) -> int:
     kernel mix64's it with the vocab index)."""
     k = (seed * _GOLDEN + pos) & 0xFFFFFFFFFFFFFFFF
     return k - (1 << 64) if k >= (1 << 63) else k
+
+
+def _uniforms(keys):
+    """Row keys (uint64 array) -> the draws' random numbers in [0, 1), f32
+    (24 bits of a 64-bit mix of the key)."""
+    import numpy as np
+
+    x = keys ^ (keys >> np.uint64(30))
+    x = x * np.uint64(0xBF58476D1CE4E5B9)
+    x = (x ^ (x >> np.uint64(27))) * np.uint64(0x94D049BB133111EB)
+    x = x ^ (x >> np.uint64(31))
+    return ((x >> np.uint64(40)).astype(np.float64) * 2.0 ** -24).astype(
+        np.float32)
 
 
 @dataclass
@@ -128,6 +158,15 @@ class GenRequest:
     #: per token keeps the asyncio side from drowning in per-token tasks
     #: at large batch (profiles/r01_bench256_gaps.md).
     on_tokens: Callable[[list[int]], None] | None = None
+    #: nucleus and relative-probability filters (1.0 and 0.0: off).  A request
+    #: that uses either is drawn by ``ops.sample_filtered`` from one random
+    #: number for each (seed, token position); the others by ``ops.sample``.
+    top_p: float = 1.0
+    min_p: float = 0.0
+
+    @property
+    def filtered(self) -> bool:
+        return self.temperature > 0 and (self.top_p < 1 or self.min_p > 0)
 
 
 @dataclass
@@ -182,7 +221,15 @@ class InferenceEngine:
 
     def __init__(self, model: LlamaShard, *, max_batch: int = 64,
                  kv_pages: int | None = None, use_graphs: bool | None = None,
-                 max_model_len: int | None = None):
+                 max_model_len: int | None = None, kv_dtype: str = "bf16",
+                 shared_prefix: bool = False):
+        #: kv_dtype "fp8": the cache holds e4m3 codes with a power-of-two
+        #: scale for each (token, head) — half the bytes, so twice the
+        #: conversations a rank holds.  shared_prefix: decode attends a prefix
+        #: that running sequences have in common (the same cached pages) once
+        #: for all of them.
+        if kv_dtype not in ("bf16", "fp8"):
+            raise ValueError(f"kv_dtype must be 'bf16' or 'fp8': {kv_dtype!r}")
         #: TP/EP>1 serving runs in lockstep: rank 0 schedules and broadcasts
         #: each action; ranks > 0 replay them via follow() — every rank then
         #: executes identical forwards (and RCCL collectives) in identical
@@ -227,7 +274,11 @@ class InferenceEngine:
                         // PAGE_SIZE + 8 + max_batch)
         self.kv = KVCache(layers=self.cfg.layers, kv_heads=model.hkv,
                           head_dim=model.dh, num_pages=kv_pages,
-                          device=self.device)
+                          device=self.device,
+                          dtype=(torch.float8_e4m3fn if kv_dtype == "fp8"
+                                 else torch.bfloat16))
+        self._kv_scales = (list(zip(self.kv.kscale, self.kv.vscale))
+                           if kv_dtype == "fp8" else None)
         # page-table width carries multi-step overshoot headroom: a sequence
         # at max_model_len batched with a longer-budget one blind-runs up to
         # RUN_STEPS[0]-1 extra slots before truncation
@@ -266,6 +317,19 @@ class InferenceEngine:
         #: per-(step, row) RNG keys = request seed x token position, so a
         #: request's sampled tokens do not depend on batch composition
         self._row_seeds = torch.zeros(MS, B, dtype=torch.int64, device=dev)
+        # filtered draws (top-p / min-p); a negative random number leaves the
+        # row's token to ops.sample
+        self._ftopk = torch.zeros(B, dtype=torch.int32, device=dev)
+        self._topp = torch.ones(B, dtype=torch.float32, device=dev)
+        self._minp = torch.zeros(B, dtype=torch.float32, device=dev)
+        self._uniform = torch.full((MS, B), -1.0, dtype=torch.float32,
+                                   device=dev)
+        self._filters_set = False  # whether the buffers hold any
+        # prefix groups of the running rows
+        self.shared_prefix = shared_prefix
+        self._group = torch.full((B,), -1, dtype=torch.int32, device=dev)
+        self._group_lens = torch.zeros(MAX_PREFIX_GROUPS, dtype=torch.int32,
+                                       device=dev)
         # tool-call grammar state (static graph I/O; trigger<0 = row off)
         from .. import ops as _gops
 
@@ -518,7 +582,7 @@ class InferenceEngine:
             logits = model.forward(
                 tokens, positions, self.kv.kcache, self.kv.vcache, slots_t,
                 prefill_scratch=self._prefill_kv, past_len=done,
-                logits_rows=slice(t - 1, t))
+                logits_rows=slice(t - 1, t), kv_scales=self._kv_scales)
             done += t
         assert logits is not None
         first = self._sample_host(logits, seq)
@@ -622,7 +686,8 @@ class InferenceEngine:
             self.kv.kcache, self.kv.vcache,
             torch.as_tensor(slots, dtype=torch.int32).to(dev),
             prefill_plan=plan,
-            logits_rows=(q_starts[1:].long() - 1))
+            logits_rows=(q_starts[1:].long() - 1),
+            kv_scales=self._kv_scales)
         for s in seqs:
             self.kv.register_prefix(s.seq_id, s.request.prompt_ids)
         sampled = self._sample_launch(logits, seqs)
@@ -671,6 +736,20 @@ class InferenceEngine:
         if not pages_l:
             return
         dev = self.device
+        if self._kv_scales is not None:
+            # scratch row -> cache slot; rows still to be written: none
+            slots = torch.full((kv_starts_l[-1],), -1, dtype=torch.int32)
+            slots[torch.as_tensor(rows_l)] = (
+                torch.as_tensor(pages_l, dtype=torch.int32)[:, None] * PG
+                + torch.arange(PG, dtype=torch.int32)).view(-1)
+            slots = slots.to(dev)
+            from .. import ops
+
+            for layer, (kbuf, vbuf) in enumerate(self._prefill_kv):
+                ops.kv_read_fp8(kbuf[:slots.numel()], vbuf[:slots.numel()],
+                                self.kv.kcache[layer], self.kv.vcache[layer],
+                                *self._kv_scales[layer], slots)
+            return
         pages = torch.as_tensor(pages_l, dtype=torch.long, device=dev)
         rows = torch.as_tensor(rows_l, dtype=torch.long, device=dev)
         hkv, dh = self.model.hkv, self.model.dh
@@ -692,8 +771,8 @@ class InferenceEngine:
         out = torch.zeros(B, dtype=torch.int32, device=logits.device)
         temp = torch.as_tensor([s.request.temperature for s in seqs],
                                dtype=torch.float32).to(logits.device)
-        topk = torch.as_tensor([s.request.top_k for s in seqs],
-                               dtype=torch.int32).to(logits.device)
+        topks = [0 if s.request.filtered else s.request.top_k for s in seqs]
+        topk = torch.as_tensor(topks, dtype=torch.int32).to(logits.device)
         seed = torch.as_tensor(
             [seqs[0].request.seed or seqs[0].seq_id, self._step_counter],
             dtype=torch.int64).to(logits.device)
@@ -703,9 +782,37 @@ class InferenceEngine:
         if any(s.request.tool_names for s in seqs):
             self._grammar_prefill(logits, seqs)
         ops.sample(out, logits, temp, seed,
-                   topk if any(s.request.top_k for s in seqs) else None,
+                   topk if any(topks) else None,
                    cand=self._prefill_cand, row_seeds=rks)
+        self._filter_first(out, logits, temp, seqs)
         return out
+
+    @staticmethod
+    def _filter_first(out: torch.Tensor, logits: torch.Tensor,
+                      temp: torch.Tensor, seqs: list["_Seq"]) -> None:
+        """Draw the first token of the requests that filter; the other rows
+        keep what ``ops.sample`` gave them."""
+        if not any(s.request.filtered for s in seqs):
+            return
+        import numpy as np
+
+        from .. import ops
+
+        keys = np.array([_row_key(s.request.seed or s.seq_id, 0)
+                         for s in seqs], dtype=np.int64).view(np.uint64)
+        u = np.where([s.request.filtered for s in seqs], _uniforms(keys),
+                     np.float32(-1))
+        dev = logits.device
+
+        def row(values, dtype):
+            return torch.as_tensor(values, dtype=dtype).to(dev)
+
+        ops.sample_filtered(
+            out, logits, temp,
+            row([s.request.top_k for s in seqs], torch.int32),
+            row([s.request.top_p for s in seqs], torch.float32),
+            row([s.request.min_p for s in seqs], torch.float32),
+            torch.from_numpy(u.astype(np.float32)).to(dev))
 
     def _grammar_prefill(self, logits: torch.Tensor,
                          seqs: list["_Seq"]) -> None:
@@ -744,8 +851,10 @@ class InferenceEngine:
         from .. import ops
         if r.tool_names:
             self._grammar_prefill(logits, [seq])
-        ops.sample(out, logits, temp, seed, topk if r.top_k else None,
+        ops.sample(out, logits, temp, seed,
+                   topk if r.top_k and not r.filtered else None,
                    row_seeds=rks)
+        self._filter_first(out, logits, temp, [seq])
         return int(out.item())
 
     # ---------------------------------------------------------------- decode
@@ -790,7 +899,7 @@ class InferenceEngine:
             pages = self.kv._slots[s.seq_id].pages
             pt[b, :len(pages)] = pages
             temps[b] = s.request.temperature
-            topks[b] = s.request.top_k
+            topks[b] = 0 if s.request.filtered else s.request.top_k
         steps = np.arange(M, dtype=np.int32)
         positions = base[None, :] + steps[:, None]
         lens = positions + 1
@@ -847,6 +956,31 @@ class InferenceEngine:
               + (toks[None, :] + steps.astype(np.uint64)[:, None]))
         self._row_seeds[:M, :pad].copy_(
             torch.from_numpy(rk.view(np.int64)), non_blocking=True)
+        filtered = np.zeros(pad, dtype=bool)
+        filtered[:B] = [s.request.filtered for s in self._running]
+        if filtered.any() or self._filters_set:
+            ftopk = np.zeros(pad, dtype=np.int32)
+            topp = np.ones(pad, dtype=np.float32)
+            minp = np.zeros(pad, dtype=np.float32)
+            ftopk[:B] = [s.request.top_k for s in self._running]
+            topp[:B] = [s.request.top_p for s in self._running]
+            minp[:B] = [s.request.min_p for s in self._running]
+            self._uniform.fill_(-1.0)  # rows of other batch sizes too
+            u = np.where(filtered[None, :], _uniforms(rk), np.float32(-1))
+            self._uniform[:M, :pad].copy_(torch.from_numpy(u),
+                                          non_blocking=True)
+            for buf, rows in ((self._ftopk, ftopk), (self._topp, topp),
+                              (self._minp, minp)):
+                buf[:pad].copy_(torch.from_numpy(rows), non_blocking=True)
+            self._filters_set = bool(filtered.any())
+        if self.shared_prefix:
+            group, lens = gops.build_prefix_groups(
+                pt[:B], base[:B], max_groups=MAX_PREFIX_GROUPS,
+                min_pages=MIN_PREFIX_PAGES)
+            full = np.full(pad, -1, dtype=np.int32)
+            full[:B] = group
+            self._group[:pad].copy_(torch.from_numpy(full), non_blocking=True)
+            self._group_lens.copy_(torch.from_numpy(lens), non_blocking=True)
         self._step_counter += M
 
     def _decode_run_gpu(self, pad: int, M: int) -> None:
@@ -860,7 +994,10 @@ class InferenceEngine:
                 tokens, self._positions[i, :pad], self.kv.kcache,
                 self.kv.vcache, self._slots[i, :pad],
                 page_table=self._page_table[:pad],
-                seq_lens=self._seq_lens[i, :pad])
+                seq_lens=self._seq_lens[i, :pad],
+                kv_scales=self._kv_scales,
+                prefix=((self._group[:pad], self._group_lens)
+                        if self.shared_prefix else None))
             # tool-call grammar: transition per-row state on the previous
             # token and bias the logits (no-op for rows without a plan)
             ops.grammar_bias(logits, tokens, self._gstate[:pad],
@@ -869,6 +1006,12 @@ class InferenceEngine:
             ops.sample(self._sampled[i, :pad], logits,
                        self._temperature[:pad], self._seeds[i],
                        self._topk[:pad], row_seeds=self._row_seeds[i, :pad])
+            # rows that filter by top-p or min-p are drawn again from their
+            # own logits; without any, every block leaves at once
+            ops.sample_filtered(self._sampled[i, :pad], logits,
+                                self._temperature[:pad], self._ftopk[:pad],
+                                self._topp[:pad], self._minp[:pad],
+                                self._uniform[i, :pad])
             tokens = self._sampled[i, :pad].long()  # on-device feedback
 
     def _capture_graphs(self) -> None:

@@ -2,7 +2,9 @@
 
 Layout per layer: [num_pages, Hkv_shard, PAGE=64, head_dim] bf16 — one
 (page, head) panel is a contiguous 16 KB run, matching the decode kernel's
-streaming pattern (ops/csrc/attn_decode.hip).
+streaming pattern (ops/csrc/attn_decode.hip).  With dtype float8_e4m3fn the
+same panels hold codes (8 KB) beside [num_pages, Hkv_shard, PAGE] scale bytes
+(ops/csrc/kv_fp8.hip): 2 x 129 bytes a token and head instead of 2 x 256.
 
 The allocator is a refcounted free-list over pages shared by all layers (a
 sequence holds the SAME page ids in every layer, so the page table is
@@ -64,11 +66,23 @@ class KVCache:
         self.num_pages = num_pages
         self.device = torch.device(device)
         self.prefix_cache = prefix_cache
+        self.dtype = dtype
         shape = (num_pages, kv_heads, PAGE_SIZE, head_dim)
-        self.kcache = [torch.zeros(shape, dtype=dtype, device=device)
-                       for _ in range(layers)]
-        self.vcache = [torch.zeros(shape, dtype=dtype, device=device)
-                       for _ in range(layers)]
+        #: scale bytes of an e4m3 cache, else None (per layer)
+        self.kscale: "list[torch.Tensor] | None" = None
+        self.vscale: "list[torch.Tensor] | None" = None
+        if dtype == torch.float8_e4m3fn:
+            self.kcache, self.vcache = (
+                [torch.zeros(shape, dtype=torch.uint8, device=device)
+                 .view(dtype) for _ in range(layers)] for _ in range(2))
+            self.kscale, self.vscale = (
+                [torch.zeros(shape[:3], dtype=torch.uint8, device=device)
+                 for _ in range(layers)] for _ in range(2))
+        else:
+            self.kcache = [torch.zeros(shape, dtype=dtype, device=device)
+                           for _ in range(layers)]
+            self.vcache = [torch.zeros(shape, dtype=dtype, device=device)
+                           for _ in range(layers)]
         self._free: list[int] = list(range(num_pages - 1, -1, -1))
         self._slots: dict[int, SequenceSlot] = {}
         self._ref: dict[int, int] = {}
@@ -84,7 +98,9 @@ class KVCache:
         return len(self._free) + len(self._lru)
 
     def bytes_per_page(self) -> int:
-        return self.layers * 2 * self.kv_heads * PAGE_SIZE * self.head_dim * 2
+        row = (self.head_dim + 1 if self.kscale is not None
+               else self.head_dim * 2)
+        return self.layers * 2 * self.kv_heads * PAGE_SIZE * row
 
     # ------------------------------------------------------------ allocation
     def _alloc_page(self) -> int:

@@ -69,7 +69,8 @@ def shared_engine(config: Any, device: str | None = None, *, tp: int = 1,
         device = "cuda" if torch.cuda.is_available() else "cpu"
     if ep > 1 and not config.is_moe:
         raise ValueError(f"{config.name} is dense; ep={ep} needs an MoE model")
-    key = (config.name, device, tp, ep)
+    key = (config.name, device, tp, ep, engine_kw.get("kv_dtype", "bf16"),
+           engine_kw.get("shared_prefix", False))
     with _ENGINES_LOCK:
         eng = _ENGINES.get(key)
         if eng is None:
@@ -109,12 +110,14 @@ class LocalModelClient:
     def __init__(self, model: Any = "llama-3-8b", *, device: str | None = None,
                  max_batch: int = 64, max_model_len: int | None = None,
                  use_graphs: bool | None = None, kv_pages: int | None = None,
-                 tp: int = 1, ep: int = 1):
+                 tp: int = 1, ep: int = 1, kv_dtype: str = "bf16",
+                 shared_prefix: bool = False):
         self._config = model
         self._device = device
         self._engine_kw = dict(max_batch=max_batch, max_model_len=max_model_len,
                                use_graphs=use_graphs, kv_pages=kv_pages, tp=tp,
-                               ep=ep)
+                               ep=ep, kv_dtype=kv_dtype,
+                               shared_prefix=shared_prefix)
         self._engine: InferenceEngine | None = None
         self._tokenizer: SyntheticTokenizer | None = None
 
@@ -210,6 +213,7 @@ class LocalModelClient:
             max_new_tokens=max(1, s.max_tokens),
             temperature=s.temperature,
             top_k=s.top_k,
+            top_p=s.top_p,
             seed=s.seed or 0,
             ignore_eos=False,
             tool_names=tool_names,

@@ -252,9 +252,14 @@ class LlamaShard:
               plan: "PrefillPlan | None",
               page_table: torch.Tensor | None,
               seq_lens: torch.Tensor | None,
+              kv_scale: "tuple[torch.Tensor, torch.Tensor] | None" = None,
+              prefix: "tuple[torch.Tensor, torch.Tensor] | None" = None,
               do_reduce: bool = True) -> torch.Tensor:
+        """``kv_scale``: the (K, V) scale bytes of an e4m3 cache; ``prefix``:
+        (group, group_lens) of rows that share prefixes (decode)."""
         T = hidden.shape[0]
         decode = plan is None
+        q = None
         qkv_w = lw.wqkv
         tplan = (self._tile_plan(T, qkv_w.shape[0], qkv_w.shape[1])
                  if decode else None)
@@ -265,25 +270,32 @@ class LlamaShard:
             Mp = ops.skinny_gemm_slabs(hidden, qkv_w, self._gemm_work, sk)
             qkv = torch.empty(T, qkv_w.shape[0], dtype=hidden.dtype,
                               device=hidden.device)
-            ops.rope_qkv_write_slab(qkv, self._gemm_work, kcache, vcache,
-                                    self.rope, positions, slots, self.hq,
-                                    self.hkv, Mp, sk)
+            self._rope_write_slab(qkv, kcache, vcache, kv_scale, positions,
+                                  slots, Mp, sk)
         elif tplan is not None and tplan[1] > 1:
             # tiled serving-batch path, same slab contract as skinny
             bn, sk = tplan
             Mp = ops.tile_gemm_slabs(hidden, qkv_w, self._gemm_work, bn, sk)
             qkv = torch.empty(T, qkv_w.shape[0], dtype=hidden.dtype,
                               device=hidden.device)
-            ops.rope_qkv_write_slab(qkv, self._gemm_work, kcache, vcache,
-                                    self.rope, positions, slots, self.hq,
-                                    self.hkv, Mp, sk)
+            self._rope_write_slab(qkv, kcache, vcache, kv_scale, positions,
+                                  slots, Mp, sk)
         else:
             qkv = self._proj(hidden, qkv_w, decode=decode)
             # fused epilogue: in-place RoPE on the packed q/k heads +
             # paged-cache scatter — q/k/v stay strided views (no copies)
-            ops.rope_qkv_write(qkv, kcache, vcache, self.rope, positions,
-                               slots, self.hq, self.hkv)
-        q = qkv[:, :self.hq * self.dh].view(T, self.hq, self.dh)
+            if kv_scale is None:
+                ops.rope_qkv_write(qkv, kcache, vcache, self.rope, positions,
+                                   slots, self.hq, self.hkv)
+            else:
+                # decode reads nothing but the queries of the packed rows
+                q = (torch.empty(T, self.hq, self.dh, dtype=qkv.dtype,
+                                 device=qkv.device) if decode else None)
+                ops.rope_qkv_write_fp8(qkv, kcache, vcache, *kv_scale,
+                                       self.rope, positions, slots, self.hq,
+                                       self.hkv, q_out=q)
+        if q is None:
+            q = qkv[:, :self.hq * self.dh].view(T, self.hq, self.dh)
         o = torch.empty(T, self.hq, self.dh, dtype=qkv.dtype, device=qkv.device)
         if plan is not None:
             if plan.kv_in_qkv:
@@ -310,6 +322,14 @@ class LlamaShard:
             ops.attn_prefill_varlen(
                 o, q, kk, vv, plan.block_map, plan.q_starts, plan.kv_starts,
                 plan.past_lens, self.scale)
+        elif prefix is not None:
+            kscale, vscale = kv_scale if kv_scale is not None else (None, None)
+            ops.attn_decode_shared(o, q, kcache, vcache, page_table, seq_lens,
+                                   *prefix, self.scale, kscale=kscale,
+                                   vscale=vscale)
+        elif kv_scale is not None:
+            ops.attn_decode_fp8(o, q, kcache, vcache, *kv_scale, page_table,
+                                seq_lens, self.scale)
         else:
             ops.attn_decode(o, q, kcache, vcache, page_table, seq_lens, self.scale)
         o2 = o.view(T, self.hq * self.dh)
@@ -328,6 +348,17 @@ class LlamaShard:
                 return ("slabs", Mp, sk)
         out = self._proj(o2, lw.wo, decode=decode)
         return all_reduce_sum(out) if (self.tp_size > 1 and do_reduce) else out
+
+    def _rope_write_slab(self, qkv, kcache, vcache, kv_scale, positions,
+                         slots, Mp: int, sk: int) -> None:
+        if kv_scale is None:
+            ops.rope_qkv_write_slab(qkv, self._gemm_work, kcache, vcache,
+                                    self.rope, positions, slots, self.hq,
+                                    self.hkv, Mp, sk)
+        else:
+            ops.rope_qkv_write_slab_fp8(qkv, self._gemm_work, kcache, vcache,
+                                        *kv_scale, self.rope, positions,
+                                        slots, self.hq, self.hkv, Mp, sk)
 
     def _mlp(self, lw: LayerWeights, hidden: torch.Tensor, *,
              decode: bool = False, do_reduce: bool = True):
@@ -361,7 +392,8 @@ class LlamaShard:
 
     # ------------------------------------------------- TP-overlap decode
     def _forward_tp_overlap(self, tokens, positions, kcaches, vcaches,
-                            slots, *, page_table, seq_lens, logits_rows):
+                            slots, *, page_table, seq_lens, logits_rows,
+                            kv_scales=None, prefix=None):
         """Decode forward as a two-chunk software pipeline: chunk c's
         row-parallel all-reduce runs on the comm stream WHILE chunk 1-c
         computes, with event ordering both ways (north star: RCCL
@@ -412,7 +444,11 @@ class LlamaShard:
                 o = self._attn(lw, hid[c], positions[cs[c]], kcaches[i],
                                vcaches[i], slots[cs[c]], prefill_kv=None,
                                plan=None, page_table=page_table[cs[c]],
-                               seq_lens=seq_lens[cs[c]], do_reduce=False)
+                               seq_lens=seq_lens[cs[c]],
+                               kv_scale=kv_scales[i] if kv_scales else None,
+                               prefix=((prefix[0][cs[c]], prefix[1])
+                                       if prefix is not None else None),
+                               do_reduce=False)
                 reduce_async(c, o)
                 nxt[c] = o
             for c in (0, 1):
@@ -464,10 +500,16 @@ class LlamaShard:
                 page_table: torch.Tensor | None = None,
                 seq_lens: torch.Tensor | None = None,
                 past_len: int = 0,
-                logits_rows: "slice | torch.Tensor | None" = None) -> torch.Tensor:
+                logits_rows: "slice | torch.Tensor | None" = None,
+                kv_scales: "list[tuple[torch.Tensor, torch.Tensor]] | None" = None,
+                prefix: "tuple[torch.Tensor, torch.Tensor] | None" = None,
+                ) -> torch.Tensor:
         """One forward pass.  Prefill mode when a plan (or the single-seq
         ``prefill_scratch``+``past_len`` convenience form) is given; decode
         mode otherwise (B sequences, one token each, via the paged tables).
+
+        ``kv_scales`` (per layer) makes the caches e4m3; ``prefix`` is the
+        (group, group_lens) pair of ``ops.attn_decode_shared`` for decode.
 
         Returns logits [rows, vocab] (rows = T or B or the logits_rows
         slice/index).
@@ -486,7 +528,8 @@ class LlamaShard:
                 return self._forward_tp_overlap(
                     tokens, positions, kcaches, vcaches, slots,
                     page_table=page_table, seq_lens=seq_lens,
-                    logits_rows=logits_rows)
+                    logits_rows=logits_rows, kv_scales=kv_scales,
+                    prefix=prefix)
         hidden = self.embed[tokens.long()]  # [T, d]
         residual = torch.zeros_like(hidden)
         for i, lw in enumerate(self.layers):
@@ -502,7 +545,8 @@ class LlamaShard:
             attn_out = self._attn(
                 lw, hidden, positions, kcaches[i], vcaches[i], slots,
                 prefill_kv=prefill_scratch[i] if prefill_scratch else None,
-                plan=plan, page_table=page_table, seq_lens=seq_lens)
+                plan=plan, page_table=page_table, seq_lens=seq_lens,
+                kv_scale=kv_scales[i] if kv_scales else None, prefix=prefix)
             if isinstance(attn_out, tuple):  # ("slabs", Mp, sk)
                 _, Mp, sk = attn_out
                 hidden = torch.empty_like(residual)
