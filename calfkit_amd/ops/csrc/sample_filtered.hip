@@ -37,7 +37,7 @@ using u32x4 = __attribute__((ext_vector_type(4))) unsigned;
 
 constexpr int BLOCK = 1024;
 constexpr int NWAVES = BLOCK / WAVE;
-constexpr int MAXCHUNKS = 129;  // of 8192 bf16 entries: up to 2^20
+constexpr int MAXCHUNKS = 257;  // of 4096 fp32 entries: up to 2^20
 constexpr int MAXV = 1 << 20;
 
 // bf16: magnitudes [2^-41, 2^23) are 64 octaves of 128 values, each sign
@@ -45,6 +45,7 @@ constexpr int BINS16 = 16384;
 constexpr int LO16 = 86 << 7, HI16 = 150 << 7;
 constexpr float FAR_VALUE = -8388608.f;  // -2^23
 constexpr int DISTINCT = 4096;
+constexpr int LISTED = BLOCK;  // equal values ranked one a thread
 // fp32
 constexpr int BINS32 = 8192;
 constexpr int MEMBERS = 2048;
@@ -85,17 +86,14 @@ struct Args {
 // What every path is asked: the row's filters.
 struct Row {
   float m;        // largest logit
-  double T, inv_T;  // temperature > 0
+  double inv_T;  // of a temperature > 0
   int k;          // top_k or V
-  double top_p;   // >= 1: off
-  double min_p;
-  double u;
   const double* pow2;  // POW2_64TH in LDS
 };
 
-// The token: an index, or (token < 0) the nth of the entries of value x.
+// The token: an index, or (token < 0) the nth of the `ties` entries of value x.
 struct Answer {
-  int token, kept, nth;
+  int token, kept, nth, ties;
   float x;
 };
 
@@ -135,43 +133,78 @@ __device__ __forceinline__ double weight(const float x, const Row& r) {
                   : exp_neg(((double)x - (double)r.m) * r.inv_T, r.pow2);
 }
 
-// ---- block-wide sums and scans; `lds` holds NWAVES + 1 values
+// ---- wave- and block-wide sums and scans over DPP lane moves (a few cycles a
+// step where a swap through LDS takes a hundred); `lds` holds NWAVES values
+
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned moved(const unsigned x) {
+  return (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf,
+                                               false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned long long moved(
+    const unsigned long long x) {
+  return ((unsigned long long)moved<CTRL, ROWS>((unsigned)(x >> 32)) << 32) |
+         moved<CTRL, ROWS>((unsigned)x);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double moved(const double x) {
+  return __longlong_as_double((long long)moved<CTRL, ROWS>(
+      (unsigned long long)__double_as_longlong(x)));
+}
+__device__ __forceinline__ unsigned lane_of(const unsigned x, const int l) {
+  return (unsigned)__builtin_amdgcn_readlane((int)x, l);
+}
+__device__ __forceinline__ unsigned long long lane_of(
+    const unsigned long long x, const int l) {
+  return ((unsigned long long)lane_of((unsigned)(x >> 32), l) << 32) |
+         lane_of((unsigned)x, l);
+}
+__device__ __forceinline__ double lane_of(const double x, const int l) {
+  return __longlong_as_double((long long)lane_of(
+      (unsigned long long)__double_as_longlong(x), l));
+}
+
+// Sums up to and with each lane, within rows of 16 lanes or the whole wave.
 template <typename S>
-__device__ __forceinline__ S block_scan(S x, S* lds, S* total) {
-  const int lane = threadIdx.x % WAVE, wid = threadIdx.x / WAVE;
-  S incl = x;
-#pragma unroll
-  for (int off = 1; off < WAVE; off <<= 1) {
-    const S y = __shfl_up(incl, off, WAVE);
-    if (lane >= off) incl += y;
-  }
-  __syncthreads();  // the last user of lds is done
-  if (lane == WAVE - 1) lds[wid] = incl;
-  __syncthreads();
-  S all = lds[lane % NWAVES];
-  S before = lane % NWAVES < wid ? all : (S)0;
-#pragma unroll
-  for (int off = NWAVES / 2; off > 0; off >>= 1) {
-    all += __shfl_xor(all, off, WAVE);
-    before += __shfl_xor(before, off, WAVE);
-  }
-  *total = all;
-  return before + incl - x;
+__device__ __forceinline__ S row_scan(S x) {
+  x += moved<0x111, 0xf>(x);  // from 1, 2, 4, 8 lanes below
+  x += moved<0x112, 0xf>(x);
+  x += moved<0x114, 0xf>(x);
+  x += moved<0x118, 0xf>(x);
+  return x;
+}
+template <typename S>
+__device__ __forceinline__ S wave_scan(S x) {
+  x = row_scan(x);
+  x += moved<0x142, 0xa>(x);  // lane 15 of each row to the next
+  x += moved<0x143, 0xc>(x);  // lane 31 to the upper half
+  return x;
 }
 
 template <typename S>
-__device__ __forceinline__ S block_total(S x, S* lds) {
+__device__ __forceinline__ S block_scan(const S x, S* lds, S* total) {
+  const int lane = threadIdx.x % WAVE;
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+  const S incl = wave_scan(x);
+  __syncthreads();  // the last user of lds is done
+  if (lane == WAVE - 1) lds[wid] = incl;
+  __syncthreads();
+  const S waves = row_scan(lds[lane % NWAVES]);
+  *total = lane_of(waves, NWAVES - 1);
+  const S before = wid > 0 ? lane_of(waves, max(wid - 1, 0)) : (S)0;
+  // and the lane below's sum (not incl - x: no rounding where S is a double)
+  return before + moved<0x138, 0xf>(incl);
+}
+
+template <typename S>
+__device__ __forceinline__ S block_total(const S x, S* lds) {
   const int lane = threadIdx.x % WAVE, wid = threadIdx.x / WAVE;
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, WAVE);
+  const S incl = wave_scan(x);
   __syncthreads();
-  if (lane == 0) lds[wid] = x;
+  if (lane == WAVE - 1) lds[wid] = incl;
   __syncthreads();
-  S all = lds[lane % NWAVES];
-#pragma unroll
-  for (int off = NWAVES / 2; off > 0; off >>= 1)
-    all += __shfl_xor(all, off, WAVE);
-  return all;
+  return lane_of(row_scan(lds[lane % NWAVES]), NWAVES - 1);
 }
 
 __device__ __forceinline__ float block_largest(float x, float* lds) {
@@ -187,7 +220,7 @@ __device__ __forceinline__ float block_largest(float x, float* lds) {
   return x;
 }
 
-// One entry a thread at a time, read (from L2) in every pass.
+// One entry a thread at a time, read again in every pass.
 template <typename T>
 struct Plain {
   const T* row;
@@ -198,30 +231,16 @@ struct Plain {
     else
       return bf2f(row[i]) + 0.f;
   }
-  // f(index, value) of every candidate, AHEAD loads in flight
-  template <int AHEAD, typename F>
-  __device__ __forceinline__ void each(F f) const {
-#pragma unroll 1
-    for (int i = threadIdx.x; i < V; i += BLOCK * AHEAD) {
-      float x[AHEAD];
-#pragma unroll
-      for (int j = 0; j < AHEAD; ++j)
-        x[j] = i + j * BLOCK < V ? at(i + j * BLOCK) : -INFINITY;
-#pragma unroll
-      for (int j = 0; j < AHEAD; ++j)
-        if (candidate(x[j])) f(i + j * BLOCK, x[j]);
-    }
-  }
 };
 
-// A bf16 row in chunks of BLOCK x 16 B: chunk c of thread t is the 8 entries
-// from (c * BLOCK + t) * 8 - lead on, so that every load is aligned whatever
-// the row's start; the first NC chunks stay in registers.  Entries outside
-// the row read as NaN, which is no candidate.
-template <int NC>
+// A row in chunks of BLOCK x 16 B: chunk c of thread t is the PER entries from
+// (c * BLOCK + t) * PER - lead on, so that every load is aligned whatever the
+// row's start; the first NC chunks stay in registers.  Entries outside the
+// row read as NaN, which is no candidate.
+template <typename T, int NC>
 struct Entries {
-  static constexpr int PER = 8;
-  const __hip_bfloat16* row;
+  static constexpr int PER = 16 / sizeof(T);
+  const T* row;
   int V, lead, chunks;
   u32x4 held[NC];
 
@@ -232,19 +251,27 @@ struct Entries {
     const int i = first_of(c);
     if (i >= 0 && i + PER <= V)
       return *reinterpret_cast<const u32x4*>(row + i);
-    u32x4 v = {~0u, ~0u, ~0u, ~0u};  // NaN
-    const unsigned short* src = reinterpret_cast<const unsigned short*>(row);
+    u32x4 v = {~0u, ~0u, ~0u, ~0u};  // NaN in either type
+    if constexpr (sizeof(T) == 4) {
+      const unsigned* src = reinterpret_cast<const unsigned*>(row);
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (i + j >= 0 && i + j < V)
-        v[j / 2] = (j & 1) ? (v[j / 2] & 0xffffu) | ((unsigned)src[i + j] << 16)
-                           : (v[j / 2] & 0xffff0000u) | src[i + j];
+      for (int j = 0; j < 4; ++j)
+        if (i + j >= 0 && i + j < V) v[j] = src[i + j];
+    } else {
+      const unsigned short* src = reinterpret_cast<const unsigned short*>(row);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (i + j >= 0 && i + j < V)
+          v[j / 2] = (j & 1)
+                         ? (v[j / 2] & 0xffffu) | ((unsigned)src[i + j] << 16)
+                         : (v[j / 2] & 0xffff0000u) | src[i + j];
+    }
     return v;
   }
-  __device__ __forceinline__ void open(const __hip_bfloat16* r, const int v) {
+  __device__ __forceinline__ void open(const T* r, const int v) {
     row = r;
     V = v;
-    lead = (int)((reinterpret_cast<uintptr_t>(r) % 16) / 2);
+    lead = (int)((reinterpret_cast<uintptr_t>(r) % 16) / sizeof(T));
     chunks = (V + lead + BLOCK * PER - 1) / (BLOCK * PER);
 #pragma unroll
     for (int c = 0; c < NC; ++c)
@@ -256,18 +283,70 @@ struct Entries {
 #pragma unroll
     for (int c = 0; c < NC; ++c)
       if (c < chunks) f(c, held[c]);
+#pragma unroll 1
     for (int c = NC; c < chunks; ++c) f(c, load(c));
   }
   static __device__ __forceinline__ float get(const u32x4 v, const int j) {
-    return __uint_as_float((j & 1) ? (v[j / 2] & 0xffff0000u)
-                                   : (v[j / 2] << 16));
+    if constexpr (sizeof(T) == 4)
+      return __uint_as_float(v[j]);
+    else
+      return __uint_as_float((j & 1) ? (v[j / 2] & 0xffff0000u)
+                                     : (v[j / 2] << 16));
+  }
+  // whether an entry is x (bf16: two compares a word)
+  static __device__ __forceinline__ bool has(const u32x4 v, const float x) {
+    if constexpr (sizeof(T) == 4) {
+      return get(v, 0) == x || get(v, 1) == x || get(v, 2) == x ||
+             get(v, 3) == x;
+    } else {
+      const unsigned short code = (unsigned short)(__float_as_uint(x) >> 16);
+      const unsigned keep = code ? ~0u : 0x7fff7fffu;  // both zeros
+      bool any = false;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const unsigned w = v[q] & keep;
+        any |= (unsigned short)w == code;
+        any |= (unsigned short)(w >> 16) == code;
+      }
+      return any;
+    }
+  }
+  // each_chunk with one instance of f's code: the held chunks pass through
+  // held[0] and end where they were (a move a register and step).
+  template <typename F>
+  __device__ __forceinline__ void each_chunk_in_turn(F f) {
+#pragma unroll 1
+    for (int c = 0; c < max(NC, chunks); ++c) {
+      u32x4 v = c < NC ? held[0] : load(c);
+      if (c < NC) {
+#pragma unroll
+        for (int k = 0; k + 1 < NC; ++k) held[k] = held[k + 1];
+        held[NC - 1] = v;
+      }
+      f(c, v);
+    }
+  }
+  // f(index, value) of every candidate, -0 as +0, one after the other
+  template <typename F>
+  __device__ __forceinline__ void each(F f) {
+    static_assert(PER == 4, "one word an entry");
+    each_chunk_in_turn([&](const int c, u32x4 v) {
+#pragma unroll 1
+      for (int j = 0; j < PER; ++j) {
+        const float x = get(v, 0) + 0.f;
+        v = (u32x4){v[1], v[2], v[3], v[0]};
+        if (candidate(x)) f(first_of(c) + j, x);
+      }
+    });
   }
 };
 
 struct Shared {
   double pow2[64];
-  double red_d[NWAVES + 1];
-  unsigned long long red_u[NWAVES + 1];
+  double T, top_p, min_p, u;  // in LDS: read where they are asked for
+  double red_d[NWAVES];
+  unsigned long long red_u[NWAVES];
+  unsigned red_n[NWAVES];
   float red_f[NWAVES];
   int flag, hit, at;
   unsigned members;
@@ -275,29 +354,49 @@ struct Shared {
   int per_chunk[MAXCHUNKS];
 };
 
-// The j-th entry, in order of index, whose value is x.
+// The j-th of the n entries, in order of index, whose value is x.  A few are
+// listed as they are met and ranked; of many, the chunks are counted first.
 template <typename E>
-__device__ __forceinline__ int nth_of_value(const E& e, const float x, const int j,
-                            Shared& s) {
+__device__ __forceinline__ int nth_of_value(const E& e, const float x,
+                                            const int j, const int n,
+                                            int* list, Shared& s) {
+  if (threadIdx.x == 0) s.members = 0;
   for (int i = threadIdx.x; i < e.chunks; i += BLOCK) s.per_chunk[i] = 0;
   __syncthreads();
-  e.each_chunk([&](const int c, const u32x4 v) {
-    int n = 0;
+  if (n <= LISTED) {
+    e.each_chunk([&](const int c, const u32x4 v) {
+      if (!e.has(v, x)) return;
 #pragma unroll
-    for (int q = 0; q < E::PER; ++q) n += E::get(v, q) == x;
-    if (n) atomicAdd(&s.per_chunk[c], n);
+      for (int q = 0; q < E::PER; ++q)
+        if (E::get(v, q) == x)
+          list[atomicAdd(&s.members, 1u)] = e.first_of(c) + q;
+    });
+    __syncthreads();
+    if (threadIdx.x < (unsigned)n) {
+      const int mine = list[threadIdx.x];
+      int rank = 0;
+      for (int q = 0; q < n; ++q) rank += list[q] < mine;
+      if (rank == j) s.at = mine;
+    }
+    __syncthreads();
+    return s.at;
+  }
+  e.each_chunk([&](const int c, const u32x4 v) {
+    int here = 0;
+#pragma unroll
+    for (int q = 0; q < E::PER; ++q) here += E::get(v, q) == x;
+    if (here) atomicAdd(&s.per_chunk[c], here);
   });
   __syncthreads();
   int chunk = 0, left = j;
   while (chunk < e.chunks - 1 && left >= s.per_chunk[chunk])
     left -= s.per_chunk[chunk++];
   const u32x4 v = e.load(chunk);
-  int n = 0;
+  unsigned here = 0, all;
 #pragma unroll
-  for (int q = 0; q < E::PER; ++q) n += E::get(v, q) == x;
-  unsigned long long all;
-  int before = (int)block_scan<unsigned long long>(n, s.red_u, &all);
-  if (left >= before && left < before + n) {
+  for (int q = 0; q < E::PER; ++q) here += E::get(v, q) == x;
+  int before = (int)block_scan<unsigned>(here, s.red_n, &all);
+  if (left >= before && left < before + (int)here) {
 #pragma unroll
     for (int q = 0; q < E::PER; ++q)
       if (E::get(v, q) == x && before++ == left) s.at = e.first_of(chunk) + q;
@@ -335,7 +434,7 @@ __device__ __forceinline__ void above(const Plain<T>& e, const Row& r,
     if (candidate(x) && (key > t || (from && key == t))) {
       const double wi = weight(x, r);
       ++cnt;
-      cm += wi >= r.min_p;
+      cm += wi >= s.min_p;
       sum += wi;
     }
   }
@@ -358,11 +457,11 @@ __device__ __forceinline__ Answer general(const Plain<T>& e, const Row& r,
 #pragma unroll 1
   for (int step = -1; step < 4;) {
     if (step == 2) N = max(1ll, min(N, nm));
-    if (step >= 0 && step < 2 && !(r.top_p < 1.0)) {
+    if (step >= 0 && step < 2 && !(s.top_p < 1.0)) {
       ++step;
       continue;
     }
-    const double goal = step == 1 ? r.top_p * Z : r.u * Z;
+    const double goal = step == 1 ? s.top_p * Z : s.u * Z;
     if (step == 1 && !(goal > 0.0)) {
       N = 0;
       ++step;
@@ -421,7 +520,7 @@ __device__ __forceinline__ Answer general(const Plain<T>& e, const Row& r,
     if (left < (int)here) token = s.at;
     left -= (int)here;
   }
-  return {token, (int)N, 0, 0.f};
+  return {token, (int)N, 0, 0, 0.f};
 }
 
 // --------------------------------------------------- bf16: bins are values
@@ -429,118 +528,174 @@ __device__ __forceinline__ Answer general(const Plain<T>& e, const Row& r,
 struct Lds16 {
   union {
     unsigned counts[BINS16];
-    double w[DISTINCT];  // of the list, once it is made
+    struct {  // once the list is made
+      double w[DISTINCT];
+      int ties[LISTED];
+    };
   };
   double before_w[DISTINCT + 1];
   int before_n[DISTINCT + 1];
   unsigned short code[DISTINCT];
+  unsigned places[BINS16 / WAVE];  // what each 64 places hold
   Shared s;
   unsigned zeros, far;
 };
 
-// The list's last entry i for which ok(i), which holds for a prefix of it.
+// Counts the row's values into their bins as its loads arrive: bin =
+// magnitude - LO16, the negative ones 8192 further; as a byte address it is
+// (offset * 4) | sign, in both halves of a word at once.  Words with a value
+// outside the bins are left for a second, rolled loop: written out for every
+// word they would not fit the instruction cache.
+template <int NC>
+__device__ __forceinline__ void count_values(
+    const Entries<__hip_bfloat16, NC>& e, Lds16& L) {
+  using u16x2 = __attribute__((ext_vector_type(2))) unsigned short;
+  const auto offsets = [](const unsigned w) __attribute__((always_inline)) {
+    return __builtin_bit_cast(u16x2, w & 0x7fff7fffu) -
+           (u16x2){(unsigned short)LO16, (unsigned short)LO16};
+  };
+  const auto outside = [](const u16x2 off) __attribute__((always_inline)) {
+    return (__builtin_bit_cast(unsigned, off) & 0xe000e000u) != 0;
+  };
+  unsigned odd = 0;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const unsigned w = e.held[c][q];
+      const u16x2 off = offsets(w);
+      if (outside(off)) {
+        odd |= 1u << c;
+      } else {
+        const unsigned at =
+            __builtin_bit_cast(unsigned, (u16x2)(off << (u16x2){2, 2})) |
+            (w & 0x80008000u);
+        char* base = reinterpret_cast<char*>(L.counts);
+        atomicAdd(reinterpret_cast<unsigned*>(base + (at & 0xffffu)), 1u);
+        atomicAdd(reinterpret_cast<unsigned*>(base + (at >> 16)), 1u);
+      }
+    }
+  }
+#pragma unroll 1
+  for (int c = 0; c < e.chunks; ++c) {
+    const bool all = c >= NC;
+    if (!all && !((odd >> c) & 1)) continue;
+    const u32x4 v = e.load(c);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if (!all && !outside(offsets(v[q]))) continue;
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const unsigned u = (v[q] >> (16 * hf)) & 0xffffu;
+        const unsigned a = u & 0x7fffu;
+        if (a >= (unsigned)LO16 && a < (unsigned)HI16)
+          atomicAdd(&L.counts[(a - LO16) + ((u >> 15) << 13)], 1u);
+        else if (a == 0)
+          atomicAdd(&L.zeros, 1u);
+        else if (a < (unsigned)LO16)
+          L.s.flag = 1;  // magnitudes below 2^-41
+        else if (u > 0x8000u && a < 0x7f80u)
+          atomicAdd(&L.far, 1u);  // finite, -2^23 or less
+      }
+    }
+  }
+}
+
+// The list's last entry i for which ok(i), which holds for a prefix of it (0
+// if for none).  Two rounds of 64 probes, the same in every wave.
 template <typename F>
-__device__ __forceinline__ int last_entry(const int entries, Shared& s, F ok) {
-  __syncthreads();
-  if (threadIdx.x == 0) s.hit = 0;
-  __syncthreads();
-  for (int i = threadIdx.x; i < entries; i += BLOCK)
-    if (ok(i) && (i + 1 == entries || !ok(i + 1))) atomicMax(&s.hit, i);
-  __syncthreads();
-  return s.hit;
+__device__ __forceinline__ int last_entry(const int entries, F ok) {
+  static_assert(DISTINCT <= 64 * 64, "two rounds");
+  const int lane = threadIdx.x % WAVE;
+  const int step = (entries + 63) / 64;
+  int i = lane * step;
+  unsigned long long yes = __ballot(i < entries && ok(i));
+  if (yes == 0) return 0;
+  const int base = (63 - __clzll((long long)yes)) * step;
+  i = base + lane;
+  yes = __ballot(lane < step && i < entries && ok(i));
+  return base + 63 - __clzll((long long)yes);
 }
 
 // Both row functions say false where the general search has to take the row.
 template <int NC>
-__device__ __forceinline__ bool bf16_row(const Entries<NC>& e,
+__device__ __forceinline__ bool bf16_row(const Entries<__hip_bfloat16, NC>& e,
                                         const Row& r, Lds16& L, Answer& ans) {
   Shared& s = L.s;
   const int tid = threadIdx.x;
-  for (int i = tid; i < BINS16 / 4; i += BLOCK)
-    reinterpret_cast<uint4*>(L.counts)[i] = make_uint4(0, 0, 0, 0);
-  if (tid == 0) L.zeros = L.far = s.flag = 0;
-  __syncthreads();
-
-  // bin = magnitude - LO16, the negative ones 8192 further: as a byte
-  // address it is (offset * 4) | sign, in both halves of a word at once
-  e.each_chunk([&](int, const u32x4 v) {
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      using u16x2 = __attribute__((ext_vector_type(2))) unsigned short;
-      const unsigned mag = v[q] & 0x7fff7fffu;
-      const u16x2 off = __builtin_bit_cast(u16x2, mag) -
-                        (u16x2){(unsigned short)LO16, (unsigned short)LO16};
-      const unsigned offs = __builtin_bit_cast(unsigned, off);
-      if ((offs & 0xe000e000u) == 0) {
-        const u16x2 by4 = off << (u16x2){2, 2};
-        const unsigned at =
-            __builtin_bit_cast(unsigned, by4) | (v[q] & 0x80008000u);
-        char* base = reinterpret_cast<char*>(L.counts);
-        atomicAdd(reinterpret_cast<unsigned*>(base + (at & 0xffffu)), 1u);
-        atomicAdd(reinterpret_cast<unsigned*>(base + (at >> 16)), 1u);
-      } else {
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          const unsigned u = (v[q] >> (16 * hf)) & 0xffffu;
-          const unsigned a = u & 0x7fffu;
-          if (a >= (unsigned)LO16 && a < (unsigned)HI16)
-            atomicAdd(&L.counts[(a - LO16) + ((u >> 15) << 13)], 1u);
-          else if (a == 0)
-            atomicAdd(&L.zeros, 1u);
-          else if (a < (unsigned)LO16)
-            s.flag = 1;  // magnitudes below 2^-41
-          else if (u > 0x8000u && a < 0x7f80u)
-            atomicAdd(&L.far, 1u);  // finite, -2^23 or less
-        }
-      }
-    }
-  });
-  __syncthreads();
+  const int lane = tid % WAVE, wid = tid / WAVE;
   // far values have to weigh nothing: exp(-746) is 0 in 64 bits
   if (s.flag || r.m >= -FAR_VALUE ||
-      (L.far && (double)r.m - (double)FAR_VALUE < 746.0 * r.T))
+      (L.far && (double)r.m - (double)FAR_VALUE < 746.0 * s.T))
     return false;
 
-  // ---- the list of distinct values, falling: thread t looks at places
-  // 16 t .., the positive values from the largest down, zero, the negative
-  const auto count_at = [&](const int p) __attribute__((always_inline)) {
-    return L.counts[p < BINS16 / 2 ? BINS16 / 2 - 1 - p : p];
+  // ---- the list of distinct values, falling.  Place p is the positive
+  // values from the largest down, then (from BINS16 / 2, after the zeros) the
+  // negative ones.  A wave takes 64 places at a time, so that the few hundred
+  // neighbours that hold nearly all values are shared among the waves.
+  constexpr int ROUNDS = BINS16 / BLOCK;
+  const auto bin_at = [](const int p) __attribute__((always_inline)) {
+    return p < BINS16 / 2 ? BINS16 / 2 - 1 - p : p;
   };
-  unsigned n = 0, distinct = 0;
-  const bool mid = tid == BLOCK / 2;  // the zeros come right before it
+  // how many values (up to 2^20) and, from bit 21 on, how many distinct
+  constexpr unsigned ONE = 1u << 21;
 #pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    const unsigned c = count_at(tid * 16 + j);
-    n += c;
-    distinct += c != 0;
+  for (int k = 0; k < ROUNDS; ++k) {
+    const unsigned c = L.counts[bin_at(k * BLOCK + tid)];
+    unsigned sum = 0;
+    if (__any(c != 0)) sum = lane_of(wave_scan(c ? c + ONE : 0u), WAVE - 1);
+    if (lane == 0) L.places[k * NWAVES + wid] = sum;
   }
-  if (mid && L.zeros) {
-    n += L.zeros;
-    ++distinct;
+  __syncthreads();
+  // the groups of 64 places before each (4 a lane, the same in every wave)
+  constexpr int GROUPS = BINS16 / WAVE / WAVE;
+  static_assert(GROUPS == 4, "one 16 B read a lane");
+  const u32x4 g = reinterpret_cast<const u32x4*>(L.places)[lane];
+  unsigned gn = 0, gd = 0;
+#pragma unroll
+  for (int q = 0; q < GROUPS; ++q) {
+    gn += g[q] & (ONE - 1);
+    gd += g[q] >> 21;
   }
-  unsigned long long total;
-  const unsigned long long pre = block_scan<unsigned long long>(
-      ((unsigned long long)distinct << 32) | n, s.red_u, &total);
-  const int entries = (int)(total >> 32);
-  const int listed = (int)(total & 0xffffffffu);
+  const unsigned zeros = L.zeros;
+  const unsigned un = wave_scan(gn), ud = wave_scan(gd);
+  const int entries = (int)lane_of(ud, WAVE - 1) + (zeros != 0);
+  const int listed = (int)(lane_of(un, WAVE - 1) + zeros);
   if (entries > DISTINCT) return false;
-  int at = (int)(pre >> 32);
-  int seen = (int)(pre & 0xffffffffu);
-  if (mid && L.zeros) {
-    L.code[at] = 0;
-    L.before_n[at++] = seen;
-    seen += L.zeros;
+#pragma unroll 1
+  for (int k = 0; k < ROUNDS; ++k) {
+    const int group = k * NWAVES + __builtin_amdgcn_readfirstlane(wid);
+    const unsigned here = L.places[group];
+    if (here == 0) continue;
+    // before the group: the lanes below its, and the groups before it there
+    unsigned n = lane_of(un - gn, group / GROUPS);
+    unsigned d = lane_of(ud - gd, group / GROUPS);
+#pragma unroll
+    for (int q = 0; q < GROUPS - 1; ++q)
+      if (q < group % GROUPS) {
+        const unsigned x = lane_of(g[q], group / GROUPS);
+        n += x & (ONE - 1);
+        d += x >> 21;
+      }
+    const int p = k * BLOCK + tid;
+    if (p >= BINS16 / 2) {
+      n += zeros;
+      d += zeros != 0;
+    }
+    const unsigned c = L.counts[bin_at(p)];
+    const unsigned upto = wave_scan(c ? c + ONE : 0u);
+    if (c) {
+      const unsigned at = d + (upto >> 21) - 1;
+      L.before_n[at] = (int)(n + (upto & (ONE - 1)) - c);
+      L.code[at] = (unsigned short)(p < BINS16 / 2
+                                        ? LO16 + BINS16 / 2 - 1 - p
+                                        : 0x8000 | (LO16 + p - BINS16 / 2));
+    }
   }
-#pragma unroll 4
-  for (int j = 0; j < 16; ++j) {
-    const int p = tid * 16 + j;
-    const unsigned c = count_at(p);
-    if (c == 0) continue;
-    L.code[at] = (unsigned short)(
-        p < BINS16 / 2 ? LO16 + BINS16 / 2 - 1 - p
-                       : (0x8000 | (LO16 + p - BINS16 / 2)));
-    L.before_n[at++] = seen;
-    seen += c;
+  if (zeros && tid == 0) {  // after lane 31's groups, the positive ones
+    const int at = (int)lane_of(ud, 31);
+    L.code[at] = 0;
+    L.before_n[at] = (int)lane_of(un, 31);
   }
   if (tid == 0) L.before_n[entries] = listed;
   __syncthreads();  // counts are done with: w takes their place
@@ -576,37 +731,37 @@ __device__ __forceinline__ bool bf16_row(const Entries<NC>& e,
   const auto sum_first = [&](const int n) __attribute__((always_inline)) {
     if (n >= listed) return w_all;
     const int i =
-        last_entry(entries, s, [&](int i) { return L.before_n[i] < n; });
+        last_entry(entries, [&](int i) { return L.before_n[i] < n; });
     return L.before_w[i] + (double)(n - L.before_n[i]) * L.w[i];
   };
   const int all = listed + (int)L.far;
   int N = min(r.k, all);
   double Z = sum_first(N);
-  if (r.top_p < 1.0) {
-    const double goal = r.top_p * Z;
+  if (s.top_p < 1.0) {
+    const double goal = s.top_p * Z;
     int np = 0;
     if (goal > 0.0) {
       const int i =
-          last_entry(entries, s, [&](int i) { return L.before_w[i] < goal; });
+          last_entry(entries, [&](int i) { return L.before_w[i] < goal; });
       np = L.before_n[i] + within(goal, L.before_w[i], L.w[i],
                                   L.before_n[i + 1] - L.before_n[i], false);
     }
     N = min(N, np);
   }
-  if (!(r.min_p <= 0.0)) {
+  if (!(s.min_p <= 0.0)) {
     const int i =
-        last_entry(entries, s, [&](int i) { return L.w[i] >= r.min_p; });
-    N = min(N, L.w[i] >= r.min_p ? L.before_n[i + 1] : 0);
+        last_entry(entries, [&](int i) { return L.w[i] >= s.min_p; });
+    N = min(N, L.w[i] >= s.min_p ? L.before_n[i + 1] : 0);
   }
   N = max(N, 1);
-  const double goal = r.u * sum_first(N);
+  const double goal = s.u * sum_first(N);
   const int i =
-      last_entry(entries, s, [&](int i) { return L.before_w[i] <= goal; });
+      last_entry(entries, [&](int i) { return L.before_w[i] <= goal; });
   int j = within(goal, L.before_w[i], L.w[i],
                  L.before_n[i + 1] - L.before_n[i] - 1, true);
   j = max(0, min(j, N - 1 - L.before_n[i]));
   const float x = __uint_as_float((unsigned)L.code[i] << 16) + 0.f;
-  ans = {-1, N, j, x};
+  ans = {-1, N, j, L.before_n[i + 1] - L.before_n[i], x};
   return true;
 }
 
@@ -622,22 +777,23 @@ struct Lds32 {
   Shared s;
 };
 
-__device__ __forceinline__ bool fp32_row(const Plain<float>& e, const Row& r,
+template <int NC>
+__device__ __forceinline__ bool fp32_row(Entries<float, NC>& e, const Row& r,
                                         Lds32& L, Answer& ans) {
   constexpr int PT = BINS32 / BLOCK;  // bins of a thread, in order
   Shared& s = L.s;
   const int tid = threadIdx.x;
-  for (int i = tid; i < BINS32; i += BLOCK) {
-    L.w[i] = 0;
-    L.n[i] = 0;
-  }
   if (r.m == INFINITY) return false;
   // values that weigh nothing (exp(-746) is 0 in 64 bits) are counted alone;
   // the bins cover the others
-  const double reach = 746.0 * r.T;
+  const float cut = __double2float_rd((double)r.m - 746.0 * s.T);
   float low = r.m;
-  e.template each<8>([&](int, const float x) {
-    if ((double)r.m - (double)x <= reach) low = fminf(low, x);
+  e.each_chunk([&](int, const u32x4 v) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float x = e.get(v, j);
+      low = x >= cut && candidate(x) ? fminf(low, x) : low;
+    }
   });
   low = -block_largest(-low, s.red_f);
   const float span = r.m - low;
@@ -649,17 +805,17 @@ __device__ __forceinline__ bool fp32_row(const Plain<float>& e, const Row& r,
     return min(BINS32 - 1, (int)((r.m - x) * by));
   };
   unsigned long long nm = 0, far = 0;
-  e.template each<2>([&](int, const float x) {
+  e.each([&](int, const float x) {
     if (x < low) {
       ++far;
-      nm += 0.0 >= r.min_p;
+      nm += 0.0 >= s.min_p;
       return;
     }
     const double w = weight(x, r);
     const int b = bin_of(x);
     atomicAdd(&L.w[b], (unsigned long long)(w * FIXED + 0.5));
     atomicAdd(&L.n[b], 1u);
-    nm += w >= r.min_p;
+    nm += w >= s.min_p;
   });
   far = block_total<unsigned long long>(far, s.red_u);
   nm = block_total<unsigned long long>(nm, s.red_u);
@@ -687,13 +843,13 @@ __device__ __forceinline__ bool fp32_row(const Plain<float>& e, const Row& r,
 #pragma unroll 1
   for (int step = 0; step < 4; ++step) {
     if (step == 2) N = max(1ll, min(N, (long long)nm));
-    if (step < 2 && !(r.top_p < 1.0)) continue;
+    if (step < 2 && !(s.top_p < 1.0)) continue;
     bool by_count = (step & 1) == 0;
     if (by_count && N >= (long long)listed) {
       Z = w_all;
       continue;
     }
-    const double goal = step == 1 ? r.top_p * Z : r.u * Z;
+    const double goal = step == 1 ? s.top_p * Z : s.u * Z;
     if (step == 1 && !(goal > 0.0)) {
       N = 0;
       continue;
@@ -742,11 +898,15 @@ __device__ __forceinline__ bool fp32_row(const Plain<float>& e, const Row& r,
       if (members > MEMBERS) return false;
       if (tid == 0) s.members = 0;
       __syncthreads();
-      e.template each<8>([&](const int i, const float x) {
-        if (x >= low && bin_of(x) == bin) {
-          const unsigned p = atomicAdd(&s.members, 1u);
-          L.key[p] = key_of(x);
-          L.index[p] = i;
+      e.each_chunk_in_turn([&](const int c, const u32x4 v) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float x = e.get(v, j) + 0.f;
+          if (x >= low && bin_of(x) == bin) {
+            const unsigned p = atomicAdd(&s.members, 1u);
+            L.key[p] = key_of(x);
+            L.index[p] = e.first_of(c) + j;
+          }
         }
       });
       __syncthreads();
@@ -754,6 +914,7 @@ __device__ __forceinline__ bool fp32_row(const Plain<float>& e, const Row& r,
         const unsigned key = L.key[p];
         const int i = L.index[p];
         int rank_in = 0;
+#pragma unroll 4
         for (int q = 0; q < members; ++q) {
           const unsigned k2 = L.key[q];
           rank_in += k2 > key || (k2 == key && L.index[q] < i);
@@ -790,8 +951,16 @@ __device__ __forceinline__ bool fp32_row(const Plain<float>& e, const Row& r,
       token = L.sorted_index[(int)min((long long)min((int)n, members - 1),
                                       N - 1 - before_n)];
   }
-  ans = {token, (int)N, 0, 0.f};
+  ans = {token, (int)N, 0, 0, 0.f};
   return true;
+}
+
+// A value that is the same in all lanes, kept in scalar registers.
+__device__ __forceinline__ double uniform_of(const double x) {
+  const long long u = __double_as_longlong(x);
+  const int lo = __builtin_amdgcn_readfirstlane((int)(u & 0xffffffffll));
+  const int hi = __builtin_amdgcn_readfirstlane((int)(u >> 32));
+  return __longlong_as_double(((long long)hi << 32) | (unsigned)lo);
 }
 
 // What is the row's filters' apart from its logits; false: not asked for.
@@ -800,12 +969,15 @@ __device__ __forceinline__ bool open_row(const Args& a, const int b, Row& r,
   const float u = a.uniform[b];
   if (u < 0.f) return false;
   const int k = a.top_k[b];
-  r.T = (double)a.temperature[b];
-  r.inv_T = 1.0 / r.T;
+  const double T = uniform_of((double)a.temperature[b]);
+  r.inv_T = uniform_of(1.0 / T);
   r.k = (k > 0 && k < a.V) ? k : a.V;
-  r.top_p = (double)a.top_p[b];
-  r.min_p = (double)a.min_p[b];
-  r.u = fmin((double)u, 1.0 - 0x1p-53);  // [0, 1); NaN too
+  if (threadIdx.x == 0) {  // seen after the first block-wide step
+    s.T = T;
+    s.top_p = (double)a.top_p[b];
+    s.min_p = (double)a.min_p[b];
+    s.u = fmin((double)u, 1.0 - 0x1p-53);  // [0, 1); NaN too
+  }
   r.pow2 = s.pow2;
   if (threadIdx.x < 64) s.pow2[threadIdx.x] = POW2_64TH[threadIdx.x];
   return true;
@@ -819,68 +991,76 @@ __device__ __forceinline__ void answer(const Args& a, const int b,
   }
 }
 
-template <int NC>
-__global__ __launch_bounds__(BLOCK) void sample_filtered_bf16_kernel(
-    const Args a) {
-  __shared__ __attribute__((aligned(16))) Lds16 L;
+template <typename T>
+struct LdsOf;
+template <>
+struct LdsOf<__hip_bfloat16> {
+  using type = Lds16;
+};
+template <>
+struct LdsOf<float> {
+  using type = Lds32;
+};
+
+__device__ __forceinline__ void clear(Lds16& L) {
+  for (int i = threadIdx.x; i < BINS16 / 4; i += BLOCK)
+    reinterpret_cast<u32x4*>(L.counts)[i] = (u32x4){0, 0, 0, 0};
+  if (threadIdx.x == 0) L.zeros = L.far = L.s.flag = 0;
+}
+__device__ __forceinline__ void clear(Lds32& L) {
+  for (int i = threadIdx.x; i < BINS32 / 2; i += BLOCK)
+    reinterpret_cast<u32x4*>(L.w)[i] = (u32x4){0, 0, 0, 0};
+  for (int i = threadIdx.x; i < BINS32 / 4; i += BLOCK)
+    reinterpret_cast<u32x4*>(L.n)[i] = (u32x4){0, 0, 0, 0};
+}
+__device__ __forceinline__ int* ties_of(Lds16& L) { return L.ties; }
+__device__ __forceinline__ int* ties_of(Lds32& L) { return L.index; }
+
+// A barrier that waits for LDS alone: the row's loads stay in flight.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+template <typename T, int NC>
+__global__ __launch_bounds__(BLOCK) void sample_filtered_kernel(const Args a) {
+  __shared__ __attribute__((aligned(16))) typename LdsOf<T>::type L;
   const int b = blockIdx.x;
   Row r;
   if (!open_row(a, b, r, L.s)) return;  // out and kept stay as they were
-  const __hip_bfloat16* row =
-      reinterpret_cast<const __hip_bfloat16*>(a.logits) + (int64_t)b * a.V;
-  Entries<NC> e;
-  e.open(row, a.V);
+  const T* row = reinterpret_cast<const T*>(a.logits) + (int64_t)b * a.V;
+  Entries<T, NC> e;
+  e.open(row, a.V);  // under the loads' flight:
+  const bool warm = (double)a.temperature[b] > 0.0;
+  clear(L);
+  lds_barrier();
+  if constexpr (sizeof(T) == 2)
+    if (warm) count_values(e, L);
   float m = -INFINITY;
   e.each_chunk([&](int, const u32x4 v) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m = fmaxf(m, e.get(v, j));  // not a NaN
+    for (int j = 0; j < e.PER; ++j) m = fmaxf(m, e.get(v, j));  // not a NaN
   });
-  r.m = block_largest(m, L.s.red_f) + 0.f;
-  Answer ans{0, 1, 0, 0.f};  // no candidate: token 0
-  bool done = true;          // the same in all threads
+  r.m = __uint_as_float(__builtin_amdgcn_readfirstlane(
+      __float_as_uint(block_largest(m, L.s.red_f) + 0.f)));
+  Answer ans{0, 1, 0, 0, 0.f};  // no candidate: token 0
+  bool done = true;             // the same in all threads
   if (r.m > -INFINITY) {
-    ans = {-1, 1, 0, r.m};  // T <= 0: the first of the largest
-    if (r.T > 0.0) done = bf16_row(e, r, L, ans);
+    ans = {-1, 1, 0, 1 << 30, r.m};  // T <= 0: the first of the largest
+    if (warm) {
+      if constexpr (sizeof(T) == 2)
+        done = bf16_row(e, r, L, ans);
+      else
+        done = fp32_row(e, r, L, ans);
+    }
   }
   // (known to be uniform, neither branch keeps the other's registers)
   if (!__builtin_amdgcn_readfirstlane(done)) {
     __syncthreads();
-    ans = general(Plain<__hip_bfloat16>{row, a.V}, r, L.s);
+    ans = general(Plain<T>{row, a.V}, r, L.s);
   } else if (__builtin_amdgcn_readfirstlane(ans.token) < 0) {
-    ans.token = nth_of_value(e, ans.x, ans.nth, L.s);
-  }
-  answer(a, b, ans.token, ans.kept);
-}
-
-__global__ __launch_bounds__(BLOCK) void sample_filtered_fp32_kernel(
-    const Args a) {
-  __shared__ __attribute__((aligned(16))) Lds32 L;
-  const int b = blockIdx.x;
-  Row r;
-  if (!open_row(a, b, r, L.s)) return;
-  const Plain<float> e{
-      reinterpret_cast<const float*>(a.logits) + (int64_t)b * a.V, a.V};
-  float m = -INFINITY;
-  e.template each<8>([&](int, const float x) { m = fmaxf(m, x); });
-  r.m = block_largest(m, L.s.red_f);
-  Answer ans{0, 1, 0, 0.f};
-  bool done = true;
-  if (r.m > -INFINITY) {
-    if (r.T > 0.0) {
-      done = fp32_row(e, r, L, ans);
-    } else {
-      if (threadIdx.x == 0) L.s.at = a.V;
-      __syncthreads();
-      e.template each<8>([&](const int i, const float x) {
-        if (x == r.m) atomicMin(&L.s.at, i);
-      });
-      __syncthreads();
-      ans.token = L.s.at;
-    }
-  }
-  if (!__builtin_amdgcn_readfirstlane(done)) {
-    __syncthreads();
-    ans = general(e, r, L.s);
+    ans.token = nth_of_value(e, ans.x, ans.nth, ans.ties, ties_of(L), L.s);
   }
   answer(a, b, ans.token, ans.kept);
 }
@@ -929,14 +1109,16 @@ void sample_filtered(torch::Tensor out, torch::Tensor logits,
                (const float*)min_p.data_ptr(),
                (const float*)uniform.data_ptr(),
                (int)V};
-  // a bf16 row's first 64 KB or 256 KB stay in registers, the rest is read
-  // again; fp32 rows are read from L2 in every pass
+  // what a row has beyond the registers' 64 KB, 128 KB or 256 KB is read again
   const dim3 grid((unsigned)B), block(BLOCK);
+#define LAUNCH(T, NC)                                                         \
+  hipLaunchKernelGGL((sample_filtered_kernel<T, NC>), grid, block, 0, s, a)
   if (logits.scalar_type() == torch::kFloat32)
-    hipLaunchKernelGGL(sample_filtered_fp32_kernel, grid, block, 0, s, a);
+    LAUNCH(float, 8);
   else if (V * 2 <= 65536 - 16)
-    hipLaunchKernelGGL((sample_filtered_bf16_kernel<4>), grid, block, 0, s, a);
+    LAUNCH(__hip_bfloat16, 4);
   else
-    hipLaunchKernelGGL((sample_filtered_bf16_kernel<16>), grid, block, 0, s, a);
+    LAUNCH(__hip_bfloat16, 16);
+#undef LAUNCH
   HIP_CHECK_LAST();
 }
