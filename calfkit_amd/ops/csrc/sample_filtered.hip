@@ -293,48 +293,52 @@ struct Entries {
       return __uint_as_float((j & 1) ? (v[j / 2] & 0xffff0000u)
                                      : (v[j / 2] << 16));
   }
-  // whether an entry is x (bf16: two compares a word)
+  // whether an entry is x
   static __device__ __forceinline__ bool has(const u32x4 v, const float x) {
     if constexpr (sizeof(T) == 4) {
       return get(v, 0) == x || get(v, 1) == x || get(v, 2) == x ||
              get(v, 3) == x;
     } else {
-      const unsigned short code = (unsigned short)(__float_as_uint(x) >> 16);
+      using u16x2 = __attribute__((ext_vector_type(2))) unsigned short;
+      const unsigned code = __float_as_uint(x) >> 16;
       const unsigned keep = code ? ~0u : 0x7fff7fffu;  // both zeros
-      bool any = false;
+      u16x2 least = {0xffff, 0xffff};
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const unsigned w = v[q] & keep;
-        any |= (unsigned short)w == code;
-        any |= (unsigned short)(w >> 16) == code;
-      }
-      return any;
+      for (int q = 0; q < 4; ++q)
+        least = __builtin_elementwise_min(
+            least, __builtin_bit_cast(
+                       u16x2, (v[q] ^ (code | code << 16)) & keep));
+      return least[0] == 0 || least[1] == 0;
     }
   }
-  // each_chunk with one instance of f's code: the held chunks pass through
-  // held[0] and end where they were (a move a register and step).
-  template <typename F>
+  // each_chunk with TURN instances of f's code: the held chunks pass through
+  // the first TURN places and end where they were (a move a register and turn).
+  template <int TURN, typename F>
   __device__ __forceinline__ void each_chunk_in_turn(F f) {
+    static_assert(NC % TURN == 0, "whole turns");
 #pragma unroll 1
-    for (int c = 0; c < max(NC, chunks); ++c) {
-      u32x4 v = c < NC ? held[0] : load(c);
-      if (c < NC) {
+    for (int c = 0; c < NC; c += TURN) {
+      u32x4 now[TURN];
 #pragma unroll
-        for (int k = 0; k + 1 < NC; ++k) held[k] = held[k + 1];
-        held[NC - 1] = v;
-      }
-      f(c, v);
+      for (int k = 0; k < TURN; ++k) now[k] = held[k];
+#pragma unroll
+      for (int k = 0; k + TURN < NC; ++k) held[k] = held[k + TURN];
+#pragma unroll
+      for (int k = 0; k < TURN; ++k) held[NC - TURN + k] = now[k];
+#pragma unroll
+      for (int k = 0; k < TURN; ++k) f(c + k, now[k]);
     }
+#pragma unroll 1
+    for (int c = NC; c < chunks; ++c) f(c, load(c));
   }
   // f(index, value) of every candidate, -0 as +0, one after the other
   template <typename F>
   __device__ __forceinline__ void each(F f) {
     static_assert(PER == 4, "one word an entry");
-    each_chunk_in_turn([&](const int c, u32x4 v) {
-#pragma unroll 1
+    each_chunk_in_turn<1>([&](const int c, u32x4 v) {
+#pragma unroll
       for (int j = 0; j < PER; ++j) {
-        const float x = get(v, 0) + 0.f;
-        v = (u32x4){v[1], v[2], v[3], v[0]};
+        const float x = get(v, j) + 0.f;
         if (candidate(x)) f(first_of(c) + j, x);
       }
     });
@@ -537,6 +541,7 @@ struct Lds16 {
   int before_n[DISTINCT + 1];
   unsigned short code[DISTINCT];
   unsigned places[BINS16 / WAVE];  // what each 64 places hold
+  uint2 before[BINS16 / WAVE];     // and what lies before them
   Shared s;
   unsigned zeros, far;
 };
@@ -639,15 +644,18 @@ __device__ __forceinline__ bool bf16_row(const Entries<__hip_bfloat16, NC>& e,
   };
   // how many values (up to 2^20) and, from bit 21 on, how many distinct
   constexpr unsigned ONE = 1u << 21;
+  unsigned c[ROUNDS], incl[ROUNDS];
+#pragma unroll
+  for (int k = 0; k < ROUNDS; ++k) c[k] = L.counts[bin_at(k * BLOCK + tid)];
 #pragma unroll
   for (int k = 0; k < ROUNDS; ++k) {
-    const unsigned c = L.counts[bin_at(k * BLOCK + tid)];
-    unsigned sum = 0;
-    if (__any(c != 0)) sum = lane_of(wave_scan(c ? c + ONE : 0u), WAVE - 1);
-    if (lane == 0) L.places[k * NWAVES + wid] = sum;
+    incl[k] = c[k] ? c[k] + ONE : 0u;
+    if (__any(c[k] != 0)) incl[k] = wave_scan(incl[k]);
+    if (lane == WAVE - 1) L.places[k * NWAVES + wid] = incl[k];
   }
   __syncthreads();
-  // the groups of 64 places before each (4 a lane, the same in every wave)
+  // what lies before each group of 64 places: 4 groups a lane, the same in
+  // every wave
   constexpr int GROUPS = BINS16 / WAVE / WAVE;
   static_assert(GROUPS == 4, "one 16 B read a lane");
   const u32x4 g = reinterpret_cast<const u32x4*>(L.places)[lane];
@@ -662,31 +670,27 @@ __device__ __forceinline__ bool bf16_row(const Entries<__hip_bfloat16, NC>& e,
   const int entries = (int)lane_of(ud, WAVE - 1) + (zeros != 0);
   const int listed = (int)(lane_of(un, WAVE - 1) + zeros);
   if (entries > DISTINCT) return false;
-#pragma unroll 1
-  for (int k = 0; k < ROUNDS; ++k) {
-    const int group = k * NWAVES + __builtin_amdgcn_readfirstlane(wid);
-    const unsigned here = L.places[group];
-    if (here == 0) continue;
-    // before the group: the lanes below its, and the groups before it there
-    unsigned n = lane_of(un - gn, group / GROUPS);
-    unsigned d = lane_of(ud - gd, group / GROUPS);
-#pragma unroll
-    for (int q = 0; q < GROUPS - 1; ++q)
-      if (q < group % GROUPS) {
-        const unsigned x = lane_of(g[q], group / GROUPS);
-        n += x & (ONE - 1);
-        d += x >> 21;
-      }
-    const int p = k * BLOCK + tid;
-    if (p >= BINS16 / 2) {
+  if (wid == 0) {
+    unsigned n = un - gn, d = ud - gd;
+    if (lane >= 32) {  // the negative places follow the zeros
       n += zeros;
       d += zeros != 0;
     }
-    const unsigned c = L.counts[bin_at(p)];
-    const unsigned upto = wave_scan(c ? c + ONE : 0u);
-    if (c) {
-      const unsigned at = d + (upto >> 21) - 1;
-      L.before_n[at] = (int)(n + (upto & (ONE - 1)) - c);
+#pragma unroll
+    for (int q = 0; q < GROUPS; ++q) {
+      L.before[lane * GROUPS + q] = make_uint2(n, d);
+      n += g[q] & (ONE - 1);
+      d += g[q] >> 21;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < ROUNDS; ++k) {
+    if (c[k]) {
+      const uint2 base = L.before[k * NWAVES + wid];
+      const int p = k * BLOCK + tid;
+      const unsigned at = base.y + (incl[k] >> 21) - 1;
+      L.before_n[at] = (int)(base.x + (incl[k] & (ONE - 1)) - c[k]);
       L.code[at] = (unsigned short)(p < BINS16 / 2
                                         ? LO16 + BINS16 / 2 - 1 - p
                                         : 0x8000 | (LO16 + p - BINS16 / 2));
@@ -813,7 +817,10 @@ __device__ __forceinline__ bool fp32_row(Entries<float, NC>& e, const Row& r,
     }
     const double w = weight(x, r);
     const int b = bin_of(x);
-    atomicAdd(&L.w[b], (unsigned long long)(w * FIXED + 0.5));
+    // the sum with 2^52 has the rounded integer for its mantissa
+    atomicAdd(&L.w[b], (unsigned long long)__double_as_longlong(
+                           fma(w, FIXED, 0x1p52)) &
+                           ((1ull << 52) - 1));
     atomicAdd(&L.n[b], 1u);
     nm += w >= s.min_p;
   });
@@ -822,10 +829,14 @@ __device__ __forceinline__ bool fp32_row(Entries<float, NC>& e, const Row& r,
   __syncthreads();
 
   unsigned long long tw = 0, tn = 0, w_fix, listed;
+  unsigned long long binw[PT];
+  unsigned binn[PT];
 #pragma unroll
   for (int j = 0; j < PT; ++j) {
-    tw += L.w[tid * PT + j];
-    tn += L.n[tid * PT + j];
+    binw[j] = L.w[tid * PT + j];
+    binn[j] = L.n[tid * PT + j];
+    tw += binw[j];
+    tn += binn[j];
   }
   const unsigned long long bw = block_scan<unsigned long long>(tw, s.red_u,
                                                                &w_fix);
@@ -862,17 +873,17 @@ __device__ __forceinline__ bool fp32_row(Entries<float, NC>& e, const Row& r,
       if (tid == 0) s.hit = -1;
       __syncthreads();
       unsigned long long cw = bw, cn = bn;
-#pragma unroll 1
-      for (int b = tid * PT; b < tid * PT + PT; ++b) {
-        const unsigned n = L.n[b];
-        const unsigned long long ew = cw + L.w[b], en = cn + n;
+#pragma unroll
+      for (int j = 0; j < PT; ++j) {
+        const unsigned n = binn[j];
+        const unsigned long long ew = cw + binw[j], en = cn + n;
         const double d0 = (double)cw * (1.0 / FIXED);
         const double d1 = (double)ew * (1.0 / FIXED);
         if (n != 0 &&
             (by_count    ? ((long long)cn < rank && (long long)en >= rank)
              : step == 1 ? (d0 < goal && d1 >= goal)
                          : (d0 <= goal && d1 > goal))) {
-          s.hit = b;
+          s.hit = tid * PT + j;
           s.at = (int)cn;
           s.hit_before = d0;
         }
@@ -898,7 +909,7 @@ __device__ __forceinline__ bool fp32_row(Entries<float, NC>& e, const Row& r,
       if (members > MEMBERS) return false;
       if (tid == 0) s.members = 0;
       __syncthreads();
-      e.each_chunk_in_turn([&](const int c, const u32x4 v) {
+      e.template each_chunk_in_turn<2>([&](const int c, const u32x4 v) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const float x = e.get(v, j) + 0.f;
@@ -966,16 +977,18 @@ __device__ __forceinline__ double uniform_of(const double x) {
 // What is the row's filters' apart from its logits; false: not asked for.
 __device__ __forceinline__ bool open_row(const Args& a, const int b, Row& r,
                                          Shared& s) {
-  const float u = a.uniform[b];
-  if (u < 0.f) return false;
+  // all at once: one latency, not one behind the other
+  const float u = a.uniform[b], t = a.temperature[b], p = a.top_p[b],
+              q = a.min_p[b];
   const int k = a.top_k[b];
-  const double T = uniform_of((double)a.temperature[b]);
+  if (u < 0.f) return false;
+  const double T = uniform_of((double)t);
   r.inv_T = uniform_of(1.0 / T);
   r.k = (k > 0 && k < a.V) ? k : a.V;
   if (threadIdx.x == 0) {  // seen after the first block-wide step
     s.T = T;
-    s.top_p = (double)a.top_p[b];
-    s.min_p = (double)a.min_p[b];
+    s.top_p = (double)p;
+    s.min_p = (double)q;
     s.u = fmin((double)u, 1.0 - 0x1p-53);  // [0, 1); NaN too
   }
   r.pow2 = s.pow2;
