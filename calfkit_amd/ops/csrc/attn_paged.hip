@@ -90,7 +90,8 @@ struct Paged {
   int64_t q_stride;
   int B, hq, hkv, G, max_pages, num_pages, ngroups;
   int nshared, nsplit;  // partial slots of the prefix and of the rest
-  float scale_log2;     // scale * log2(e)
+  float scale_log2;     // |scale| * log2(e), above 0
+  unsigned flip;        // sign bits for the queries where scale < 0
 };
 
 __device__ __forceinline__ int row_len(const Paged& a, const int b) {
@@ -105,33 +106,59 @@ __device__ __forceinline__ int prefix_len(const Paged& a, const int b,
   return (g >= 0 && g < a.ngroups) ? min(max(a.group_lens[g], 0), n) : 0;
 }
 
+// 8 query values, their signs turned where the scale is negative: the scale's
+// own factor is then positive, and the largest score is the largest product.
+__device__ __forceinline__ bf16x8v load_q(const Paged& a,
+                                          const __hip_bfloat16* src) {
+  return __builtin_bit_cast(bf16x8v,
+                            *reinterpret_cast<const u32x4*>(src) ^ a.flip);
+}
+
+// Weights that join up to 64 partial results, one a lane: exp2(m - M) where
+// the lane's l is not 0 (its o is not read otherwise), and their sum of l.
+__device__ __forceinline__ float join_weight(const float m, const float l,
+                                             float& M, float& L) {
+  M = wave_max(m);
+  const float mu = (M == -INFINITY) ? 0.f : M;
+  const float w = (l == 0.f) ? 0.f : exp2_fast(m - mu);
+  L = wave_sum(l == 0.f ? 0.f : w * l);
+  return w;
+}
+
 }  // namespace
 
 // ------------------------------------------------------------ each row's own
 //
-// One block = (row, KV head, split): NW waves take the split's pages in turn.
-// A wave reads K straight into A fragments (a lane's 16 B of one token; the
-// Q fragments take the dims in the same order) and turns V in its own LDS
-// page, so that the page loop has no block barrier.  Bound: the bytes of the
-// cache; the matrix instructions run mostly empty (G of 16 columns) and still
-// take a tenth of the vector instructions that dot products would.
+// One block = (row, KV head, split): NW waves take the split's half pages in
+// turn.  A wave reads K straight into A fragments (a lane's 16 B of one token;
+// the Q fragments take the dims in the same order) and turns V in its own LDS
+// rows, so that the loop has no block barrier.  Half pages, because 128 (bf16:
+// 168) registers and 9 KB a wave let 4 (3) blocks share a CU: what hides the
+// loads' latency is other waves.  Page ids come 64 at a time, one a lane.
+// Bound: the bytes of the cache; the matrix instructions run mostly empty (G
+// of 16 columns) and still take a tenth of the vector instructions that dot
+// products would.
+#define UNIT 32  // tokens of one step
+
 template <bool FP8, int NW>
-__global__ __launch_bounds__(NW* WAVE, 2) void paged_decode_kernel(
+__global__ __launch_bounds__(NW* WAVE, FP8 ? 4 : 3) void paged_decode_kernel(
     const Paged a, __hip_bfloat16* __restrict__ out) {
   __shared__ __attribute__((aligned(16)))
-  __hip_bfloat16 v_lds[NW][KVPAGE * V_PITCH];
+  __hip_bfloat16 v_lds[NW][UNIT * V_PITCH];
   __shared__ float ml_lds[NW][MAXG][2];
 
   const int b = blockIdx.x, kvh = blockIdx.y, split = blockIdx.z;
-  const int wid = threadIdx.x / WAVE, lane = threadIdx.x % WAVE;
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+  const int lane = threadIdx.x % WAVE;
   const int l16 = lane & 15, g4 = lane >> 4;
   const int n = row_len(a, b);
   const int first = prefix_len(a, b, n);
-  const int page0 = first / KVPAGE;
-  const int npages = (n + KVPAGE - 1) / KVPAGE - page0;
-  const int each = (max(npages, 0) + a.nsplit - 1) / a.nsplit;
-  const int pbegin = page0 + split * each;
-  const int pend = page0 + min(npages, (split + 1) * each);
+  const int unit0 = first / UNIT;
+  const int nunits = (n + UNIT - 1) / UNIT - unit0;
+  const int each = (max(nunits, 0) + a.nsplit - 1) / a.nsplit;
+  const int ubegin = unit0 + split * each + wid;
+  const int uend = unit0 + min(nunits, (split + 1) * each);
+  const int steps = uend > ubegin ? (uend - ubegin + NW - 1) / NW : 0;
 
   // fragment c of lane group g4 holds dims 32c + 8*g4 .. of a bf16 row, or of
   // an e4m3 row (whose 16 B are 16 dims) 64*(c/2) + 16*g4 + 8*(c%2) ..
@@ -139,11 +166,10 @@ __global__ __launch_bounds__(NW* WAVE, 2) void paged_decode_kernel(
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
     const int d = FP8 ? (c / 2) * 64 + g4 * 16 + (c % 2) * 8 : c * 32 + g4 * 8;
-    u32x4 v = {0, 0, 0, 0};
+    const u32x4 none = {0, 0, 0, 0};
+    qf[c] = __builtin_bit_cast(bf16x8v, none);
     if (l16 < a.G)
-      v = *reinterpret_cast<const u32x4*>(
-          a.q + b * a.q_stride + (kvh * a.G + l16) * HD + d);
-    qf[c] = __builtin_bit_cast(bf16x8v, v);
+      qf[c] = load_q(a, a.q + b * a.q_stride + (kvh * a.G + l16) * HD + d);
   }
 
   float m = -INFINITY, l = 0.f;
@@ -156,37 +182,47 @@ __global__ __launch_bounds__(NW* WAVE, 2) void paged_decode_kernel(
       vt + (g4 * 4 + (l16 >> 2)) * V_PITCH + (l16 & 3) * 4;
   const int32_t* table = a.page_table + (int64_t)b * a.max_pages;
 
-  for (int pi = pbegin + wid; pi < pend; pi += NW) {
-    const int page = table[pi];
-    if (page < 0 || page >= a.num_pages) continue;  // no such page: no tokens
-    const int64_t panel = ((int64_t)page * a.hkv + kvh) * KVPAGE;
-    const int tok0 = pi * KVPAGE;
-    const bool whole = tok0 >= first && tok0 + KVPAGE <= n;
+  constexpr int ROWB = FP8 ? HD : 2 * HD;  // bytes of a cache row
+  constexpr int KLD = FP8 ? 2 : 4;    // 16 B loads of a lane, a 16-token tile
+  constexpr int VROW = FP8 ? 8 : 16;  // lanes of one row of V
+  constexpr int VLD = UNIT * VROW / WAVE;
+  const int koff = l16 * ROWB + g4 * 16, voff = lane * 16;
 
-    constexpr int KLD = FP8 ? 2 : 4;    // 16 B loads of a lane, a 16-token tile
-    constexpr int VLD = FP8 ? 8 : 16;   // 16 B loads of a lane, a page of V
-    constexpr int VROW = FP8 ? 8 : 16;  // lanes of one row of V
-    u32x4 kr[4][KLD], vr[VLD];
-    unsigned char ks[4], vs[VLD];
-    const char* kp = (const char*)a.kcache + panel * (FP8 ? HD : 2 * HD);
-    const char* vp = (const char*)a.vcache + panel * (FP8 ? HD : 2 * HD);
+  int ids = 0;
+  for (int i = 0; i < steps; ++i) {
+    const int u = ubegin + i * NW;
+    if (i % WAVE == 0) {
+      const int mine = u + lane * NW;
+      ids = mine < uend ? table[mine / (KVPAGE / UNIT)] : -1;
+    }
+    const int page = __builtin_amdgcn_readlane(ids, i % WAVE);
+    if (page < 0 || page >= a.num_pages) continue;  // no such page: no tokens
+    const int tok0 = u * UNIT;
+    const int64_t panel = ((int64_t)page * a.hkv + kvh) * KVPAGE +
+                          (u % (KVPAGE / UNIT)) * UNIT;
+    const bool whole = tok0 >= first && tok0 + UNIT <= n;
+
+    u32x4 kr[2][KLD], vr[VLD];
+    unsigned char ks[2], vs[VLD];
+    const char* kp = (const char*)a.kcache + panel * ROWB;
+    const char* vp = (const char*)a.vcache + panel * ROWB;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
+    for (int t = 0; t < 2; ++t) {
 #pragma unroll
       for (int c = 0; c < KLD; ++c)
-        kr[t][c] = *reinterpret_cast<const u32x4*>(
-            kp + (t * 16 + l16) * (FP8 ? HD : 2 * HD) + c * 64 + g4 * 16);
-      if (FP8) ks[t] = a.kscale[panel + t * 16 + l16];
+        kr[t][c] = *reinterpret_cast<const u32x4*>(kp + t * 16 * ROWB + c * 64 +
+                                                   koff);
+      if (FP8) ks[t] = (a.kscale + panel)[t * 16 + l16];
     }
 #pragma unroll
-    for (int i = 0; i < VLD; ++i) {
-      vr[i] = *reinterpret_cast<const u32x4*>(vp + (i * WAVE + lane) * 16);
-      if (FP8) vs[i] = a.vscale[panel + (i * WAVE + lane) / VROW];
+    for (int j = 0; j < VLD; ++j) {
+      vr[j] = *reinterpret_cast<const u32x4*>(vp + j * WAVE * 16 + voff);
+      if (FP8) vs[j] = (a.vscale + panel)[j * (WAVE / VROW) + lane / VROW];
     }
 
-    f32x4 s[4];
+    f32x4 s[2];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
+    for (int t = 0; t < 2; ++t) {
       u32x4 kf[4];
       if constexpr (FP8) {
         const float sc = e8m0_scale(ks[t]);
@@ -201,69 +237,65 @@ __global__ __launch_bounds__(NW* WAVE, 2) void paged_decode_kernel(
       for (int c = 0; c < 4; ++c)
         s[t] = MFMA16(__builtin_bit_cast(bf16x8v, kf[c]), qf[c], s[t]);
     }
-
-    float mt = -INFINITY;
+    if (!whole) {
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        s[t][r] *= a.scale_log2;
-        if (!whole) {
+        for (int r = 0; r < 4; ++r) {
           const int tok = tok0 + t * 16 + g4 * 4 + r;
           if (tok < first || tok >= n) s[t][r] = -INFINITY;
         }
-        mt = fmaxf(mt, s[t][r]);
-      }
+    }
+    float mt = s[0][0];
+#pragma unroll
+    for (int j = 1; j < 8; ++j) mt = fmaxf(mt, s[j / 4][j % 4]);
     mt = fmaxf(mt, __shfl_xor(mt, 16, WAVE));
     mt = fmaxf(mt, __shfl_xor(mt, 32, WAVE));
-    const float mn = fmaxf(m, mt);
+    const float mn = fmaxf(m, mt * a.scale_log2);
     const float mu = (mn == -INFINITY) ? 0.f : mn;  // nothing seen yet
-    const float keep = exp2_fast(m - mu);
+    if (__any(mn > m)) {  // a factor of 1 otherwise
+      const float keep = exp2_fast(m - mu);
+      l *= keep;
+#pragma unroll
+      for (int d = 0; d < 8; ++d) o[d] *= keep;
+    }
     m = mn;
-    l *= keep;
+    bf16x8v pf;
 #pragma unroll
-    for (int d = 0; d < 8; ++d) o[d] *= keep;
-
-    bf16x8v pf[2];
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float p = exp2_fast(s[t][r] - mu);
-        l += p;
-        pf[t >> 1][(t & 1) * 4 + r] = (__bf16)p;
-      }
+    for (int j = 0; j < 8; ++j) {
+      const float p = exp2_fast(fmaf(s[j / 4][j % 4], a.scale_log2, -mu));
+      l += p;
+      pf[j] = (__bf16)p;
+    }
 
     // V to LDS as bf16; rows outside the sequence as zeros (weight 0 times
     // whatever a recycled page holds may be NaN)
 #pragma unroll
-    for (int i = 0; i < VLD; ++i) {
-      const int row = (i * WAVE + lane) / VROW;
-      const int tok = tok0 + row;
-      const bool gone = !whole && (tok < first || tok >= n);
+    for (int j = 0; j < VLD; ++j) {
+      const int row = j * (WAVE / VROW) + lane / VROW;
+      const bool gone =
+          !whole && (tok0 + row < first || tok0 + row >= n);
       __hip_bfloat16* dst = vt + row * V_PITCH;
       if constexpr (FP8) {
         u32x4 lo, hi;
-        widen(vr[i], e8m0_scale(vs[i]), lo, hi);
-        if (gone) lo = hi = (u32x4){0, 0, 0, 0};
+        if (gone) vr[j] = (u32x4){0, 0, 0, 0};
+        widen(vr[j], gone ? 1.f : e8m0_scale(vs[j]), lo, hi);
         dst += (lane % VROW) * 16;
         reinterpret_cast<u32x4*>(dst)[0] = lo;
         reinterpret_cast<u32x4*>(dst)[1] = hi;
       } else {
-        if (gone) vr[i] = (u32x4){0, 0, 0, 0};
-        reinterpret_cast<u32x4*>(dst + (lane % VROW) * 8)[0] = vr[i];
+        if (gone) vr[j] = (u32x4){0, 0, 0, 0};
+        reinterpret_cast<u32x4*>(dst + (lane % VROW) * 8)[0] = vr[j];
       }
     }
     // one wave's LDS operations run in order: only the compiler has to be told
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int d = 0; d < 8; ++d) {
-        const __hip_bfloat16* p = vt_read + u * 32 * V_PITCH + d * 16;
-        o[d] = MFMA16(join(read_tr(p), read_tr(p + 16 * V_PITCH)), pf[u], o[d]);
-      }
+    for (int d = 0; d < 8; ++d)
+      o[d] = MFMA16(join(read_tr(vt_read + d * 16),
+                         read_tr(vt_read + d * 16 + 16 * V_PITCH)),
+                    pf, o[d]);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
   }
@@ -271,9 +303,15 @@ __global__ __launch_bounds__(NW* WAVE, 2) void paged_decode_kernel(
   l += __shfl_xor(l, 16, WAVE);
   l += __shfl_xor(l, 32, WAVE);
 
-  // ---- join the waves: O rows over the V pages, now free
+  // ---- join the waves and, where this block writes the output, the prefix's
+  // partial results: O rows over the V rows, now free
+  const int slots = a.nshared + a.nsplit;
+  const int joined = (a.nsplit == 1 && first > 0) ? a.nshared : 0;
   __syncthreads();
   float* o_lds = reinterpret_cast<float*>(&v_lds[0][0]);  // [NW][16][128]
+  float* w_lds = o_lds + NW * MAXG * HD;                  // [16][64]
+  static_assert((NW * MAXG * HD + MAXG * WAVE) * 4 <= sizeof(v_lds),
+                "O and the weights fit V's rows");
   if (l16 < a.G) {
 #pragma unroll
     for (int d = 0; d < 8; ++d)
@@ -285,41 +323,56 @@ __global__ __launch_bounds__(NW* WAVE, 2) void paged_decode_kernel(
     }
   }
   __syncthreads();
-  const int slots = a.nshared + a.nsplit;
-  for (int i = threadIdx.x; i < a.G * HD; i += NW * WAVE) {
-    const int g = i / HD, d = i % HD;
+  for (int g = wid; g < a.G; g += NW) {
     const int64_t row = (int64_t)b * a.hq + kvh * a.G + g;
-    const float* pml = a.part_ml + row * slots * 2;
-    const int joined = (a.nsplit == 1 && first > 0) ? a.nshared : 0;
-    float M = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) M = fmaxf(M, ml_lds[w][g][0]);
-    for (int k = 0; k < joined; ++k) M = fmaxf(M, pml[k * 2]);
-    const float mu = (M == -INFINITY) ? 0.f : M;
-    float L = 0.f, acc = 0.f;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      const float c = exp2_fast(ml_lds[w][g][0] - mu);
-      L = fmaf(c, ml_lds[w][g][1], L);
-      acc = fmaf(c, o_lds[(w * MAXG + g) * HD + d], acc);
+    float mk = -INFINITY, lk = 0.f, M, L;
+    if (lane < NW) {
+      mk = ml_lds[lane][g][0];
+      lk = ml_lds[lane][g][1];
+    } else if (lane - NW < joined) {
+      const float2 ml = reinterpret_cast<const float2*>(
+          a.part_ml)[row * slots + lane - NW];
+      mk = ml.x;
+      lk = ml.y;
     }
+    const float w = join_weight(mk, lk, M, L);
+    // no weight at all (an empty row): zeros
+    w_lds[g * WAVE + lane] = a.nsplit > 1 ? w : L == 0.f ? 0.f : w / L;
+    if (a.nsplit > 1 && lane == 0)
+      reinterpret_cast<float2*>(a.part_ml)[row * slots + a.nshared + split] =
+          make_float2(M, L);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < a.G * (HD / 2); i += NW * WAVE) {
+    const int g = i / (HD / 2), d = i % (HD / 2) * 2;
+    const int64_t row = (int64_t)b * a.hq + kvh * a.G + g;
+    const float* part = a.part_o + row * slots * HD + d;
+    float2 acc = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < NW; ++k) {
+      const float w = w_lds[g * WAVE + k];
+      const float2 x =
+          *reinterpret_cast<const float2*>(&o_lds[(k * MAXG + g) * HD + d]);
+      acc.x = fmaf(w, x.x, acc.x);
+      acc.y = fmaf(w, x.y, acc.y);
+    }
+#pragma unroll 4
     for (int k = 0; k < joined; ++k) {
-      const float lk = pml[k * 2 + 1];
-      if (lk == 0.f) continue;  // an empty range: its o is not written
-      const float c = exp2_fast(pml[k * 2] - mu);
-      L = fmaf(c, lk, L);
-      acc = fmaf(c, a.part_o[(row * slots + k) * HD + d], acc);
+      const float w = w_lds[g * WAVE + NW + k];
+      // an empty range has weight 0 and its o is not written
+      const float2 x = w == 0.f ? make_float2(0.f, 0.f)
+                                : *reinterpret_cast<const float2*>(part +
+                                                                   k * HD);
+      acc.x = fmaf(w, x.x, acc.x);
+      acc.y = fmaf(w, x.y, acc.y);
     }
     if (a.nsplit == 1) {
-      // no weight at all (an empty row): zeros
-      out[row * HD + d] = f2bf(L == 0.f ? 0.f : acc / L);
+      __hip_bfloat16* dst = out + row * HD + d;
+      dst[0] = f2bf(acc.x);
+      dst[1] = f2bf(acc.y);
     } else {
-      const int64_t slot = row * slots + a.nshared + split;
-      a.part_o[slot * HD + d] = acc;
-      if (d == 0) {
-        a.part_ml[slot * 2] = M;
-        a.part_ml[slot * 2 + 1] = L;
-      }
+      *reinterpret_cast<float2*>(
+          a.part_o + (row * slots + a.nshared + split) * HD + d) = acc;
     }
   }
 }
@@ -331,28 +384,29 @@ __global__ __launch_bounds__(4 * WAVE) void paged_join_kernel(
   if (row >= (int64_t)a.B * a.hq) return;
   const int lane = threadIdx.x % WAVE;
   const int b = (int)(row / a.hq);
-  const int slots = a.nshared + a.nsplit;
+  const int slots = a.nshared + a.nsplit;  // up to 64
   const bool has_prefix = prefix_len(a, b, row_len(a, b)) > 0;
   const int from = has_prefix ? 0 : a.nshared;
-  const float* ml = a.part_ml + row * slots * 2;
-  float M = -INFINITY;
-  for (int k = from; k < slots; ++k) M = fmaxf(M, ml[k * 2]);
-  const float mu = (M == -INFINITY) ? 0.f : M;
-  float L = 0.f, o0 = 0.f, o1 = 0.f;
+  float2 ml = make_float2(-INFINITY, 0.f);
+  if (lane >= from && lane < slots)
+    ml = reinterpret_cast<const float2*>(a.part_ml)[row * slots + lane];
+  float M, L;
+  const float w = join_weight(ml.x, ml.y, M, L);
+  const float2* part =
+      reinterpret_cast<const float2*>(a.part_o + row * slots * HD) + lane;
+  float2 acc = make_float2(0.f, 0.f);
+#pragma unroll 8
   for (int k = from; k < slots; ++k) {
-    const float lk = ml[k * 2 + 1];
-    if (lk == 0.f) continue;
-    const float c = exp2_fast(ml[k * 2] - mu);
-    const float2 o =
-        reinterpret_cast<const float2*>(a.part_o + (row * slots + k) * HD)[lane];
-    L = fmaf(c, lk, L);
-    o0 = fmaf(c, o.x, o0);
-    o1 = fmaf(c, o.y, o1);
+    const float wk = __uint_as_float(
+        __builtin_amdgcn_readlane(__float_as_uint(w), k));
+    const float2 x = wk == 0.f ? make_float2(0.f, 0.f) : part[k * (HD / 2)];
+    acc.x = fmaf(wk, x.x, acc.x);
+    acc.y = fmaf(wk, x.y, acc.y);
   }
   const float inv = (L == 0.f) ? 0.f : 1.f / L;
   __hip_bfloat16* dst = out + row * HD + lane * 2;
-  dst[0] = f2bf(L == 0.f ? 0.f : o0 * inv);
-  dst[1] = f2bf(L == 0.f ? 0.f : o1 * inv);
+  dst[0] = f2bf(L == 0.f ? 0.f : acc.x * inv);
+  dst[1] = f2bf(L == 0.f ? 0.f : acc.y * inv);
 }
 
 // -------------------------------------------------------- the shared prefix
@@ -456,8 +510,7 @@ __global__ __launch_bounds__(4 * WAVE, 2) void paged_shared_kernel(
   bf16x8v qf[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k)
-    qf[k] = *reinterpret_cast<const bf16x8v*>(
-        a.q + b * a.q_stride + head * HD + k * 16 + h * 8);
+    qf[k] = load_q(a, a.q + b * a.q_stride + head * HD + k * 16 + h * 8);
 
   float m = -INFINITY, l = 0.f;
   f32x16 o[4];
@@ -472,8 +525,11 @@ __global__ __launch_bounds__(4 * WAVE, 2) void paged_shared_kernel(
   unsigned char ks[LD], vs[LD];
   const int trow = tid / ROW, tcol = tid % ROW;
 
+  // page ids 64 at a time, one a lane: no load waits for another
+  int ids = 0;
   auto fetch = [&](int pi) {
-    const int page = table[pi];
+    if ((pi - pbegin) % WAVE == 0) ids = pi + lane < pend ? table[pi + lane] : -1;
+    const int page = __builtin_amdgcn_readlane(ids, (pi - pbegin) % WAVE);
     const bool ok = page >= 0 && page < a.num_pages;
     const int64_t panel = ((int64_t)(ok ? page : 0) * a.hkv + kvh) * KVPAGE;
     const char* kp = (const char*)a.kcache + panel * (FP8 ? HD : 2 * HD);
@@ -491,10 +547,15 @@ __global__ __launch_bounds__(4 * WAVE, 2) void paged_shared_kernel(
     return ok;
   };
   auto stage = [&](int buf, int pi) {
+    const bool whole = (pi + 1) * KVPAGE <= glen;
 #pragma unroll
     for (int j = 0; j < LD; ++j) {
       const int row = j * (4 * WAVE / ROW) + trow;
-      const bool gone = pi * KVPAGE + row >= glen;  // NaN there times weight 0
+      // beyond the prefix: zeros (NaN there times weight 0)
+      if (!whole && pi * KVPAGE + row >= glen) {
+        vr[j] = (u32x4){0, 0, 0, 0};
+        if (FP8) vs[j] = 127;
+      }
       __hip_bfloat16* kd = &k_lds[buf][row * K_PITCH];
       __hip_bfloat16* vd = &v_lds[buf][row * V_PITCH];
       if constexpr (FP8) {
@@ -503,11 +564,9 @@ __global__ __launch_bounds__(4 * WAVE, 2) void paged_shared_kernel(
         reinterpret_cast<u32x4*>(kd + tcol * 16)[0] = lo;
         reinterpret_cast<u32x4*>(kd + tcol * 16)[1] = hi;
         widen(vr[j], e8m0_scale(vs[j]), lo, hi);
-        if (gone) lo = hi = (u32x4){0, 0, 0, 0};
         reinterpret_cast<u32x4*>(vd + tcol * 16)[0] = lo;
         reinterpret_cast<u32x4*>(vd + tcol * 16)[1] = hi;
       } else {
-        if (gone) vr[j] = (u32x4){0, 0, 0, 0};
         reinterpret_cast<u32x4*>(kd + tcol * 8)[0] = kr[j];
         reinterpret_cast<u32x4*>(vd + tcol * 8)[0] = vr[j];
       }
@@ -531,17 +590,17 @@ __global__ __launch_bounds__(4 * WAVE, 2) void paged_shared_kernel(
                       ((lane >> 4) & 1) * 16 + (lane & 3) * 4];
       f32x16 s[2];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[t][r] = 0.f;
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
+      for (int k = 0; k < 8; ++k)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
           s[t] = MFMA32(*reinterpret_cast<const bf16x8v*>(
                             kt + t * 32 * K_PITCH + k * 16),
                         qf[k], s[t]);
-      }
       const int left = limit - pi * KVPAGE;  // this row's tokens of the page
-      float mt = -INFINITY;
       if (__any(left < KVPAGE)) {
 #pragma unroll
         for (int t = 0; t < 2; ++t)
@@ -549,18 +608,12 @@ __global__ __launch_bounds__(4 * WAVE, 2) void paged_shared_kernel(
           for (int r = 0; r < 16; ++r)
             if (t * 32 + 8 * (r / 4) + 4 * h + r % 4 >= left)
               s[t][r] = -INFINITY;
-            else
-              s[t][r] *= a.scale_log2;
-      } else {
-#pragma unroll
-        for (int t = 0; t < 2; ++t) s[t] *= a.scale_log2;
       }
+      float mt = s[0][0];
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[t][r]);
+      for (int j = 1; j < 32; ++j) mt = fmaxf(mt, s[j / 16][j % 16]);
       mt = fmaxf(mt, __shfl_xor(mt, 32, WAVE));
-      const float mn = fmaxf(m, mt);
+      const float mn = fmaxf(m, mt * a.scale_log2);
       const float mu = (mn == -INFINITY) ? 0.f : mn;
       if (__any(mn > m)) {  // a factor of 1 otherwise
         const float keep = exp2_fast(m - mu);
@@ -574,7 +627,7 @@ __global__ __launch_bounds__(4 * WAVE, 2) void paged_shared_kernel(
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const float p = exp2_fast(s[t][r] - mu);
+          const float p = exp2_fast(fmaf(s[t][r], a.scale_log2, -mu));
           l += p;
           pf[t * 2 + r / 8][r % 8] = (__bf16)p;
         }
@@ -593,10 +646,7 @@ __global__ __launch_bounds__(4 * WAVE, 2) void paged_shared_kernel(
   if (!live) return;
   const int64_t slot =
       ((int64_t)b * a.hq + head) * (a.nshared + a.nsplit) + split;
-  if (h == 0) {
-    a.part_ml[slot * 2] = m;
-    a.part_ml[slot * 2 + 1] = l;
-  }
+  if (h == 0) reinterpret_cast<float2*>(a.part_ml)[slot] = make_float2(m, l);
 #pragma unroll
   for (int d = 0; d < 4; ++d)
 #pragma unroll
@@ -610,6 +660,7 @@ __global__ __launch_bounds__(4 * WAVE, 2) void paged_shared_kernel(
 #include <torch/extension.h>
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
+#include <cmath>
 
 namespace {
 
@@ -658,16 +709,20 @@ Paged paged_args(const torch::Tensor& out, const torch::Tensor& q,
   a.G = (int)(hq / hkv);
   a.max_pages = (int)page_table.size(1);
   a.num_pages = (int)kcache.size(0);
-  a.scale_log2 = (float)(scale * 1.4426950408889634);
+  // above 0, so that a masked score stays -inf: at a scale of 0 every weight
+  // comes out as 2^(1e-37 * score) = 1
+  a.scale_log2 = std::max((float)(std::fabs(scale) * 1.4426950408889634), 1e-37f);
+  a.flip = scale < 0 ? 0x80008000u : 0u;
   return a;
 }
 
-// Blocks that fill the card's 256 CUs twice; a split has at least `least`
-// pages of the widest table row (the lengths themselves are on the device).
-int splits_for(int64_t blocks, int pages, int least) {
-  const int64_t want = (512 + blocks - 1) / std::max<int64_t>(blocks, 1);
+// Splits of one row's (or tile's) pages so that `blocks` of them fill the
+// `room` blocks that the card holds at once; a split has at least `least` pages
+// of the widest table row (the lengths themselves are on the device).
+int splits_for(int64_t blocks, int64_t room, int pages, int least, int most) {
+  const int64_t want = room / std::max<int64_t>(blocks, 1);
   return (int)std::max<int64_t>(
-      1, std::min<int64_t>({want, (pages + least - 1) / least, 128}));
+      1, std::min<int64_t>({want, (pages + least - 1) / least, most}));
 }
 
 template <bool FP8>
@@ -708,7 +763,7 @@ void attn_decode_fp8(torch::Tensor out, torch::Tensor q, torch::Tensor kcache,
   a.kscale = (const uint8_t*)kscale.data_ptr();
   a.vscale = (const uint8_t*)vscale.data_ptr();
   c10::DeviceGuard guard(dev);
-  a.nsplit = splits_for((int64_t)a.B * a.hkv, a.max_pages, 4);
+  a.nsplit = splits_for((int64_t)a.B * a.hkv, 1024, a.max_pages, 2, 64);
   const auto work = partials(a, q);
   launch_decode<true>(a, out, at::hip::getCurrentHIPStream().stream());
   HIP_CHECK_LAST();
@@ -755,17 +810,17 @@ void attn_decode_shared(torch::Tensor out, torch::Tensor q,
   a.ngroups = (int)group_lens.size(0);
   c10::DeviceGuard guard(dev);
   hipStream_t s = at::hip::getCurrentHIPStream().stream();
-  a.nsplit = splits_for((int64_t)a.B * a.hkv, a.max_pages, 4);
+  a.nsplit = splits_for((int64_t)a.B * a.hkv, 768, a.max_pages, 2, 32);
   if (a.ngroups > 0) {
     a.group = (const int32_t*)group.data_ptr();
     a.group_lens = (const int32_t*)group_lens.data_ptr();
     const int per_tile = 128 / a.G;
     const int full = (a.B + per_tile - 1) / per_tile;
-    a.nshared = splits_for((int64_t)full * a.hkv, a.max_pages, 2);
-    const auto work = partials(a, q);
     // each group may leave one tile part full; no more tiles than rows
-    const dim3 grid(a.hkv, a.nshared,
-                    std::min<int>(a.B, full + a.ngroups));
+    const int tiles = std::min<int>(a.B, full + a.ngroups);
+    a.nshared = splits_for((int64_t)tiles * a.hkv, 512, a.max_pages, 2, 32);
+    const auto work = partials(a, q);
+    const dim3 grid(a.hkv, a.nshared, tiles);
     if (fp8)
       hipLaunchKernelGGL((paged_shared_kernel<true>), grid, dim3(4 * WAVE), 0,
                          s, a);
