@@ -427,8 +427,9 @@ def _check_paged(out, q, kcache, page_table, seq_lens) -> None:
     _require(out.dtype == torch.bfloat16 and out.shape == q.shape
              and out.is_contiguous(),
              "out must be contiguous bf16 of q's shape")
-    _require(hq % hkv == 0 and hq // hkv <= 16,
+    _require(hq % hkv == 0 and 1 <= hq // hkv <= 16,
              "hq must be a multiple of hkv, up to 16 times it")
+    _require(kcache.shape[0] > 0, "the cache has no pages")
     _require(page_table.dtype == torch.int32 and page_table.dim() == 2
              and page_table.shape[0] == B and page_table.is_contiguous(),
              "page_table must be a contiguous int32 [B, max_pages]")
@@ -499,7 +500,7 @@ def attn_decode_shared(out: torch.Tensor, q: torch.Tensor,
     row by row, and the two are joined.  ``build_prefix_groups`` finds the
     groups.  The result is that of ``attn_decode`` (or, with the scales of
     an e4m3 cache, ``attn_decode_fp8``) up to the order of its sums, whatever
-    the grouping.
+    the grouping; a row may be shorter than its group's prefix.
     """
     if _native(q):
         _K.attn_decode_shared(out, q, kcache, vcache, page_table, seq_lens,
@@ -526,20 +527,20 @@ def attn_decode_shared(out: torch.Tensor, q: torch.Tensor,
              and group_lens.is_contiguous(),
              "group_lens must be a contiguous int32 [groups]")
     _require(group_lens.shape[0] <= 64, "at most 64 prefix groups")
-    first: dict[int, int] = {}  # group -> the row whose pages stand for it
+    lead: dict[int, int] = {}  # group -> the longest row: its pages are read
     for b, g in enumerate(group.tolist()):
         if 0 <= g < group_lens.shape[0]:
-            first.setdefault(g, b)
+            if g not in lead or seq_lens[b] > seq_lens[lead[g]]:
+                lead[g] = b
 
     def pages_of(b: int, count: int):
         pages = page_table[b, :count].long()
         g = int(group[b])
-        if g in first:
+        if g in lead:
             upto = min(max(int(group_lens[g]), 0), count * 64)
             pages = pages.clone()
-            # a prefix's last page may be its rows' own beyond the prefix:
-            # the common tokens of it lie in the first row's page
-            pages[:upto // 64] = page_table[first[g], :upto // 64].long()
+            # a prefix's last page may be its rows' own beyond the prefix
+            pages[:upto // 64] = page_table[lead[g], :upto // 64].long()
         at = pages.clamp(0, P - 1)
         if kscale is None:
             return pages, kcache[at].float(), vcache[at].float()

@@ -18,9 +18,9 @@
 // so B's slots m = 0..7 are read as {4 tokens of one half, 4 of the other}
 // and V^T is read in the same order: P never leaves its registers.
 //
-// P is rounded to bf16 for the matrix instruction (2^-9 of each weight, with
-// independent signs: the same size as the rounding of the output itself);
-// its sum l is taken before that rounding.
+// P is rounded to bf16 for the matrix instruction (at most 2^-8 of each weight,
+// with independent signs: the size of the output's own rounding); its sum l is
+// the rounded weights', so that they sum to 1.
 //
 // e4m3 rows become bf16 on the way in (scale times code is exact in bf16), so
 // both caches share one arithmetic.
@@ -32,6 +32,7 @@
 #define KVPAGE 64
 #define MAXG 16        // query heads of one KV head: one MFMA column block
 #define MAXGROUPS 64   // prefix groups of one call: one wave finds a tile's
+#define MAXB 65535     // rows of one call
 
 using f32x4 = __attribute__((ext_vector_type(4))) float;
 using f32x16 = __attribute__((ext_vector_type(16))) float;
@@ -48,6 +49,9 @@ using u32x4 = __attribute__((ext_vector_type(4))) unsigned;
 #define V_PITCH 144
 // Row pitch of K: 272 B, 16 B reads of 16 rows cover all banks.
 #define K_PITCH 136
+// Of V in the shared kernel, whose reads take 32 dims of 4 tokens: 320 B, the
+// tokens fall 16 banks apart.
+#define V_PITCH32 160
 
 namespace {
 
@@ -73,6 +77,17 @@ __device__ __forceinline__ void widen(const u32x4 c, const float s, u32x4& lo,
 
 __device__ __forceinline__ float exp2_fast(const float x) {
   return __builtin_amdgcn_exp2f(x);
+}
+
+// l + the sum of 8 bf16, two a dot product with ones, each sum in fp32.
+__device__ __forceinline__ float add8(const bf16x8v p, float l) {
+  using bf16x2 = __attribute__((ext_vector_type(2))) __bf16;
+  const bf16x2 ones = {(__bf16)1.f, (__bf16)1.f};
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    l = __builtin_amdgcn_fdot2_f32_bf16((bf16x2){p[2 * j], p[2 * j + 1]}, ones,
+                                        l, false);
+  return l;
 }
 
 struct Paged {
@@ -147,7 +162,7 @@ __global__ __launch_bounds__(NW* WAVE, FP8 ? 4 : 3) void paged_decode_kernel(
   __hip_bfloat16 v_lds[NW][UNIT * V_PITCH];
   __shared__ float ml_lds[NW][MAXG][2];
 
-  const int b = blockIdx.x, kvh = blockIdx.y, split = blockIdx.z;
+  const int kvh = blockIdx.x, b = blockIdx.y, split = blockIdx.z;
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
   const int lane = threadIdx.x % WAVE;
   const int l16 = lane & 15, g4 = lane >> 4;
@@ -262,11 +277,9 @@ __global__ __launch_bounds__(NW* WAVE, FP8 ? 4 : 3) void paged_decode_kernel(
     m = mn;
     bf16x8v pf;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float p = exp2_fast(fmaf(s[j / 4][j % 4], a.scale_log2, -mu));
-      l += p;
-      pf[j] = (__bf16)p;
-    }
+    for (int j = 0; j < 8; ++j)
+      pf[j] = (__bf16)exp2_fast(fmaf(s[j / 4][j % 4], a.scale_log2, -mu));
+    l = add8(pf, l);
 
     // V to LDS as bf16; rows outside the sequence as zeros (weight 0 times
     // whatever a recycled page holds may be NaN)
@@ -307,6 +320,20 @@ __global__ __launch_bounds__(NW* WAVE, FP8 ? 4 : 3) void paged_decode_kernel(
   // partial results: O rows over the V rows, now free
   const int slots = a.nshared + a.nsplit;
   const int joined = (a.nsplit == 1 && first > 0) ? a.nshared : 0;
+  // the prefix's first o's are on their way before their weights are known
+  constexpr int AHEAD = 4;
+  float2 ahead[AHEAD];
+  const auto early = [&](const float* part) __attribute__((always_inline)) {
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k)
+      if (k < joined)
+        ahead[k] = *reinterpret_cast<const float2*>(part + k * HD);
+  };
+  if (threadIdx.x < a.G * (HD / 2))
+    early(a.part_o +
+          ((int64_t)b * a.hq + kvh * a.G + threadIdx.x / (HD / 2)) * slots *
+              HD +
+          threadIdx.x % (HD / 2) * 2);
   __syncthreads();
   float* o_lds = reinterpret_cast<float*>(&v_lds[0][0]);  // [NW][16][128]
   float* w_lds = o_lds + NW * MAXG * HD;                  // [16][64]
@@ -347,6 +374,7 @@ __global__ __launch_bounds__(NW* WAVE, FP8 ? 4 : 3) void paged_decode_kernel(
     const int g = i / (HD / 2), d = i % (HD / 2) * 2;
     const int64_t row = (int64_t)b * a.hq + kvh * a.G + g;
     const float* part = a.part_o + row * slots * HD + d;
+    if (i != (int)threadIdx.x) early(part);
     float2 acc = make_float2(0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < NW; ++k) {
@@ -356,16 +384,20 @@ __global__ __launch_bounds__(NW* WAVE, FP8 ? 4 : 3) void paged_decode_kernel(
       acc.x = fmaf(w, x.x, acc.x);
       acc.y = fmaf(w, x.y, acc.y);
     }
-#pragma unroll 4
-    for (int k = 0; k < joined; ++k) {
+    // an empty range has weight 0 and its o, read all the same (no branch
+    // between the loads), is not written
+    const auto add = [&](const int k, const float2 x)
+        __attribute__((always_inline)) {
       const float w = w_lds[g * WAVE + NW + k];
-      // an empty range has weight 0 and its o is not written
-      const float2 x = w == 0.f ? make_float2(0.f, 0.f)
-                                : *reinterpret_cast<const float2*>(part +
-                                                                   k * HD);
-      acc.x = fmaf(w, x.x, acc.x);
-      acc.y = fmaf(w, x.y, acc.y);
-    }
+      acc.x = w == 0.f ? acc.x : fmaf(w, x.x, acc.x);
+      acc.y = w == 0.f ? acc.y : fmaf(w, x.y, acc.y);
+    };
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k)
+      if (k < joined) add(k, ahead[k]);
+#pragma unroll 4
+    for (int k = AHEAD; k < joined; ++k)
+      add(k, *reinterpret_cast<const float2*>(part + k * HD));
     if (a.nsplit == 1) {
       __hip_bfloat16* dst = out + row * HD + d;
       dst[0] = f2bf(acc.x);
@@ -385,24 +417,34 @@ __global__ __launch_bounds__(4 * WAVE) void paged_join_kernel(
   const int lane = threadIdx.x % WAVE;
   const int b = (int)(row / a.hq);
   const int slots = a.nshared + a.nsplit;  // up to 64
-  const bool has_prefix = prefix_len(a, b, row_len(a, b)) > 0;
-  const int from = has_prefix ? 0 : a.nshared;
-  float2 ml = make_float2(-INFINITY, 0.f);
-  if (lane >= from && lane < slots)
-    ml = reinterpret_cast<const float2*>(a.part_ml)[row * slots + lane];
-  float M, L;
-  const float w = join_weight(ml.x, ml.y, M, L);
+  // The first o's are on their way before their weights are known: what is
+  // not written (an empty range, a row without a prefix) weighs nothing.
+  constexpr int AHEAD = 16;
   const float2* part =
       reinterpret_cast<const float2*>(a.part_o + row * slots * HD) + lane;
+  float2 x[AHEAD];
+#pragma unroll
+  for (int k = 0; k < AHEAD; ++k) x[k] = part[min(k, slots - 1) * (HD / 2)];
+  float2 ml = make_float2(-INFINITY, 0.f);
+  if (lane < slots)
+    ml = reinterpret_cast<const float2*>(a.part_ml)[row * slots + lane];
+  if (lane < a.nshared && prefix_len(a, b, row_len(a, b)) == 0)
+    ml = make_float2(-INFINITY, 0.f);
+  float M, L;
+  const float w = join_weight(ml.x, ml.y, M, L);
   float2 acc = make_float2(0.f, 0.f);
+  const auto add = [&](const int k, const float2 o)
+      __attribute__((always_inline)) {
+    const float wk =
+        __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), k));
+    acc.x = wk == 0.f ? acc.x : fmaf(wk, o.x, acc.x);
+    acc.y = wk == 0.f ? acc.y : fmaf(wk, o.y, acc.y);
+  };
+#pragma unroll
+  for (int k = 0; k < AHEAD; ++k)
+    if (k < slots) add(k, x[k]);
 #pragma unroll 8
-  for (int k = from; k < slots; ++k) {
-    const float wk = __uint_as_float(
-        __builtin_amdgcn_readlane(__float_as_uint(w), k));
-    const float2 x = wk == 0.f ? make_float2(0.f, 0.f) : part[k * (HD / 2)];
-    acc.x = fmaf(wk, x.x, acc.x);
-    acc.y = fmaf(wk, x.y, acc.y);
-  }
+  for (int k = AHEAD; k < slots; ++k) add(k, part[k * (HD / 2)]);
   const float inv = (L == 0.f) ? 0.f : 1.f / L;
   __hip_bfloat16* dst = out + row * HD + lane * 2;
   dst[0] = f2bf(L == 0.f ? 0.f : acc.x * inv);
@@ -422,26 +464,37 @@ __global__ __launch_bounds__(4 * WAVE) void paged_join_kernel(
 template <bool FP8>
 __global__ __launch_bounds__(4 * WAVE, 2) void paged_shared_kernel(
     const Paged a) {
+  // two pages of K, then two of V
   __shared__ __attribute__((aligned(16)))
-  __hip_bfloat16 k_lds[2][KVPAGE * K_PITCH];
-  __shared__ __attribute__((aligned(16)))
-  __hip_bfloat16 v_lds[2][KVPAGE * V_PITCH];
+  __hip_bfloat16 lds[2 * KVPAGE * (K_PITCH + V_PITCH32)];
+  __hip_bfloat16* const k_lds = lds;
+  __hip_bfloat16* const v_lds = lds + 2 * KVPAGE * K_PITCH;
   __shared__ int counts[MAXGROUPS];
   __shared__ int tile_rows[128];
-  __shared__ int tile_of[4];  // group, its tile, rows in it, longest row
+  __shared__ int tile_of[2];           // group, rows
+  __shared__ unsigned long long longest;  // length of a tile's row << 32 | row
 
   const int kvh = blockIdx.x, split = blockIdx.y, tile = blockIdx.z;
   const int tid = threadIdx.x;
   const int wid = tid / WAVE, lane = tid % WAVE;
   const int per_tile = 128 / a.G;
 
-  // ---- which group's which rows: count members, walk the tiles, then the
-  // members in batch order (a few hundred loads from L2)
+  // ---- which group's which rows: each row's group goes to LDS (a byte, in
+  // what the pages take later) and is counted, one wave walks the tiles and then the
+  // members in batch order
+  unsigned char* groups = reinterpret_cast<unsigned char*>(lds);
+  static_assert(MAXB <= sizeof(lds), "a byte a row");
   if (tid < MAXGROUPS) counts[tid] = 0;
+  if (tid == 0) {
+    tile_of[0] = -1;
+    longest = 0;
+  }
   __syncthreads();
   for (int b = tid; b < a.B; b += 4 * WAVE) {
     const int g = a.group[b];
-    if (g >= 0 && g < a.ngroups) atomicAdd(&counts[g], 1);
+    const bool in = g >= 0 && g < a.ngroups;
+    groups[b] = in ? g : 255;
+    if (in) atomicAdd(&counts[g], 1);
   }
   __syncthreads();
   if (wid == 0) {
@@ -452,51 +505,30 @@ __global__ __launch_bounds__(4 * WAVE, 2) void paged_shared_kernel(
       const int x = __shfl_up(upto, off, WAVE);
       if (lane >= off) upto += x;
     }
-    const bool mine = tile >= upto - tiles && tile < upto;
-    if (lane == 0) tile_of[0] = -1;
-    __builtin_amdgcn_wave_barrier();
+    const unsigned long long mine =
+        __ballot(tile >= upto - tiles && tile < upto);
     if (mine) {
-      tile_of[0] = lane;
-      tile_of[1] = tile - (upto - tiles);
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    const int g = tile_of[0];
-    if (g >= 0) {
-      const int skip = tile_of[1] * per_tile;
-      int seen = 0, longest = 0;
+      const int g = 63 - __clzll((long long)mine);
+      const int skip =
+          (tile - __builtin_amdgcn_readlane(upto - tiles, g)) * per_tile;
+      int seen = 0;
       for (int b0 = 0; b0 < a.B && seen < skip + per_tile; b0 += WAVE) {
-        const int b = b0 + lane;
-        const bool in = b < a.B && a.group[b] == g;
+        const bool in = b0 + lane < a.B && groups[b0 + lane] == g;
         const unsigned long long bal = __ballot(in);
         const int rank = seen + __popcll(bal & ((1ull << lane) - 1)) - skip;
-        if (in && rank >= 0 && rank < per_tile) {
-          tile_rows[rank] = b;
-          longest = max(longest, row_len(a, b));
-        }
+        if (in && rank >= 0 && rank < per_tile) tile_rows[rank] = b0 + lane;
         seen += __popcll(bal);
       }
-#pragma unroll
-      for (int off = 32; off > 0; off >>= 1)
-        longest = max(longest, __shfl_xor(longest, off, WAVE));
       if (lane == 0) {
-        tile_of[2] = min(seen - skip, per_tile);
-        tile_of[3] = longest;
+        tile_of[0] = g;
+        tile_of[1] = min(seen - skip, per_tile);
       }
     }
   }
   __syncthreads();
   const int grp = tile_of[0];
   if (grp < 0) return;  // fewer tiles than blocks
-  const int nrows = tile_of[2] * a.G;
-
-  // no token past the longest row: what lies there may be anything
-  const int glen = min(max(a.group_lens[grp], 0), tile_of[3]);
-  const int npages = (glen + KVPAGE - 1) / KVPAGE;
-  const int each = (npages + a.nshared - 1) / a.nshared;
-  const int pbegin = split * each;
-  const int pend = min(npages, pbegin + each);
-  const int32_t* table = a.page_table + (int64_t)tile_rows[0] * a.max_pages;
+  const int nrows = tile_of[1] * a.G;
 
   // ---- this wave's 32 query rows: one a lane, halves h of the MFMA's K
   const int r32 = lane & 31, h = lane >> 5;
@@ -504,13 +536,25 @@ __global__ __launch_bounds__(4 * WAVE, 2) void paged_shared_kernel(
   const bool live = i < nrows;
   const int b = tile_rows[live ? i / a.G : 0];
   const int head = kvh * a.G + (live ? i % a.G : 0);
-  // a lane without a row computes row 0 again and writes nothing
-  const int limit = live ? min(row_len(a, b), glen) : glen;
   const bool wave_live = wid * 32 < nrows;
+  const int len = row_len(a, b);
   bf16x8v qf[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k)
     qf[k] = load_q(a, a.q + b * a.q_stride + head * HD + k * 16 + h * 8);
+  if (live) atomicMax(&longest, (unsigned long long)len << 32 | (unsigned)b);
+  __syncthreads();
+  // the longest row's pages, and no token past it: what lies there, or in the
+  // table past a shorter row, may be anything
+  const int glen = min(max(a.group_lens[grp], 0), (int)(longest >> 32));
+  const int32_t* table =
+      a.page_table + (int64_t)(unsigned)longest * a.max_pages;
+  // a lane without a row computes row 0 again and writes nothing
+  const int limit = live ? min(len, glen) : glen;
+  const int npages = (glen + KVPAGE - 1) / KVPAGE;
+  const int each = (npages + a.nshared - 1) / a.nshared;
+  const int pbegin = split * each;
+  const int pend = min(npages, pbegin + each);
 
   float m = -INFINITY, l = 0.f;
   f32x16 o[4];
@@ -556,8 +600,8 @@ __global__ __launch_bounds__(4 * WAVE, 2) void paged_shared_kernel(
         vr[j] = (u32x4){0, 0, 0, 0};
         if (FP8) vs[j] = 127;
       }
-      __hip_bfloat16* kd = &k_lds[buf][row * K_PITCH];
-      __hip_bfloat16* vd = &v_lds[buf][row * V_PITCH];
+      __hip_bfloat16* kd = &k_lds[(buf * KVPAGE + row) * K_PITCH];
+      __hip_bfloat16* vd = &v_lds[(buf * KVPAGE + row) * V_PITCH32];
       if constexpr (FP8) {
         u32x4 lo, hi;
         widen(kr[j], e8m0_scale(ks[j]), lo, hi);
@@ -584,10 +628,10 @@ __global__ __launch_bounds__(4 * WAVE, 2) void paged_shared_kernel(
     const bool cur = ok;
     if (pi + 1 < pend) ok = fetch(pi + 1);
     if (wave_live && cur) {
-      const __hip_bfloat16* kt = &k_lds[buf][r32 * K_PITCH + h * 8];
+      const __hip_bfloat16* kt = &k_lds[(buf * KVPAGE + r32) * K_PITCH + h * 8];
       const __hip_bfloat16* vt =
-          &v_lds[buf][(4 * h + ((lane & 15) >> 2)) * V_PITCH +
-                      ((lane >> 4) & 1) * 16 + (lane & 3) * 4];
+          &v_lds[(buf * KVPAGE + 4 * h + ((lane & 15) >> 2)) * V_PITCH32 +
+                 ((lane >> 4) & 1) * 16 + (lane & 3) * 4];
       f32x16 s[2];
 #pragma unroll
       for (int t = 0; t < 2; ++t)
@@ -627,16 +671,18 @@ __global__ __launch_bounds__(4 * WAVE, 2) void paged_shared_kernel(
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const float p = exp2_fast(fmaf(s[t][r], a.scale_log2, -mu));
-          l += p;
-          pf[t * 2 + r / 8][r % 8] = (__bf16)p;
+          pf[t * 2 + r / 8][r % 8] =
+              (__bf16)exp2_fast(fmaf(s[t][r], a.scale_log2, -mu));
         }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) l = add8(pf[u], l);
 #pragma unroll
       for (int u = 0; u < 4; ++u)
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
-          const __hip_bfloat16* p = vt + u * 16 * V_PITCH + d * 32;
-          o[d] = MFMA32(join(read_tr(p), read_tr(p + 8 * V_PITCH)), pf[u], o[d]);
+          const __hip_bfloat16* p = vt + u * 16 * V_PITCH32 + d * 32;
+          o[d] = MFMA32(join(read_tr(p), read_tr(p + 8 * V_PITCH32)), pf[u],
+                        o[d]);
         }
     }
     if (pi + 1 < pend) stage(buf ^ 1, pi + 1);
@@ -682,8 +728,10 @@ Paged paged_args(const torch::Tensor& out, const torch::Tensor& q,
   TORCH_CHECK(out.device() == dev && out.scalar_type() == torch::kBFloat16 &&
                   out.sizes() == q.sizes() && out.is_contiguous(),
               "out must be contiguous bf16 of q's shape");
-  TORCH_CHECK(hq % hkv == 0 && hq / hkv <= MAXG,
+  TORCH_CHECK(hq % hkv == 0 && hq / hkv >= 1 && hq / hkv <= MAXG,
               "hq must be a multiple of hkv, up to 16 times it");
+  TORCH_CHECK(kcache.size(0) > 0 && kcache.size(0) <= INT32_MAX,
+              "the cache has no pages");
   TORCH_CHECK(page_table.device() == dev &&
                   page_table.scalar_type() == torch::kInt32 &&
                   page_table.dim() == 2 && page_table.size(0) == B &&
@@ -695,7 +743,7 @@ Paged paged_args(const torch::Tensor& out, const torch::Tensor& q,
                   seq_lens.dim() == 1 && seq_lens.size(0) == B &&
                   seq_lens.is_contiguous(),
               "seq_lens must be a contiguous int32 [B]");
-  TORCH_CHECK(hkv <= 65535, "too many KV heads");
+  TORCH_CHECK(B <= MAXB, "too many rows");
   Paged a{};
   a.kcache = kcache.data_ptr();
   a.vcache = vcache.data_ptr();
@@ -727,7 +775,7 @@ int splits_for(int64_t blocks, int64_t room, int pages, int least, int most) {
 
 template <bool FP8>
 void launch_decode(const Paged& a, torch::Tensor& out, hipStream_t s) {
-  const dim3 grid(a.B, a.hkv, a.nsplit);
+  const dim3 grid(a.hkv, a.B, a.nsplit);
   hipLaunchKernelGGL((paged_decode_kernel<FP8, 4>), grid, dim3(4 * WAVE), 0, s,
                      a, (__hip_bfloat16*)out.data_ptr());
   if (a.nsplit > 1)

@@ -444,6 +444,44 @@ def test_attn_decode_shared_any_prefix_length(device, fp8):
     _close(_shared(s, device), *want)
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_attn_decode_shared_short_rows_first(device):
+    """A group's first rows may have ended: the entries past a row's length
+    name other pages, and none of them is read."""
+    s = _shared_batch([0, 0, 0, 0], [192], [9, 40, 77, 3], 8, 2)
+    other = min(set(range(s["k"].shape[0])) - set(s["table"][2].tolist()))
+    for b, n in ((0, 0), (1, 70), (3, 192)):
+        s["lens"][b] = n
+        s["table"][b, (n + PAGE - 1) // PAGE:] = other
+    s["k"][other] = math.nan
+    s["v"][other] = math.nan
+    _close(_shared(s, device), *_expect(s, HD ** -0.5))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B", [4097, 65535])
+def test_attn_decode_shared_most_rows(B):
+    """Rows up to the limit, one group of them: every row is some tile's."""
+    g = torch.Generator().manual_seed(B)
+    s = _batch([2 * PAGE + 3], 1, 1, seed=3, fp8=False)
+    s["q"] = torch.randn(B, 1, HD, generator=g).to(torch.bfloat16)
+    s["table"] = s["table"].expand(B, -1).contiguous()
+    s["lens"] = s["lens"].expand(B).contiguous()
+    s["group"] = torch.arange(B, dtype=torch.int32) % 3 - 1
+    s["glens"] = torch.tensor([128, 64], dtype=torch.int32)
+    n = int(s["lens"][0])
+    kk, vv = (s[x][s["table"][0].long()].double().view(-1, HD)[:n]
+              for x in ("k", "v"))
+    q = s["q"][:, 0].double()
+    p = torch.softmax(q @ kk.T * HD ** -0.5, -1)
+    want = p @ vv
+    # as in _expect
+    ds = 2 ** -17 * HD ** -0.5 * (q.abs() @ kk.abs().T).amax(-1, keepdim=True)
+    rel = 2 ** -8 + 2 * (ds + 2 ** -20) + n * 2 ** -24
+    tol = 2 ** -8 * want.abs() + rel * (p @ vv.abs())
+    _close(_shared(s, "cuda")[:, 0], want, tol)
+
+
 def test_build_prefix_groups():
     table = np.array([[3, 4, 5, 6], [3, 4, 9, 0], [8, 1, 2, 0], [3, 4, 5, 7],
                       [8, 1, 2, 0], [11, 0, 0, 0], [3, 0, 0, 0]], np.int32)
@@ -518,6 +556,9 @@ def test_refusals(device):
     refused(dec, out, q, kc, vc, ks, vs, t[:1], n, 1.0)
     refused(dec, out, q, kc, vc, ks, vs, t, n.long(), 1.0)
     refused(dec, out[:, :3].contiguous(), q[:, :3], kc, vc, ks, vs, t, n, 1.0)
+    refused(dec, out, q, kc[:0], vc[:0], ks[:0], vs[:0], t, n, 1.0)
+    none = out[:, :0].contiguous()
+    refused(dec, none, none, kc, vc, ks, vs, t, n, 1.0)
     wide = torch.zeros(2, 34, HD, dtype=torch.bfloat16, device=device)
     refused(dec, wide, wide, kc, vc, ks, vs, t, n, 1.0)
     sh = ops.attn_decode_shared
@@ -526,6 +567,7 @@ def test_refusals(device):
     refused(sh, out, q, bf16, bf16, t, n, g, gl, 1.0, kscale=ks)
     refused(sh, out, q, bf16, bf16, t, n, g, gl, 1.0, kscale=ks, vscale=vs)
     refused(sh, out, q, bf16, bf16, t, n, g[:1], gl, 1.0)
+    refused(sh, out, q, bf16[:0], bf16[:0], t, n, g, gl, 1.0)
     refused(sh, out, q, bf16, bf16, t, n, g, gl.long(), 1.0)
     refused(sh, out, q, bf16, bf16, t, n, g,
             torch.zeros(65, dtype=torch.int32, device=device), 1.0)
