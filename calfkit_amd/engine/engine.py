@@ -56,8 +56,13 @@ RUN_STEPS = (8, 4, 2, 1)
 
 #: prefix groups of one decode run (more share without being grouped)
 MAX_PREFIX_GROUPS = 16
-#: whole pages a group's rows have in common before it is worth a pass
-MIN_PREFIX_PAGES = 2
+#: bytes of one layer's cache that groups save a step from being read, below
+#: which rows run without them: a pass over prefixes and its joins cost 5 to
+#: 9 us.  Measured with cold caches, 32/8 heads, bf16, groups against none:
+#: 126 MB (16 rows of 2048 shared tokens) 30.7 against 26.7 us, 132 MB (64 of
+#: 512) 38.0 / 37.7, 252 MB (16 of 4096) 36.6 / 38.5, 264 MB (64 of 1024)
+#: 40.5 / 46.2, 267 MB (256 of 256) 101 / 97, 528 MB (64 of 2048) 43.5 / 63.1
+MIN_SHARED_BYTES = 256 << 20
 
 #: lockstep op channel opcodes (tensor-coded: the
 #: pickled broadcast_object_list per visit becomes one fixed int64[2]
@@ -976,7 +981,7 @@ class InferenceEngine:
         if self.shared_prefix:
             group, lens = gops.build_prefix_groups(
                 pt[:B], base[:B], max_groups=MAX_PREFIX_GROUPS,
-                min_pages=MIN_PREFIX_PAGES)
+                min_saved=MIN_SHARED_BYTES // self.kv.bytes_per_layer_page())
             full = np.full(pad, -1, dtype=np.int32)
             full[:B] = group
             self._group[:pad].copy_(torch.from_numpy(full), non_blocking=True)

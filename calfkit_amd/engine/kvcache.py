@@ -97,6 +97,10 @@ class KVCache:
     def free_pages(self) -> int:
         return len(self._free) + len(self._lru)
 
+    def bytes_per_layer_page(self) -> int:
+        """Of one layer: what attention reads of a page."""
+        return self.bytes_per_page() // self.layers
+
     def bytes_per_page(self) -> int:
         row = (self.head_dim + 1 if self.kscale is not None
                else self.head_dim * 2)

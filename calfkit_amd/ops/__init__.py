@@ -553,15 +553,16 @@ def attn_decode_shared(out: torch.Tensor, q: torch.Tensor,
 
 def build_prefix_groups(page_table: "np.ndarray", lengths: "np.ndarray",
                         max_groups: int = 64, min_rows: int = 2,
-                        min_pages: int = 1) -> tuple["np.ndarray",
-                                                     "np.ndarray"]:
+                        min_pages: int = 1, min_saved: int = 0) -> tuple[
+                            "np.ndarray", "np.ndarray"]:
     """Host-side prefix groups of a batch for ``attn_decode_shared``.
 
     page_table [B, max_pages] and lengths [B] as numpy arrays.  Rows with the
     same first page form a group; its prefix is the run of whole pages that
     all of them have in common.  Groups of fewer rows or pages than the
     minimum are left out, and of more than ``max_groups`` those that save the
-    least reading.  Returns (group [B] i32, group_lens [max_groups] i32).
+    least reading; where all of them together save fewer than ``min_saved``
+    page reads, there are none.  Returns (group [B] i32, group_lens [max_groups] i32).
     """
     import numpy as np
 
@@ -585,6 +586,8 @@ def build_prefix_groups(page_table: "np.ndarray", lengths: "np.ndarray",
         if pages >= max(1, min_pages):
             found.append(((members.size - 1) * pages, pages, members))
     found.sort(key=lambda f: -f[0])
+    if sum(f[0] for f in found[:max_groups]) < min_saved:
+        return group, lens
     for g, (_, pages, members) in enumerate(found[:max_groups]):
         group[members] = g
         lens[g] = pages * 64

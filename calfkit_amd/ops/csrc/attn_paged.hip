@@ -33,6 +33,10 @@
 #define MAXG 16        // query heads of one KV head: one MFMA column block
 #define MAXGROUPS 64   // prefix groups of one call: one wave finds a tile's
 #define MAXB 65535     // rows of one call
+#define TILE 128       // query rows of one block in the shared pass
+#define MAXPIECES 32   // of one tile's prefix
+#define LEAST 2        // pages of a piece or of a split, at least
+#define SLACK 8.f      // log2 by which a weight may pass 1
 
 using f32x4 = __attribute__((ext_vector_type(4))) float;
 using f32x16 = __attribute__((ext_vector_type(16))) float;
@@ -43,6 +47,11 @@ using u32x4 = __attribute__((ext_vector_type(4))) unsigned;
 
 #define MFMA16(a, b, c) __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0)
 #define MFMA32(a, b, c) __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0)
+
+// The order of a block's instructions, by kind.
+#define SCHED(kind, n) __builtin_amdgcn_sched_group_barrier(kind, n, 0)
+#define MFMA 0x8
+#define DS_READ 0x100
 
 // Row pitch of V in LDS, in halfwords: 288 B = 72 banks, so that the 4-token
 // blocks of a transposing read fall on banks 8 apart.
@@ -100,11 +109,15 @@ struct Paged {
   const int32_t* seq_lens;    // [B]
   const int32_t* group;       // [B] or null: prefix group, < 0 for none
   const int32_t* group_lens;  // [ngroups] tokens of each group's prefix
-  float* part_o;              // [B * hq, slots, 128]
-  float* part_ml;             // [B * hq, slots, 2]
+  float* part_o;              // [B * hq, nsplit, 128]
+  float* part_ml;             // [B * hq, nsplit, 2]
+  float* pre_o;               // [pieces, hkv, 128, 128]
+  float* pre_ml;              // [pieces, hkv, 128, 2]
+  int4* pre_at;               // [B] where a row's are: first piece, pieces, row
   int64_t q_stride;
   int B, hq, hkv, G, max_pages, num_pages, ngroups;
-  int nshared, nsplit;  // partial slots of the prefix and of the rest
+  int nsplit;           // of each row's own tokens
+  int npre;             // blocks of a KV head in the shared pass
   float scale_log2;     // |scale| * log2(e), above 0
   unsigned flip;        // sign bits for the queries where scale < 0
 };
@@ -119,6 +132,13 @@ __device__ __forceinline__ int prefix_len(const Paged& a, const int b,
   if (a.group == nullptr) return 0;
   const int g = a.group[b];
   return (g >= 0 && g < a.ngroups) ? min(max(a.group_lens[g], 0), n) : 0;
+}
+
+// A row's first partial result of the prefix, for the first head of kvh; the
+// next piece's is hkv * TILE rows on.
+__device__ __forceinline__ int64_t prefix_row(const Paged& a, const int4 at,
+                                              const int kvh) {
+  return ((int64_t)at.x * a.hkv + kvh) * TILE + at.z * a.G;
 }
 
 // 8 query values, their signs turned where the scale is negative: the scale's
@@ -318,8 +338,10 @@ __global__ __launch_bounds__(NW* WAVE, FP8 ? 4 : 3) void paged_decode_kernel(
 
   // ---- join the waves and, where this block writes the output, the prefix's
   // partial results: O rows over the V rows, now free
-  const int slots = a.nshared + a.nsplit;
-  const int joined = (a.nsplit == 1 && first > 0) ? a.nshared : 0;
+  int4 at = make_int4(0, 0, 0, 0);
+  if (a.nsplit == 1 && first > 0) at = a.pre_at[b];
+  const int joined = at.y;
+  const int64_t pre = prefix_row(a, at, kvh);
   // the prefix's first o's are on their way before their weights are known
   constexpr int AHEAD = 4;
   float2 ahead[AHEAD];
@@ -327,12 +349,12 @@ __global__ __launch_bounds__(NW* WAVE, FP8 ? 4 : 3) void paged_decode_kernel(
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k)
       if (k < joined)
-        ahead[k] = *reinterpret_cast<const float2*>(part + k * HD);
+        ahead[k] =
+            *reinterpret_cast<const float2*>(part +
+                                             (int64_t)k * a.hkv * (TILE * HD));
   };
   if (threadIdx.x < a.G * (HD / 2))
-    early(a.part_o +
-          ((int64_t)b * a.hq + kvh * a.G + threadIdx.x / (HD / 2)) * slots *
-              HD +
+    early(a.pre_o + (pre + threadIdx.x / (HD / 2)) * HD +
           threadIdx.x % (HD / 2) * 2);
   __syncthreads();
   float* o_lds = reinterpret_cast<float*>(&v_lds[0][0]);  // [NW][16][128]
@@ -358,7 +380,7 @@ __global__ __launch_bounds__(NW* WAVE, FP8 ? 4 : 3) void paged_decode_kernel(
       lk = ml_lds[lane][g][1];
     } else if (lane - NW < joined) {
       const float2 ml = reinterpret_cast<const float2*>(
-          a.part_ml)[row * slots + lane - NW];
+          a.pre_ml)[pre + g + (int64_t)(lane - NW) * a.hkv * TILE];
       mk = ml.x;
       lk = ml.y;
     }
@@ -366,14 +388,14 @@ __global__ __launch_bounds__(NW* WAVE, FP8 ? 4 : 3) void paged_decode_kernel(
     // no weight at all (an empty row): zeros
     w_lds[g * WAVE + lane] = a.nsplit > 1 ? w : L == 0.f ? 0.f : w / L;
     if (a.nsplit > 1 && lane == 0)
-      reinterpret_cast<float2*>(a.part_ml)[row * slots + a.nshared + split] =
+      reinterpret_cast<float2*>(a.part_ml)[row * a.nsplit + split] =
           make_float2(M, L);
   }
   __syncthreads();
   for (int i = threadIdx.x; i < a.G * (HD / 2); i += NW * WAVE) {
     const int g = i / (HD / 2), d = i % (HD / 2) * 2;
     const int64_t row = (int64_t)b * a.hq + kvh * a.G + g;
-    const float* part = a.part_o + row * slots * HD + d;
+    const float* part = a.pre_o + (pre + g) * HD + d;
     if (i != (int)threadIdx.x) early(part);
     float2 acc = make_float2(0.f, 0.f);
 #pragma unroll
@@ -397,14 +419,15 @@ __global__ __launch_bounds__(NW* WAVE, FP8 ? 4 : 3) void paged_decode_kernel(
       if (k < joined) add(k, ahead[k]);
 #pragma unroll 4
     for (int k = AHEAD; k < joined; ++k)
-      add(k, *reinterpret_cast<const float2*>(part + k * HD));
+      add(k, *reinterpret_cast<const float2*>(part + (int64_t)k * a.hkv *
+                                                         (TILE * HD)));
     if (a.nsplit == 1) {
       __hip_bfloat16* dst = out + row * HD + d;
       dst[0] = f2bf(acc.x);
       dst[1] = f2bf(acc.y);
     } else {
       *reinterpret_cast<float2*>(
-          a.part_o + (row * slots + a.nshared + split) * HD + d) = acc;
+          a.part_o + (row * a.nsplit + split) * HD + d) = acc;
     }
   }
 }
@@ -415,21 +438,34 @@ __global__ __launch_bounds__(4 * WAVE) void paged_join_kernel(
   const int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / WAVE;
   if (row >= (int64_t)a.B * a.hq) return;
   const int lane = threadIdx.x % WAVE;
-  const int b = (int)(row / a.hq);
-  const int slots = a.nshared + a.nsplit;  // up to 64
+  const int b = (int)(row / a.hq);  // one a wave: its branches are uniform
+  const int own = a.nsplit;  // up to 32 where rows have prefixes, 64 if not
   // The first o's are on their way before their weights are known: what is
-  // not written (an empty range, a row without a prefix) weighs nothing.
-  constexpr int AHEAD = 16;
+  // not written (an empty range) weighs nothing.
+  constexpr int AHEAD = 8;
   const float2* part =
-      reinterpret_cast<const float2*>(a.part_o + row * slots * HD) + lane;
-  float2 x[AHEAD];
+      reinterpret_cast<const float2*>(a.part_o + row * own * HD) + lane;
+  float2 x[AHEAD], y[AHEAD];
 #pragma unroll
-  for (int k = 0; k < AHEAD; ++k) x[k] = part[min(k, slots - 1) * (HD / 2)];
+  for (int k = 0; k < AHEAD; ++k) x[k] = part[min(k, own - 1) * (HD / 2)];
   float2 ml = make_float2(-INFINITY, 0.f);
-  if (lane < slots)
-    ml = reinterpret_cast<const float2*>(a.part_ml)[row * slots + lane];
-  if (lane < a.nshared && prefix_len(a, b, row_len(a, b)) == 0)
-    ml = make_float2(-INFINITY, 0.f);
+  if (lane < own)
+    ml = reinterpret_cast<const float2*>(a.part_ml)[row * own + lane];
+  int joined = 0;
+  const float2* pre = nullptr;
+  const int64_t step = (int64_t)a.hkv * TILE * (HD / 2);
+  if (prefix_len(a, b, row_len(a, b)) > 0) {
+    const int4 at = a.pre_at[b];
+    const int head = (int)(row % a.hq);
+    const int64_t r = prefix_row(a, at, head / a.G) + head % a.G;
+    joined = at.y;
+    pre = reinterpret_cast<const float2*>(a.pre_o + r * HD) + lane;
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) y[k] = pre[min(k, joined - 1) * step];
+    if (lane >= own && lane - own < joined)
+      ml = reinterpret_cast<const float2*>(
+          a.pre_ml)[r + (int64_t)(lane - own) * a.hkv * TILE];
+  }
   float M, L;
   const float w = join_weight(ml.x, ml.y, M, L);
   float2 acc = make_float2(0.f, 0.f);
@@ -442,9 +478,14 @@ __global__ __launch_bounds__(4 * WAVE) void paged_join_kernel(
   };
 #pragma unroll
   for (int k = 0; k < AHEAD; ++k)
-    if (k < slots) add(k, x[k]);
+    if (k < own) add(k, x[k]);
 #pragma unroll 8
-  for (int k = AHEAD; k < slots; ++k) add(k, part[k * (HD / 2)]);
+  for (int k = AHEAD; k < own; ++k) add(k, part[k * (HD / 2)]);
+#pragma unroll
+  for (int k = 0; k < AHEAD; ++k)
+    if (k < joined) add(own + k, y[k]);
+#pragma unroll 8
+  for (int k = AHEAD; k < joined; ++k) add(own + k, pre[k * step]);
   const float inv = (L == 0.f) ? 0.f : 1.f / L;
   __hip_bfloat16* dst = out + row * HD + lane * 2;
   dst[0] = f2bf(L == 0.f ? 0.f : acc.x * inv);
@@ -453,14 +494,17 @@ __global__ __launch_bounds__(4 * WAVE) void paged_join_kernel(
 
 // -------------------------------------------------------- the shared prefix
 //
-// One block = (KV head, split of the prefix, tile of up to 128 query rows of
-// one group): rows (b, g) of the group's members in batch order.  4 waves own
-// 32 rows each; pages of K and V pass through LDS, double-buffered, the next
+// A tile is up to 128 query rows (b, g) of one group's members, in batch order;
+// its work is its prefix's pages.  A KV head's blocks take equal runs of all
+// its tiles' pages, one after the other, as the groups are on the device: a
+// block may end one tile and begin the next, each such piece leaves a partial
+// result, and no block idles for the number of rows or groups.  4 waves own 32
+// rows each; pages of K and V pass through LDS, double-buffered, the next
 // page's loads in flight under this page's products.  Bound: the matrix
 // instructions and, at 32 rows a wave, LDS reads at the same rate (each 1 KB
 // fragment feeds one 32x32x16 product of 32 cycles, four SIMDs to 128 B a
 // cycle).  blockIdx.x is the KV head, so that with 8 of them each XCD's L2
-// holds one head's prefix for every tile and split.
+// holds one head's prefixes for every tile.
 template <bool FP8>
 __global__ __launch_bounds__(4 * WAVE, 2) void paged_shared_kernel(
     const Paged a) {
@@ -469,238 +513,292 @@ __global__ __launch_bounds__(4 * WAVE, 2) void paged_shared_kernel(
   __hip_bfloat16 lds[2 * KVPAGE * (K_PITCH + V_PITCH32)];
   __hip_bfloat16* const k_lds = lds;
   __hip_bfloat16* const v_lds = lds + 2 * KVPAGE * K_PITCH;
-  __shared__ int counts[MAXGROUPS];
-  __shared__ int tile_rows[128];
-  __shared__ int tile_of[2];           // group, rows
+  // of each group: rows, prefix, its pages, tiles before it, work before and
+  // up to its end
+  __shared__ int counts[MAXGROUPS], g_len[MAXGROUPS], g_pages[MAXGROUPS],
+      g_tile0[MAXGROUPS], g_work0[MAXGROUPS], g_work1[MAXGROUPS];
+  __shared__ int2 all_work;  // pages of all tiles, of the longest prefix
+  __shared__ int tile_rows[TILE];
+  __shared__ int tile_count;
   __shared__ unsigned long long longest;  // length of a tile's row << 32 | row
 
-  const int kvh = blockIdx.x, split = blockIdx.y, tile = blockIdx.z;
+  const int kvh = blockIdx.x, block = blockIdx.y;
   const int tid = threadIdx.x;
-  const int wid = tid / WAVE, lane = tid % WAVE;
-  const int per_tile = 128 / a.G;
+  const int wid = __builtin_amdgcn_readfirstlane(tid / WAVE);
+  const int lane = tid % WAVE;
+  const int r32 = lane & 31, h = lane >> 5;
+  const int per_tile = TILE / a.G;
 
-  // ---- which group's which rows: each row's group goes to LDS (a byte, in
-  // what the pages take later) and is counted, one wave walks the tiles and then the
-  // members in batch order
-  unsigned char* groups = reinterpret_cast<unsigned char*>(lds);
-  static_assert(MAXB <= sizeof(lds), "a byte a row");
+  // ---- the groups' tiles and work, one group a lane
   if (tid < MAXGROUPS) counts[tid] = 0;
-  if (tid == 0) {
-    tile_of[0] = -1;
-    longest = 0;
-  }
   __syncthreads();
+  const int len = lane < a.ngroups ? max(a.group_lens[lane], 0) : 0;
+  const int first = tid < a.B ? a.group[tid] : -1;
   for (int b = tid; b < a.B; b += 4 * WAVE) {
-    const int g = a.group[b];
-    const bool in = g >= 0 && g < a.ngroups;
-    groups[b] = in ? g : 255;
-    if (in) atomicAdd(&counts[g], 1);
+    const int g = b == tid ? first : a.group[b];
+    if (g >= 0 && g < a.ngroups) atomicAdd(&counts[g], 1);
   }
   __syncthreads();
   if (wid == 0) {
+    const int pages = min((len + KVPAGE - 1) / KVPAGE, a.max_pages);
     const int tiles = (counts[lane] + per_tile - 1) / per_tile;
-    int upto = tiles;
+    int tiles_to = tiles, work = tiles * pages;
+    int most = tiles > 0 ? pages : 0;
 #pragma unroll
     for (int off = 1; off < WAVE; off <<= 1) {
-      const int x = __shfl_up(upto, off, WAVE);
-      if (lane >= off) upto += x;
+      const int x = __shfl_up(tiles_to, off, WAVE);
+      const int y = __shfl_up(work, off, WAVE);
+      if (lane >= off) {
+        tiles_to += x;
+        work += y;
+      }
+      most = max(most, __shfl_xor(most, off, WAVE));
     }
-    const unsigned long long mine =
-        __ballot(tile >= upto - tiles && tile < upto);
-    if (mine) {
-      const int g = 63 - __clzll((long long)mine);
-      const int skip =
-          (tile - __builtin_amdgcn_readlane(upto - tiles, g)) * per_tile;
+    g_len[lane] = len;
+    g_pages[lane] = pages;
+    g_tile0[lane] = tiles_to - tiles;
+    g_work0[lane] = work - tiles * pages;
+    g_work1[lane] = work;
+    if (lane == WAVE - 1) all_work = make_int2(work, most);
+  }
+  __syncthreads();
+  const int work = __builtin_amdgcn_readfirstlane(all_work.x);
+  // a tile ends in up to one piece more than its pages fill
+  const int each =
+      max(max((work + a.npre - 1) / a.npre, LEAST),
+          (__builtin_amdgcn_readfirstlane(all_work.y) + MAXPIECES - 2) /
+              (MAXPIECES - 1));
+  const int work_end = min(work, (block + 1) * each);
+  int at = block * each;
+  while (at < work_end) {
+    // ---- this piece's group, tile, pages and rows: each row's group goes to
+    // LDS (a byte, in what the pages take later), one wave walks the members
+    const int grp = __ffsll((long long)__ballot(at < g_work1[lane])) - 1;
+    const int pages = __builtin_amdgcn_readfirstlane(g_pages[grp]);
+    const int into = at - __builtin_amdgcn_readfirstlane(g_work0[grp]);
+    const int tile = into / pages;  // of the group's
+    const int pbegin = into % pages;
+    const int piece =
+        block + tile + __builtin_amdgcn_readfirstlane(g_tile0[grp]);
+    const int taken = min(pages - pbegin, work_end - at);
+    const int tile_end = at - pbegin + pages;  // in the head's work
+    at += taken;
+
+    unsigned char* groups = reinterpret_cast<unsigned char*>(lds);
+    static_assert(MAXB <= sizeof(lds), "a byte a row");
+    __syncthreads();  // nothing reads the last piece's pages or rows
+    for (int b = tid; b < a.B; b += 4 * WAVE)
+      groups[b] = (b == tid ? first : a.group[b]) == grp;
+    if (tid == 0) longest = 0;
+    __syncthreads();
+    if (wid == 0) {
+      const int skip = tile * per_tile;
       int seen = 0;
       for (int b0 = 0; b0 < a.B && seen < skip + per_tile; b0 += WAVE) {
-        const bool in = b0 + lane < a.B && groups[b0 + lane] == g;
+        const bool in = b0 + lane < a.B && groups[b0 + lane];
         const unsigned long long bal = __ballot(in);
         const int rank = seen + __popcll(bal & ((1ull << lane) - 1)) - skip;
         if (in && rank >= 0 && rank < per_tile) tile_rows[rank] = b0 + lane;
         seen += __popcll(bal);
       }
-      if (lane == 0) {
-        tile_of[0] = g;
-        tile_of[1] = min(seen - skip, per_tile);
-      }
+      if (lane == 0) tile_count = min(seen - skip, per_tile);
     }
-  }
-  __syncthreads();
-  const int grp = tile_of[0];
-  if (grp < 0) return;  // fewer tiles than blocks
-  const int nrows = tile_of[1] * a.G;
+    __syncthreads();
+    const int nrows = tile_count * a.G;
+    if (pbegin == 0 && kvh == 0 && tid < tile_count)
+      a.pre_at[tile_rows[tid]] =
+          make_int4(piece, (tile_end - 1) / each - block + 1, tid, 0);
 
-  // ---- this wave's 32 query rows: one a lane, halves h of the MFMA's K
-  const int r32 = lane & 31, h = lane >> 5;
-  const int i = wid * 32 + r32;
-  const bool live = i < nrows;
-  const int b = tile_rows[live ? i / a.G : 0];
-  const int head = kvh * a.G + (live ? i % a.G : 0);
-  const bool wave_live = wid * 32 < nrows;
-  const int len = row_len(a, b);
-  bf16x8v qf[8];
+    // ---- this wave's 32 query rows: one a lane, halves h of the MFMA's K
+    const int i = wid * 32 + r32;
+    const bool live = i < nrows;
+    const int b = tile_rows[live ? i / a.G : 0];
+    const int head = kvh * a.G + (live ? i % a.G : 0);
+    const bool wave_live = wid * 32 < nrows;
+    const int n = row_len(a, b);
+    bf16x8v qf[8];
 #pragma unroll
-  for (int k = 0; k < 8; ++k)
-    qf[k] = load_q(a, a.q + b * a.q_stride + head * HD + k * 16 + h * 8);
-  if (live) atomicMax(&longest, (unsigned long long)len << 32 | (unsigned)b);
-  __syncthreads();
-  // the longest row's pages, and no token past it: what lies there, or in the
-  // table past a shorter row, may be anything
-  const int glen = min(max(a.group_lens[grp], 0), (int)(longest >> 32));
-  const int32_t* table =
-      a.page_table + (int64_t)(unsigned)longest * a.max_pages;
-  // a lane without a row computes row 0 again and writes nothing
-  const int limit = live ? min(len, glen) : glen;
-  const int npages = (glen + KVPAGE - 1) / KVPAGE;
-  const int each = (npages + a.nshared - 1) / a.nshared;
-  const int pbegin = split * each;
-  const int pend = min(npages, pbegin + each);
+    for (int k = 0; k < 8; ++k)
+      qf[k] = load_q(a, a.q + b * a.q_stride + head * HD + k * 16 + h * 8);
+    if (live) atomicMax(&longest, (unsigned long long)n << 32 | (unsigned)b);
+    __syncthreads();
+    // the longest row's pages, and no token past it: what lies there, or in the
+    // table past a shorter row, may be anything
+    const int glen = min(g_len[grp], (int)(longest >> 32));
+    const int32_t* table =
+        a.page_table + (int64_t)(unsigned)longest * a.max_pages;
+    // a lane without a row computes row 0 again and writes nothing
+    const int limit = live ? min(n, glen) : glen;
+    const int pend = min((glen + KVPAGE - 1) / KVPAGE, pbegin + taken);
 
-  float m = -INFINITY, l = 0.f;
-  f32x16 o[4];
+    float m = -INFINITY, l = 0.f;
+    f32x16 o[4];
 #pragma unroll
-  for (int d = 0; d < 4; ++d)
+    for (int d = 0; d < 4; ++d)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+      for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
 
-  constexpr int LD = FP8 ? 2 : 4;     // 16 B loads of a thread, a page
-  constexpr int ROW = FP8 ? 8 : 16;   // threads of one row
-  u32x4 kr[LD], vr[LD];
-  unsigned char ks[LD], vs[LD];
-  const int trow = tid / ROW, tcol = tid % ROW;
+    constexpr int LD = FP8 ? 2 : 4;     // 16 B loads of a thread, a page
+    constexpr int ROW = FP8 ? 8 : 16;   // threads of one row
+    u32x4 kr[LD], vr[LD];
+    unsigned char ks[LD], vs[LD];
+    const int trow = tid / ROW, tcol = tid % ROW;
 
-  // page ids 64 at a time, one a lane: no load waits for another
-  int ids = 0;
-  auto fetch = [&](int pi) {
-    if ((pi - pbegin) % WAVE == 0) ids = pi + lane < pend ? table[pi + lane] : -1;
-    const int page = __builtin_amdgcn_readlane(ids, (pi - pbegin) % WAVE);
-    const bool ok = page >= 0 && page < a.num_pages;
-    const int64_t panel = ((int64_t)(ok ? page : 0) * a.hkv + kvh) * KVPAGE;
-    const char* kp = (const char*)a.kcache + panel * (FP8 ? HD : 2 * HD);
-    const char* vp = (const char*)a.vcache + panel * (FP8 ? HD : 2 * HD);
+    // page ids 64 at a time, one a lane: no load waits for another
+    int ids = 0;
+    auto fetch = [&](int pi) {
+      if ((pi - pbegin) % WAVE == 0)
+        ids = pi + lane < pend ? table[pi + lane] : -1;
+      const int page = __builtin_amdgcn_readlane(ids, (pi - pbegin) % WAVE);
+      const bool ok = page >= 0 && page < a.num_pages;
+      const int64_t panel = ((int64_t)(ok ? page : 0) * a.hkv + kvh) * KVPAGE;
+      const char* kp = (const char*)a.kcache + panel * (FP8 ? HD : 2 * HD);
+      const char* vp = (const char*)a.vcache + panel * (FP8 ? HD : 2 * HD);
 #pragma unroll
-    for (int j = 0; j < LD; ++j) {
-      kr[j] = *reinterpret_cast<const u32x4*>(kp + (j * 4 * WAVE + tid) * 16);
-      vr[j] = *reinterpret_cast<const u32x4*>(vp + (j * 4 * WAVE + tid) * 16);
-      if (FP8) {
-        const int64_t at = panel + j * (4 * WAVE / ROW) + trow;
-        ks[j] = a.kscale[at];
-        vs[j] = a.vscale[at];
+      for (int j = 0; j < LD; ++j) {
+        kr[j] = *reinterpret_cast<const u32x4*>(kp + (j * 4 * WAVE + tid) * 16);
+        vr[j] = *reinterpret_cast<const u32x4*>(vp + (j * 4 * WAVE + tid) * 16);
+        if (FP8) {
+          const int64_t at = panel + j * (4 * WAVE / ROW) + trow;
+          ks[j] = a.kscale[at];
+          vs[j] = a.vscale[at];
+        }
       }
+      return ok;
+    };
+    auto stage = [&](int buf, int pi) {
+      const bool whole = (pi + 1) * KVPAGE <= glen;
+#pragma unroll
+      for (int j = 0; j < LD; ++j) {
+        const int row = j * (4 * WAVE / ROW) + trow;
+        // beyond the prefix: zeros (NaN there times weight 0)
+        if (!whole && pi * KVPAGE + row >= glen) {
+          vr[j] = (u32x4){0, 0, 0, 0};
+          if (FP8) vs[j] = 127;
+        }
+        __hip_bfloat16* kd = &k_lds[(buf * KVPAGE + row) * K_PITCH];
+        __hip_bfloat16* vd = &v_lds[(buf * KVPAGE + row) * V_PITCH32];
+        if constexpr (FP8) {
+          u32x4 lo, hi;
+          widen(kr[j], e8m0_scale(ks[j]), lo, hi);
+          reinterpret_cast<u32x4*>(kd + tcol * 16)[0] = lo;
+          reinterpret_cast<u32x4*>(kd + tcol * 16)[1] = hi;
+          widen(vr[j], e8m0_scale(vs[j]), lo, hi);
+          reinterpret_cast<u32x4*>(vd + tcol * 16)[0] = lo;
+          reinterpret_cast<u32x4*>(vd + tcol * 16)[1] = hi;
+        } else {
+          reinterpret_cast<u32x4*>(kd + tcol * 8)[0] = kr[j];
+          reinterpret_cast<u32x4*>(vd + tcol * 8)[0] = vr[j];
+        }
+      }
+    };
+
+    bool ok = false;
+    if (pbegin < pend) {
+      ok = fetch(pbegin);
+      stage(0, pbegin);
     }
-    return ok;
-  };
-  auto stage = [&](int buf, int pi) {
-    const bool whole = (pi + 1) * KVPAGE <= glen;
-#pragma unroll
-    for (int j = 0; j < LD; ++j) {
-      const int row = j * (4 * WAVE / ROW) + trow;
-      // beyond the prefix: zeros (NaN there times weight 0)
-      if (!whole && pi * KVPAGE + row >= glen) {
-        vr[j] = (u32x4){0, 0, 0, 0};
-        if (FP8) vs[j] = 127;
-      }
-      __hip_bfloat16* kd = &k_lds[(buf * KVPAGE + row) * K_PITCH];
-      __hip_bfloat16* vd = &v_lds[(buf * KVPAGE + row) * V_PITCH32];
-      if constexpr (FP8) {
-        u32x4 lo, hi;
-        widen(kr[j], e8m0_scale(ks[j]), lo, hi);
-        reinterpret_cast<u32x4*>(kd + tcol * 16)[0] = lo;
-        reinterpret_cast<u32x4*>(kd + tcol * 16)[1] = hi;
-        widen(vr[j], e8m0_scale(vs[j]), lo, hi);
-        reinterpret_cast<u32x4*>(vd + tcol * 16)[0] = lo;
-        reinterpret_cast<u32x4*>(vd + tcol * 16)[1] = hi;
-      } else {
-        reinterpret_cast<u32x4*>(kd + tcol * 8)[0] = kr[j];
-        reinterpret_cast<u32x4*>(vd + tcol * 8)[0] = vr[j];
-      }
-    }
-  };
-
-  bool ok = false;
-  if (pbegin < pend) {
-    ok = fetch(pbegin);
-    stage(0, pbegin);
-  }
-  for (int pi = pbegin; pi < pend; ++pi) {
-    __syncthreads();  // this page is staged; the other buffer is free
-    const int buf = (pi - pbegin) & 1;
-    const bool cur = ok;
-    if (pi + 1 < pend) ok = fetch(pi + 1);
-    if (wave_live && cur) {
-      const __hip_bfloat16* kt = &k_lds[(buf * KVPAGE + r32) * K_PITCH + h * 8];
-      const __hip_bfloat16* vt =
-          &v_lds[(buf * KVPAGE + 4 * h + ((lane & 15) >> 2)) * V_PITCH32 +
-                 ((lane >> 4) & 1) * 16 + (lane & 3) * 4];
-      f32x16 s[2];
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[t][r] = 0.f;
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-          s[t] = MFMA32(*reinterpret_cast<const bf16x8v*>(
-                            kt + t * 32 * K_PITCH + k * 16),
-                        qf[k], s[t]);
-      const int left = limit - pi * KVPAGE;  // this row's tokens of the page
-      if (__any(left < KVPAGE)) {
+    for (int pi = pbegin; pi < pend; ++pi) {
+      __syncthreads();  // this page is staged; the other buffer is free
+      const int buf = (pi - pbegin) & 1;
+      const bool cur = ok;
+      if (pi + 1 < pend) ok = fetch(pi + 1);
+      if (wave_live && cur) {
+        const __hip_bfloat16* kt =
+            &k_lds[(buf * KVPAGE + r32) * K_PITCH + h * 8];
+        const __hip_bfloat16* vt =
+            &v_lds[(buf * KVPAGE + 4 * h + ((lane & 15) >> 2)) * V_PITCH32 +
+                   ((lane >> 4) & 1) * 16 + (lane & 3) * 4];
+        f32x16 s[2];
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (t * 32 + 8 * (r / 4) + 4 * h + r % 4 >= left)
-              s[t][r] = -INFINITY;
-      }
-      float mt = s[0][0];
+          for (int r = 0; r < 16; ++r) s[t][r] = 0.f;
 #pragma unroll
-      for (int j = 1; j < 32; ++j) mt = fmaxf(mt, s[j / 16][j % 16]);
-      mt = fmaxf(mt, __shfl_xor(mt, 32, WAVE));
-      const float mn = fmaxf(m, mt * a.scale_log2);
-      const float mu = (mn == -INFINITY) ? 0.f : mn;
-      if (__any(mn > m)) {  // a factor of 1 otherwise
-        const float keep = exp2_fast(m - mu);
-        l *= keep;
+        for (int k = 0; k < 8; ++k)
 #pragma unroll
-        for (int d = 0; d < 4; ++d) o[d] *= keep;
-      }
-      m = mn;
-      bf16x8v pf[4];
+          for (int t = 0; t < 2; ++t)
+            s[t] = MFMA32(*reinterpret_cast<const bf16x8v*>(
+                              kt + t * 32 * K_PITCH + k * 16),
+                          qf[k], s[t]);
+        // six fragments ahead of the products (the compiler's own order has
+        // two, each product waits for LDS: 27.4 us against 25.7 at 256 rows of
+        // 2048 shared tokens, bf16)
+        SCHED(DS_READ, 6);
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          pf[t * 2 + r / 8][r % 8] =
-              (__bf16)exp2_fast(fmaf(s[t][r], a.scale_log2, -mu));
+        for (int k = 0; k < 10; ++k) {
+          SCHED(MFMA, 1);
+          SCHED(DS_READ, 1);
         }
+        SCHED(MFMA, 6);
+        // this row's tokens of the page, from its lane's first one
+        const int left = limit - 4 * h - pi * KVPAGE;
+        if (__any(left < KVPAGE - 4 * h)) {
 #pragma unroll
-      for (int u = 0; u < 4; ++u) l = add8(pf[u], l);
+          for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-#pragma unroll
-        for (int d = 0; d < 4; ++d) {
-          const __hip_bfloat16* p = vt + u * 16 * V_PITCH32 + d * 32;
-          o[d] = MFMA32(join(read_tr(p), read_tr(p + 8 * V_PITCH32)), pf[u],
-                        o[d]);
+            for (int r = 0; r < 16; ++r)
+              if (t * 32 + 8 * (r / 4) + r % 4 >= left)
+                s[t][r] = -INFINITY;
         }
+        float mt = s[0][0];
+#pragma unroll
+        for (int j = 1; j < 32; ++j) mt = fmaxf(mt, s[j / 16][j % 16]);
+        mt = fmaxf(mt, __shfl_xor(mt, 32, WAVE));
+        const float mn = mt * a.scale_log2;
+        if (__any(mn > m + SLACK)) {
+          const float mu = fmaxf(m, mn);
+          const float keep = exp2_fast(m - (mu == -INFINITY ? 0.f : mu));
+          m = mu;
+          l *= keep;
+#pragma unroll
+          for (int d = 0; d < 4; ++d) o[d] *= keep;
+        }
+        const float mu = (m == -INFINITY) ? 0.f : m;
+        bf16x8v pf[4];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            pf[t * 2 + r / 8][r % 8] =
+                (__bf16)exp2_fast(fmaf(s[t][r], a.scale_log2, -mu));
+          }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) l = add8(pf[u], l);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+          for (int d = 0; d < 4; ++d) {
+            const __hip_bfloat16* p = vt + u * 16 * V_PITCH32 + d * 32;
+            o[d] = MFMA32(join(read_tr(p), read_tr(p + 8 * V_PITCH32)), pf[u],
+                          o[d]);
+          }
+        SCHED(DS_READ, 8);
+#pragma unroll
+        for (int k = 0; k < 12; ++k) {
+          SCHED(MFMA, 1);
+          SCHED(DS_READ, 2);
+        }
+        SCHED(MFMA, 4);
+      }
+      if (pi + 1 < pend) stage(buf ^ 1, pi + 1);
     }
-    if (pi + 1 < pend) stage(buf ^ 1, pi + 1);
-  }
 
-  l += __shfl_xor(l, 32, WAVE);
-  if (!live) return;
-  const int64_t slot =
-      ((int64_t)b * a.hq + head) * (a.nshared + a.nsplit) + split;
-  if (h == 0) reinterpret_cast<float2*>(a.part_ml)[slot] = make_float2(m, l);
+    l += __shfl_xor(l, 32, WAVE);
+    if (live) {
+      const int64_t slot =
+          prefix_row(a, make_int4(piece, 0, i / a.G, 0), kvh) + i % a.G;
+      if (h == 0) reinterpret_cast<float2*>(a.pre_ml)[slot] = make_float2(m, l);
 #pragma unroll
-  for (int d = 0; d < 4; ++d)
+      for (int d = 0; d < 4; ++d)
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      *reinterpret_cast<f32x4*>(
-          &a.part_o[slot * HD + d * 32 + r * 8 + h * 4]) =
-          (f32x4){o[d][r * 4], o[d][r * 4 + 1], o[d][r * 4 + 2],
-                  o[d][r * 4 + 3]};
+        for (int r = 0; r < 4; ++r)
+          *reinterpret_cast<f32x4*>(
+              &a.pre_o[slot * HD + d * 32 + r * 8 + h * 4]) =
+              (f32x4){o[d][r * 4], o[d][r * 4 + 1], o[d][r * 4 + 2],
+                      o[d][r * 4 + 3]};
+    }
+  }
 }
 
 #include <torch/extension.h>
@@ -764,13 +862,13 @@ Paged paged_args(const torch::Tensor& out, const torch::Tensor& q,
   return a;
 }
 
-// Splits of one row's (or tile's) pages so that `blocks` of them fill the
-// `room` blocks that the card holds at once; a split has at least `least` pages
-// of the widest table row (the lengths themselves are on the device).
-int splits_for(int64_t blocks, int64_t room, int pages, int least, int most) {
+// Splits of one row's pages so that `blocks` of them fill the `room` blocks
+// that the card holds at once, by the table's width (the lengths themselves
+// are on the device).
+int splits_for(int64_t blocks, int64_t room, int pages, int most) {
   const int64_t want = room / std::max<int64_t>(blocks, 1);
   return (int)std::max<int64_t>(
-      1, std::min<int64_t>({want, (pages + least - 1) / least, most}));
+      1, std::min<int64_t>({want, (pages + LEAST - 1) / LEAST, most}));
 }
 
 template <bool FP8>
@@ -785,16 +883,20 @@ void launch_decode(const Paged& a, torch::Tensor& out, hipStream_t s) {
                        (__hip_bfloat16*)out.data_ptr());
 }
 
-// The partial slots: of this call alone (the allocator orders its reuse on
-// the stream, and a captured graph keeps its own).
-torch::Tensor partials(Paged& a, const torch::Tensor& q) {
-  const int64_t slots = a.nshared + a.nsplit;
-  if (slots == 1) return torch::Tensor();
-  const int64_t rows = (int64_t)a.B * a.hq * slots;
-  auto work = torch::empty({rows * (HD + 2)},
+// The partial results, pieces of them the prefixes': of this call alone (the
+// allocator orders its reuse on the stream, and a captured graph keeps its own).
+torch::Tensor partials(Paged& a, const torch::Tensor& q, int64_t pieces) {
+  const int64_t own = a.nsplit > 1 ? (int64_t)a.B * a.hq * a.nsplit : 0;
+  const int64_t pre = pieces * a.hkv * TILE;
+  if (own + pre == 0) return torch::Tensor();
+  const int64_t at = pieces > 0 ? (int64_t)a.B * 4 : 0;
+  auto work = torch::empty({(own + pre) * (HD + 2) + at},
                            q.options().dtype(torch::kFloat32));
   a.part_o = (float*)work.data_ptr();
-  a.part_ml = a.part_o + rows * HD;
+  a.pre_o = a.part_o + own * HD;
+  a.pre_at = (int4*)(a.pre_o + pre * HD);
+  a.part_ml = (float*)a.pre_at + at;
+  a.pre_ml = a.part_ml + own * 2;
   return work;
 }
 
@@ -811,8 +913,8 @@ void attn_decode_fp8(torch::Tensor out, torch::Tensor q, torch::Tensor kcache,
   a.kscale = (const uint8_t*)kscale.data_ptr();
   a.vscale = (const uint8_t*)vscale.data_ptr();
   c10::DeviceGuard guard(dev);
-  a.nsplit = splits_for((int64_t)a.B * a.hkv, 1024, a.max_pages, 2, 64);
-  const auto work = partials(a, q);
+  a.nsplit = splits_for((int64_t)a.B * a.hkv, 1024, a.max_pages, 64);
+  const auto work = partials(a, q, 0);
   launch_decode<true>(a, out, at::hip::getCurrentHIPStream().stream());
   HIP_CHECK_LAST();
 }
@@ -858,33 +960,32 @@ void attn_decode_shared(torch::Tensor out, torch::Tensor q,
   a.ngroups = (int)group_lens.size(0);
   c10::DeviceGuard guard(dev);
   hipStream_t s = at::hip::getCurrentHIPStream().stream();
-  a.nsplit = splits_for((int64_t)a.B * a.hkv, 768, a.max_pages, 2, 32);
-  if (a.ngroups > 0) {
+  a.nsplit = splits_for((int64_t)a.B * a.hkv, 768, a.max_pages, 32);
+  // each group may leave one tile part full; no more tiles than rows
+  const int per_tile = TILE / a.G;
+  const int64_t tiles =
+      std::min<int64_t>(a.B, (a.B + per_tile - 1) / per_tile + a.ngroups);
+  TORCH_CHECK(tiles * a.max_pages <= 1 << 30, "the page table is too large");
+  if (a.ngroups > 0 && a.max_pages > 0) {
     a.group = (const int32_t*)group.data_ptr();
     a.group_lens = (const int32_t*)group_lens.data_ptr();
-    const int per_tile = 128 / a.G;
-    const int full = (a.B + per_tile - 1) / per_tile;
-    // each group may leave one tile part full; no more tiles than rows
-    const int tiles = std::min<int>(a.B, full + a.ngroups);
-    a.nshared = splits_for((int64_t)tiles * a.hkv, 512, a.max_pages, 2, 32);
-    const auto work = partials(a, q);
-    const dim3 grid(a.hkv, a.nshared, tiles);
+    a.npre = (int)std::max<int64_t>(
+        1, std::min<int64_t>(512 / a.hkv,
+                             tiles * ((a.max_pages + LEAST - 1) / LEAST)));
+  }
+  const auto work = partials(a, q, a.npre > 0 ? a.npre + tiles : 0);
+  if (a.npre > 0) {
+    const dim3 grid(a.hkv, a.npre);
     if (fp8)
       hipLaunchKernelGGL((paged_shared_kernel<true>), grid, dim3(4 * WAVE), 0,
                          s, a);
     else
       hipLaunchKernelGGL((paged_shared_kernel<false>), grid, dim3(4 * WAVE), 0,
                          s, a);
-    if (fp8)
-      launch_decode<true>(a, out, s);
-    else
-      launch_decode<false>(a, out, s);
-  } else {
-    const auto work = partials(a, q);
-    if (fp8)
-      launch_decode<true>(a, out, s);
-    else
-      launch_decode<false>(a, out, s);
   }
+  if (fp8)
+    launch_decode<true>(a, out, s);
+  else
+    launch_decode<false>(a, out, s);
   HIP_CHECK_LAST();
 }

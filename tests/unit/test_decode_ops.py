@@ -497,6 +497,10 @@ def test_build_prefix_groups():
     assert one.tolist() == [0, 0, -1, 0, -1, -1, -1] and lens1.tolist() == [128]
     none, _ = ops.build_prefix_groups(table, lens, min_rows=4)
     assert (none == -1).all()
+    # (3 - 1) * 2 + (2 - 1) * 2 page reads are saved
+    for least, some in ((6, True), (7, False)):
+        group, _ = ops.build_prefix_groups(table, lens, min_saved=least)
+        assert bool((group >= 0).any()) == some
     none, _ = ops.build_prefix_groups(table[:0], lens[:0])
     assert none.shape == (0,)
 

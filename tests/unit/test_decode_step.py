@@ -63,10 +63,16 @@ def _staged(eng, n=6, **kw):
         eng.stop()
 
 
+@pytest.fixture(autouse=True)
+def _group_small_batches(monkeypatch):
+    monkeypatch.setattr(engine_mod, "MIN_SHARED_BYTES", 0)
+
+
 def test_fp8_cache_bytes_and_refusal():
     kv = KVCache(layers=2, kv_heads=3, head_dim=HD, num_pages=4, device="cpu",
                  dtype=torch.float8_e4m3fn)
     assert kv.bytes_per_page() == 2 * 2 * 3 * PAGE * (HD + 1)
+    assert kv.bytes_per_layer_page() == 2 * 3 * PAGE * (HD + 1)
     assert kv.kscale[0].shape == (4, 3, PAGE)
     assert KVCache(layers=2, kv_heads=3, head_dim=HD, num_pages=4,
                    device="cpu").kscale is None
@@ -87,7 +93,8 @@ def test_shared_prefix_engine_gives_the_same_tokens(monkeypatch):
     monkeypatch.setattr(ops, "build_prefix_groups", spy)
     grouped = _staged(_engine(shared_prefix=True))
     assert max(seen) >= 2, "no run shared a prefix"
-    monkeypatch.setattr(engine_mod, "MIN_PREFIX_PAGES", 1 << 20)
+    monkeypatch.undo()  # so few rows are not worth a pass by the rule
+    monkeypatch.setattr(ops, "build_prefix_groups", spy)
     seen.clear()
     assert _staged(_engine(shared_prefix=True)) == grouped
     assert max(seen) == 0
