@@ -34,8 +34,19 @@
 #define MAXGROUPS 64   // prefix groups of one call: one wave finds a tile's
 #define MAXB 65535     // rows of one call
 #define TILE 128       // query rows of one block in the shared pass
-#define MAXPIECES 32   // of one tile's prefix
-#define LEAST 2        // pages of a piece or of a split, at least
+// Blocks of a launch, two a CU.  Own tokens, cold, e4m3, 32/8 heads: 8 rows of
+// 32768 tokens 161 us at 256, 159 at 512, 165 at 1024; 64 rows of 1000 tokens
+// 52.9, 52.2, 56.4.  Shared pass, 512 rows in 3 groups of 8192 tokens: 232 us
+// at 256 blocks, 213 at 512, 221 at 1024 (the rest of the call included).
+#define ROOM 512
+// Pages of a split or of a prefix's piece, at least.  One row of 777 tokens:
+// 12.1 us at 1, 10.1 at 2, 11.9 at 4; 4 rows of 1024 shared tokens 22.4, 21.0,
+// 23.9.
+#define LEAST 2
+// Splits of a row and pieces of a tile's prefix, at most: each one's o is read
+// again.  One row of 8192 tokens: 20.5 us at 32, 28.0 at 64.  Both together are
+// joined by one wave.
+#define MAXPARTS 32
 #define SLACK 8.f      // log2 by which a weight may pass 1
 
 using f32x4 = __attribute__((ext_vector_type(4))) float;
@@ -167,16 +178,25 @@ __device__ __forceinline__ float join_weight(const float m, const float l,
 // One block = (row, KV head, split): NW waves take the split's half pages in
 // turn.  A wave reads K straight into A fragments (a lane's 16 B of one token;
 // the Q fragments take the dims in the same order) and turns V in its own LDS
-// rows, so that the loop has no block barrier.  Half pages, because 128 (bf16:
-// 168) registers and 9 KB a wave let 4 (3) blocks share a CU: what hides the
-// loads' latency is other waves.  Page ids come 64 at a time, one a lane.
-// Bound: the bytes of the cache; the matrix instructions run mostly empty (G
-// of 16 columns) and still take a tenth of the vector instructions that dot
-// products would.
+// rows, so that the loop has no block barrier.  Half pages, because 122
+// registers and 9 KB a wave let 4 blocks share a CU: what hides the loads'
+// latency is other waves (whole pages: 2 blocks, 55.9 us where this takes 49;
+// the next half page's loads under this one's products gained nothing).  Page
+// ids come 64 at a time, one a lane.
+//
+// Bound: the bytes of the cache, in random panels of 4 KB (bf16: 8 KB) halves:
+// a kernel that only loads them, cold, reaches 3.5 to 3.9 TB/s where a plain
+// read of one block of memory reaches 6.1.  Measured, e4m3, 32/8 heads: 256
+// rows of up to 700 tokens 49 us, 4.2 TB/s; 8 rows of up to 32768 tokens (64/8
+// heads) 92 us, 5.0 TB/s; one row of 777 tokens (8/2 heads) 9.6 us, of which the
+// join is 4.  The matrix instructions run mostly empty (G of 16 columns) and
+// still take a tenth of the vector instructions that dot products would.
 #define UNIT 32  // tokens of one step
 
-template <bool FP8, int NW>
-__global__ __launch_bounds__(NW* WAVE, FP8 ? 4 : 3) void paged_decode_kernel(
+#define NW 4  // waves of a block
+
+template <bool FP8>
+__global__ __launch_bounds__(NW * WAVE, 4) void paged_decode_kernel(
     const Paged a, __hip_bfloat16* __restrict__ out) {
   __shared__ __attribute__((aligned(16)))
   __hip_bfloat16 v_lds[NW][UNIT * V_PITCH];
@@ -439,7 +459,7 @@ __global__ __launch_bounds__(4 * WAVE) void paged_join_kernel(
   if (row >= (int64_t)a.B * a.hq) return;
   const int lane = threadIdx.x % WAVE;
   const int b = (int)(row / a.hq);  // one a wave: its branches are uniform
-  const int own = a.nsplit;  // up to 32 where rows have prefixes, 64 if not
+  const int own = a.nsplit;  // up to 32, as of prefixes
   // The first o's are on their way before their weights are known: what is
   // not written (an empty range) weighs nothing.
   constexpr int AHEAD = 8;
@@ -503,8 +523,11 @@ __global__ __launch_bounds__(4 * WAVE) void paged_join_kernel(
 // page's loads in flight under this page's products.  Bound: the matrix
 // instructions and, at 32 rows a wave, LDS reads at the same rate (each 1 KB
 // fragment feeds one 32x32x16 product of 32 cycles, four SIMDs to 128 B a
-// cycle).  blockIdx.x is the KV head, so that with 8 of them each XCD's L2
-// holds one head's prefixes for every tile.
+// cycle); of 2 waves a SIMD neither is kept busy alone.  Measured: 512 rows
+// (32/8 heads) in 3 groups of 8192 e4m3 tokens 102 us, 670 TFLOP/s, the matrix
+// units 40, vector units 45 and LDS 42 in a hundred cycles; 256 rows of 2048
+// bf16 tokens 25.7 us.  blockIdx.x is the KV head, so that with 8 of them each
+// XCD's L2 holds one head's prefixes for every tile.
 template <bool FP8>
 __global__ __launch_bounds__(4 * WAVE, 2) void paged_shared_kernel(
     const Paged a) {
@@ -566,8 +589,8 @@ __global__ __launch_bounds__(4 * WAVE, 2) void paged_shared_kernel(
   // a tile ends in up to one piece more than its pages fill
   const int each =
       max(max((work + a.npre - 1) / a.npre, LEAST),
-          (__builtin_amdgcn_readfirstlane(all_work.y) + MAXPIECES - 2) /
-              (MAXPIECES - 1));
+          (__builtin_amdgcn_readfirstlane(all_work.y) + MAXPARTS - 2) /
+              (MAXPARTS - 1));
   const int work_end = min(work, (block + 1) * each);
   int at = block * each;
   while (at < work_end) {
@@ -862,19 +885,18 @@ Paged paged_args(const torch::Tensor& out, const torch::Tensor& q,
   return a;
 }
 
-// Splits of one row's pages so that `blocks` of them fill the `room` blocks
-// that the card holds at once, by the table's width (the lengths themselves
-// are on the device).
-int splits_for(int64_t blocks, int64_t room, int pages, int most) {
-  const int64_t want = room / std::max<int64_t>(blocks, 1);
+// Splits of one row's pages so that `blocks` of them make ROOM, by the table's
+// width (the lengths themselves are on the device).
+int splits_for(int64_t blocks, int pages) {
+  const int64_t want = ROOM / std::max<int64_t>(blocks, 1);
   return (int)std::max<int64_t>(
-      1, std::min<int64_t>({want, (pages + LEAST - 1) / LEAST, most}));
+      1, std::min<int64_t>({want, (pages + LEAST - 1) / LEAST, MAXPARTS}));
 }
 
 template <bool FP8>
 void launch_decode(const Paged& a, torch::Tensor& out, hipStream_t s) {
   const dim3 grid(a.hkv, a.B, a.nsplit);
-  hipLaunchKernelGGL((paged_decode_kernel<FP8, 4>), grid, dim3(4 * WAVE), 0, s,
+  hipLaunchKernelGGL((paged_decode_kernel<FP8>), grid, dim3(NW * WAVE), 0, s,
                      a, (__hip_bfloat16*)out.data_ptr());
   if (a.nsplit > 1)
     hipLaunchKernelGGL(paged_join_kernel,
@@ -913,7 +935,7 @@ void attn_decode_fp8(torch::Tensor out, torch::Tensor q, torch::Tensor kcache,
   a.kscale = (const uint8_t*)kscale.data_ptr();
   a.vscale = (const uint8_t*)vscale.data_ptr();
   c10::DeviceGuard guard(dev);
-  a.nsplit = splits_for((int64_t)a.B * a.hkv, 1024, a.max_pages, 64);
+  a.nsplit = splits_for((int64_t)a.B * a.hkv, a.max_pages);
   const auto work = partials(a, q, 0);
   launch_decode<true>(a, out, at::hip::getCurrentHIPStream().stream());
   HIP_CHECK_LAST();
@@ -960,7 +982,7 @@ void attn_decode_shared(torch::Tensor out, torch::Tensor q,
   a.ngroups = (int)group_lens.size(0);
   c10::DeviceGuard guard(dev);
   hipStream_t s = at::hip::getCurrentHIPStream().stream();
-  a.nsplit = splits_for((int64_t)a.B * a.hkv, 768, a.max_pages, 32);
+  a.nsplit = splits_for((int64_t)a.B * a.hkv, a.max_pages);
   // each group may leave one tile part full; no more tiles than rows
   const int per_tile = TILE / a.G;
   const int64_t tiles =
@@ -970,7 +992,7 @@ void attn_decode_shared(torch::Tensor out, torch::Tensor q,
     a.group = (const int32_t*)group.data_ptr();
     a.group_lens = (const int32_t*)group_lens.data_ptr();
     a.npre = (int)std::max<int64_t>(
-        1, std::min<int64_t>(512 / a.hkv,
+        1, std::min<int64_t>(ROOM / a.hkv,
                              tiles * ((a.max_pages + LEAST - 1) / LEAST)));
   }
   const auto work = partials(a, q, a.npre > 0 ? a.npre + tiles : 0);

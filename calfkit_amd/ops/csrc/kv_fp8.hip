@@ -16,7 +16,10 @@
 //
 // Bound: bytes.  A row is 8 lanes x (8 low + 8 high) values: both halves of
 // the rotation pair (i, i + 64) sit in one lane as one 16 B load each, the
-// largest value takes three lane swaps, and a wave handles 8 rows.
+// largest value takes three lane swaps, and a wave handles 8 rows.  Measured,
+// rotate and write then read back, 32/8 heads: 12288 tokens 72.4 us, 4.96 TB/s,
+// the rate of a large copy (4.94); 512 tokens 8.0 us and one token 4.6 us on
+// the GPU, 4.6 us a call on the host.
 
 #include "common.h"
 #include "fp8.h"
