@@ -524,8 +524,8 @@ __global__ __launch_bounds__(4 * WAVE) void paged_join_kernel(
 // instructions and, at 32 rows a wave, LDS reads at the same rate (each 1 KB
 // fragment feeds one 32x32x16 product of 32 cycles, four SIMDs to 128 B a
 // cycle); of 2 waves a SIMD neither is kept busy alone.  Measured: 512 rows
-// (32/8 heads) in 3 groups of 8192 e4m3 tokens 102 us, 670 TFLOP/s, the matrix
-// units 40, vector units 45 and LDS 42 in a hundred cycles; 256 rows of 2048
+// (32/8 heads) in 3 groups of 8192 e4m3 tokens 102 us, 670 TFLOP/s, of a CU's
+// busy cycles the matrix units 35 %, vector units 40 %, LDS 37 %; 256 rows of 2048
 // bf16 tokens 25.7 us.  blockIdx.x is the KV head, so that with 8 of them each
 // XCD's L2 holds one head's prefixes for every tile.
 template <bool FP8>
