@@ -235,6 +235,12 @@ class InferenceEngine:
         #: for all of them.
         if kv_dtype not in ("bf16", "fp8"):
             raise ValueError(f"kv_dtype must be 'bf16' or 'fp8': {kv_dtype!r}")
+        if ((kv_dtype == "fp8" or shared_prefix)
+                and (model.dh != 128 or model.hq > 16 * model.hkv)):
+            raise ValueError(
+                "kv_dtype='fp8' and shared_prefix need heads of 128 and up to "
+                f"16 query heads a KV head, not {model.hq}/{model.hkv} heads "
+                f"of {model.dh}")
         #: TP/EP>1 serving runs in lockstep: rank 0 schedules and broadcasts
         #: each action; ranks > 0 replay them via follow() — every rank then
         #: executes identical forwards (and RCCL collectives) in identical

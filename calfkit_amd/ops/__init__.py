@@ -500,7 +500,8 @@ def attn_decode_shared(out: torch.Tensor, q: torch.Tensor,
     row by row, and the two are joined.  ``build_prefix_groups`` finds the
     groups.  The result is that of ``attn_decode`` (or, with the scales of
     an e4m3 cache, ``attn_decode_fp8``) up to the order of its sums, whatever
-    the grouping; a row may be shorter than its group's prefix.
+    the grouping; a row that ends inside its group's prefix is attended by
+    itself.
     """
     if _native(q):
         _K.attn_decode_shared(out, q, kcache, vcache, page_table, seq_lens,
@@ -536,8 +537,8 @@ def attn_decode_shared(out: torch.Tensor, q: torch.Tensor,
     def pages_of(b: int, count: int):
         pages = page_table[b, :count].long()
         g = int(group[b])
-        if g in lead:
-            upto = min(max(int(group_lens[g]), 0), count * 64)
+        if g in lead and group_lens[g] <= min(seq_lens[b], count * 64):
+            upto = max(int(group_lens[g]), 0)
             pages = pages.clone()
             # a prefix's last page may be its rows' own beyond the prefix
             pages[:upto // 64] = page_table[lead[g], :upto // 64].long()

@@ -137,12 +137,15 @@ __device__ __forceinline__ int row_len(const Paged& a, const int b) {
   return min(max(a.seq_lens[b], 0), a.max_pages * KVPAGE);
 }
 
-// Tokens of row b that its group's shared pass covers.
+// Tokens of row b that its group's shared pass covers: the prefix, or nothing
+// of a row that ends inside it (a weight of 0 would not keep out what a token
+// past the row's end holds, if that is not finite).
 __device__ __forceinline__ int prefix_len(const Paged& a, const int b,
                                           const int n) {
   if (a.group == nullptr) return 0;
   const int g = a.group[b];
-  return (g >= 0 && g < a.ngroups) ? min(max(a.group_lens[g], 0), n) : 0;
+  const int p = (g >= 0 && g < a.ngroups) ? max(a.group_lens[g], 0) : 0;
+  return p <= n ? p : 0;
 }
 
 // A row's first partial result of the prefix, for the first head of kvh; the
@@ -638,21 +641,21 @@ __global__ __launch_bounds__(4 * WAVE, 2) void paged_shared_kernel(
     const int b = tile_rows[live ? i / a.G : 0];
     const int head = kvh * a.G + (live ? i % a.G : 0);
     const bool wave_live = wid * 32 < nrows;
-    const int n = row_len(a, b);
     bf16x8v qf[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k)
       qf[k] = load_q(a, a.q + b * a.q_stride + head * HD + k * 16 + h * 8);
-    if (live) atomicMax(&longest, (unsigned long long)n << 32 | (unsigned)b);
+    // (a lane without a row computes row 0 again and writes nothing)
+    if (live)
+      atomicMax(&longest,
+                (unsigned long long)row_len(a, b) << 32 | (unsigned)b);
     __syncthreads();
-    // the longest row's pages, and no token past it: what lies there, or in the
-    // table past a shorter row, may be anything
-    const int glen = min(g_len[grp], (int)(longest >> 32));
+    // the longest row's pages (a shorter one's table may end before), none if
+    // it ends inside the prefix
+    const int glen = __builtin_amdgcn_readfirstlane(g_len[grp]);
     const int32_t* table =
         a.page_table + (int64_t)(unsigned)longest * a.max_pages;
-    // a lane without a row computes row 0 again and writes nothing
-    const int limit = live ? min(n, glen) : glen;
-    const int pend = min((glen + KVPAGE - 1) / KVPAGE, pbegin + taken);
+    const int pend = glen <= (int)(longest >> 32) ? pbegin + taken : pbegin;
 
     float m = -INFINITY, l = 0.f;
     f32x16 o[4];
@@ -754,9 +757,9 @@ __global__ __launch_bounds__(4 * WAVE, 2) void paged_shared_kernel(
           SCHED(DS_READ, 1);
         }
         SCHED(MFMA, 6);
-        // this row's tokens of the page, from its lane's first one
-        const int left = limit - 4 * h - pi * KVPAGE;
-        if (__any(left < KVPAGE - 4 * h)) {
+        if ((pi + 1) * KVPAGE > glen) {
+          // the prefix's tokens of the page, from this lane's first one
+          const int left = glen - pi * KVPAGE - 4 * h;
 #pragma unroll
           for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -962,6 +965,8 @@ void attn_decode_shared(torch::Tensor out, torch::Tensor q,
                       c->size(1) > 0 && c->is_contiguous() &&
                       c->sizes() == kcache.sizes(),
                   "the caches must be contiguous [P, Hkv, 64, 128]");
+      TORCH_CHECK(reinterpret_cast<uintptr_t>(c->data_ptr()) % 16 == 0,
+                  "the caches must start on 16 bytes");
     }
   }
   Paged a = paged_args(out, q, kcache, vcache, page_table, seq_lens, scale);

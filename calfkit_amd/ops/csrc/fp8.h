@@ -52,6 +52,8 @@ inline void check_fp8_cache(const torch::Tensor& kcache,
                     c->size(1) > 0 && c->is_contiguous() &&
                     c->sizes() == kcache.sizes(),
                 "the caches must be contiguous [P, Hkv, 64, 128]");
+    TORCH_CHECK(reinterpret_cast<uintptr_t>(c->data_ptr()) % 16 == 0,
+                "the caches must start on 16 bytes");
   }
   for (const auto* c : {&kscale, &vscale}) {
     TORCH_CHECK(c->device() == dev, "the scales are on another device");

@@ -267,6 +267,8 @@ void launch_rope(torch::Tensor& qkv, const torch::Tensor* work,
   TORCH_CHECK(qkv.scalar_type() == torch::kBFloat16 && qkv.dim() == 2 &&
                   qkv.is_contiguous() && qkv.size(1) == (hq + 2 * hkv) * HD,
               "qkv must be a contiguous bf16 [T, (hq + 2 hkv) * 128]");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(qkv.data_ptr()) % 16 == 0,
+              "qkv must start on 16 bytes");
   TORCH_CHECK(cos_sin.device() == dev &&
                   cos_sin.scalar_type() == torch::kFloat32 &&
                   cos_sin.dim() == 2 && cos_sin.size(1) == HD &&
@@ -282,6 +284,8 @@ void launch_rope(torch::Tensor& qkv, const torch::Tensor* work,
                     q_out->size(1) == hq && q_out->size(2) == HD &&
                     q_out->is_contiguous(),
                 "q_out must be a contiguous bf16 [T, hq, 128]");
+    TORCH_CHECK(reinterpret_cast<uintptr_t>(q_out->data_ptr()) % 16 == 0,
+                "q_out must start on 16 bytes");
     qo = q_out->data_ptr();
   }
   if (work != nullptr) {

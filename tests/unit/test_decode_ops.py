@@ -458,6 +458,22 @@ def test_attn_decode_shared_short_rows_first(device):
     _close(_shared(s, device), *_expect(s, HD ** -0.5))
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_attn_decode_shared_row_ends_inside_a_prefix_with_nan(device):
+    """What lies in the common pages past a row's end does not reach it."""
+    s = _shared_batch([0, 0, 0], [192], [9, 40, 77], 8, 2, fp8=False)
+    s["lens"][0] = 100
+    bad = int(s["table"][1, 1])              # tokens 64..127 of all rows
+    s["v"][bad, :, 100 - PAGE + 1:] = math.inf
+    s["k"][bad, :, 100 - PAGE + 1:] = math.nan
+    got = _shared(s, device)
+    assert not torch.isfinite(got[1:].float()).any()  # theirs to read
+    s["v"][bad, :, 100 - PAGE + 1:] = 0
+    s["k"][bad, :, 100 - PAGE + 1:] = 0
+    want, tol = _expect(s, HD ** -0.5)
+    _close(got[:1], want[:1], tol[:1])
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("B", [4097, 65535])
 def test_attn_decode_shared_most_rows(B):
@@ -548,6 +564,13 @@ def test_refusals(device):
     refused(rope, qkv, kc, vc, ks, vs, table[:, :64], i32, i32, 4, 2)
     refused(rope, qkv, kc, vc, ks, vs, table, i32.long(), i32, 4, 2)
     refused(rope, qkv, kc, vc, ks, vs, table, i32, i32, 4, 2, q_out=out.float())
+    if device == "cuda":  # 16 B accesses
+        odd = torch.zeros(qkv.numel() + 1, dtype=qkv.dtype, device=device)
+        refused(rope, odd[1:].view(qkv.shape), kc, vc, ks, vs, table, i32, i32,
+                4, 2)
+        shifted = torch.zeros(kc.numel() + 1, dtype=torch.uint8, device=device)
+        shifted = shifted[1:].view(torch.float8_e4m3fn).view(kc.shape)
+        refused(w, shifted, vc, ks, vs, rows, rows, i32)
     refused(ops.rope_qkv_write_slab_fp8, qkv,
             torch.zeros(8 * HD * 2, device=device), kc, vc, ks, vs, table,
             i32, i32, 4, 2, 2, 2)

@@ -3,6 +3,7 @@ prefixes and filtered draws, and a captured run of the three kernels."""
 
 import threading
 import time
+import types
 
 import pytest
 import torch
@@ -78,6 +79,10 @@ def test_fp8_cache_bytes_and_refusal():
                    device="cpu").kscale is None
     with pytest.raises(ValueError):
         _engine(kv_dtype="int4")
+    model = types.SimpleNamespace(dh=64, hq=8, hkv=2)
+    for kw in (dict(kv_dtype="fp8"), dict(shared_prefix=True)):
+        with pytest.raises(ValueError):
+            InferenceEngine(model, **kw)
 
 
 def test_shared_prefix_engine_gives_the_same_tokens(monkeypatch):
