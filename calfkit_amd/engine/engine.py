@@ -57,12 +57,13 @@ RUN_STEPS = (8, 4, 2, 1)
 #: prefix groups of one decode run (more share without being grouped)
 MAX_PREFIX_GROUPS = 16
 #: bytes of one layer's cache that groups save a step from being read, below
-#: which rows run without them: a pass over prefixes and its joins cost 5 to
-#: 9 us.  Measured with cold caches, 32/8 heads, bf16, groups against none:
-#: 126 MB (16 rows of 2048 shared tokens) 30.7 against 26.7 us, 132 MB (64 of
-#: 512) 38.0 / 37.7, 252 MB (16 of 4096) 36.6 / 38.5, 264 MB (64 of 1024)
-#: 40.5 / 46.2, 267 MB (256 of 256) 101 / 97, 528 MB (64 of 2048) 43.5 / 63.1
-MIN_SHARED_BYTES = 256 << 20
+#: which rows run without them: a pass over prefixes and its join cost up to
+#: 5 us.  Measured with cold caches, 32/8 heads, bf16, groups against none:
+#: 67 MB (256 rows of 64 shared tokens) 96.5 against 91.8 us, 66 MB (64 of 256)
+#: 32.2 / 31.1, 126 MB (16 of 2048) 25.2 / 25.1, 132 MB (64 of 512) 34.1 / 37.1,
+#: 134 MB (256 of 128) 95.0 / 93.8, 252 MB (16 of 4096) 28.9 / 36.2, 264 MB (64
+#: of 1024) 34.8 / 44.6
+MIN_SHARED_BYTES = 128 << 20
 
 #: lockstep op channel opcodes (tensor-coded: the
 #: pickled broadcast_object_list per visit becomes one fixed int64[2]

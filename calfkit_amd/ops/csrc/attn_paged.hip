@@ -34,11 +34,15 @@
 #define MAXGROUPS 64   // prefix groups of one call: one wave finds a tile's
 #define MAXB 65535     // rows of one call
 #define TILE 128       // query rows of one block in the shared pass
-// Blocks of a launch, two a CU.  Own tokens, cold, e4m3, 32/8 heads: 8 rows of
+// Blocks of a launch's own tokens, two a CU.  Cold, e4m3, 32/8 heads: 8 rows of
 // 32768 tokens 161 us at 256, 159 at 512, 165 at 1024; 64 rows of 1000 tokens
-// 52.9, 52.2, 56.4.  Shared pass, 512 rows in 3 groups of 8192 tokens: 232 us
-// at 256 blocks, 213 at 512, 221 at 1024 (the rest of the call included).
+// 52.9, 52.2, 56.4.
 #define ROOM 512
+// Blocks of its prefixes, one a CU, beside which one of own tokens runs.  512
+// rows in 3 groups of 8192 tokens (300 of their own, e4m3): 155 us at 192, 134
+// at 256, 143 at 384, 159 at 512; 256 rows of 2048 tokens (300, bf16): 65.1,
+// 66.8, 72.6, 77.3.
+#define PRE_ROOM 256
 // Pages of a split or of a prefix's piece, at least.  One row of 777 tokens:
 // 12.1 us at 1, 10.1 at 2, 11.9 at 4; 4 rows of 1024 shared tokens 22.4, 21.0,
 // 23.9.
@@ -125,6 +129,7 @@ struct Paged {
   float* pre_o;               // [pieces, hkv, 128, 128]
   float* pre_ml;              // [pieces, hkv, 128, 2]
   int4* pre_at;               // [B] where a row's are: first piece, pieces, row
+  int32_t* pre_has;           // [B] whether a row has any
   int64_t q_stride;
   int B, hq, hkv, G, max_pages, num_pages, ngroups;
   int nsplit;           // of each row's own tokens
@@ -198,14 +203,16 @@ __device__ __forceinline__ float join_weight(const float m, const float l,
 
 #define NW 4  // waves of a block
 
-template <bool FP8>
-__global__ __launch_bounds__(NW * WAVE, 4) void paged_decode_kernel(
-    const Paged a, __hip_bfloat16* __restrict__ out) {
-  __shared__ __attribute__((aligned(16)))
-  __hip_bfloat16 v_lds[NW][UNIT * V_PITCH];
-  __shared__ float ml_lds[NW][MAXG][2];
+struct OwnLds {
+  __hip_bfloat16 v[NW][UNIT * V_PITCH];
+  float ml[NW][MAXG][2];
+};
 
-  const int kvh = blockIdx.x, b = blockIdx.y, split = blockIdx.z;
+template <bool FP8>
+__device__ __forceinline__ void own_tokens(const Paged& a,
+                                           __hip_bfloat16* __restrict__ out,
+                                           const int kvh, const int b,
+                                           const int split, OwnLds& L) {
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
   const int lane = threadIdx.x % WAVE;
   const int l16 = lane & 15, g4 = lane >> 4;
@@ -235,7 +242,7 @@ __global__ __launch_bounds__(NW * WAVE, 4) void paged_decode_kernel(
 #pragma unroll
   for (int d = 0; d < 8; ++d) o[d] = (f32x4){0.f, 0.f, 0.f, 0.f};
 
-  __hip_bfloat16* vt = v_lds[wid];
+  __hip_bfloat16* vt = L.v[wid];
   const __hip_bfloat16* vt_read =
       vt + (g4 * 4 + (l16 >> 2)) * V_PITCH + (l16 & 3) * 4;
   const int32_t* table = a.page_table + (int64_t)b * a.max_pages;
@@ -359,30 +366,15 @@ __global__ __launch_bounds__(NW * WAVE, 4) void paged_decode_kernel(
   l += __shfl_xor(l, 16, WAVE);
   l += __shfl_xor(l, 32, WAVE);
 
-  // ---- join the waves and, where this block writes the output, the prefix's
-  // partial results: O rows over the V rows, now free
-  int4 at = make_int4(0, 0, 0, 0);
-  if (a.nsplit == 1 && first > 0) at = a.pre_at[b];
-  const int joined = at.y;
-  const int64_t pre = prefix_row(a, at, kvh);
-  // the prefix's first o's are on their way before their weights are known
-  constexpr int AHEAD = 4;
-  float2 ahead[AHEAD];
-  const auto early = [&](const float* part) __attribute__((always_inline)) {
-#pragma unroll
-    for (int k = 0; k < AHEAD; ++k)
-      if (k < joined)
-        ahead[k] =
-            *reinterpret_cast<const float2*>(part +
-                                             (int64_t)k * a.hkv * (TILE * HD));
-  };
-  if (threadIdx.x < a.G * (HD / 2))
-    early(a.pre_o + (pre + threadIdx.x / (HD / 2)) * HD +
-          threadIdx.x % (HD / 2) * 2);
+  // ---- join the waves: O rows over the V rows, now free.  The whole row
+  // where nothing else is joined to it, else a partial result
+  const bool whole_row = a.nsplit == 1 && first == 0;
+  if (a.npre > 0 && kvh == 0 && split == 0 && threadIdx.x == 0)
+    a.pre_has[b] = first > 0;
   __syncthreads();
-  float* o_lds = reinterpret_cast<float*>(&v_lds[0][0]);  // [NW][16][128]
-  float* w_lds = o_lds + NW * MAXG * HD;                  // [16][64]
-  static_assert((NW * MAXG * HD + MAXG * WAVE) * 4 <= sizeof(v_lds),
+  float* o_lds = reinterpret_cast<float*>(&L.v[0][0]);  // [NW][16][128]
+  float* w_lds = o_lds + NW * MAXG * HD;                 // [16][NW]
+  static_assert((NW * MAXG * HD + MAXG * NW) * 4 <= sizeof(L.v),
                 "O and the weights fit V's rows");
   if (l16 < a.G) {
 #pragma unroll
@@ -390,61 +382,40 @@ __global__ __launch_bounds__(NW * WAVE, 4) void paged_decode_kernel(
       *reinterpret_cast<f32x4*>(
           &o_lds[(wid * MAXG + l16) * HD + d * 16 + g4 * 4]) = o[d];
     if (g4 == 0) {
-      ml_lds[wid][l16][0] = m;
-      ml_lds[wid][l16][1] = l;
+      L.ml[wid][l16][0] = m;
+      L.ml[wid][l16][1] = l;
     }
   }
   __syncthreads();
   for (int g = wid; g < a.G; g += NW) {
     const int64_t row = (int64_t)b * a.hq + kvh * a.G + g;
-    float mk = -INFINITY, lk = 0.f, M, L;
+    float mk = -INFINITY, lk = 0.f, M, S;
     if (lane < NW) {
-      mk = ml_lds[lane][g][0];
-      lk = ml_lds[lane][g][1];
-    } else if (lane - NW < joined) {
-      const float2 ml = reinterpret_cast<const float2*>(
-          a.pre_ml)[pre + g + (int64_t)(lane - NW) * a.hkv * TILE];
-      mk = ml.x;
-      lk = ml.y;
+      mk = L.ml[lane][g][0];
+      lk = L.ml[lane][g][1];
     }
-    const float w = join_weight(mk, lk, M, L);
+    const float w = join_weight(mk, lk, M, S);
     // no weight at all (an empty row): zeros
-    w_lds[g * WAVE + lane] = a.nsplit > 1 ? w : L == 0.f ? 0.f : w / L;
-    if (a.nsplit > 1 && lane == 0)
+    if (lane < NW)
+      w_lds[g * NW + lane] = !whole_row ? w : S == 0.f ? 0.f : w / S;
+    if (!whole_row && lane == 0)
       reinterpret_cast<float2*>(a.part_ml)[row * a.nsplit + split] =
-          make_float2(M, L);
+          make_float2(M, S);
   }
   __syncthreads();
   for (int i = threadIdx.x; i < a.G * (HD / 2); i += NW * WAVE) {
     const int g = i / (HD / 2), d = i % (HD / 2) * 2;
     const int64_t row = (int64_t)b * a.hq + kvh * a.G + g;
-    const float* part = a.pre_o + (pre + g) * HD + d;
-    if (i != (int)threadIdx.x) early(part);
     float2 acc = make_float2(0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < NW; ++k) {
-      const float w = w_lds[g * WAVE + k];
+      const float w = w_lds[g * NW + k];
       const float2 x =
           *reinterpret_cast<const float2*>(&o_lds[(k * MAXG + g) * HD + d]);
       acc.x = fmaf(w, x.x, acc.x);
       acc.y = fmaf(w, x.y, acc.y);
     }
-    // an empty range has weight 0 and its o, read all the same (no branch
-    // between the loads), is not written
-    const auto add = [&](const int k, const float2 x)
-        __attribute__((always_inline)) {
-      const float w = w_lds[g * WAVE + NW + k];
-      acc.x = w == 0.f ? acc.x : fmaf(w, x.x, acc.x);
-      acc.y = w == 0.f ? acc.y : fmaf(w, x.y, acc.y);
-    };
-#pragma unroll
-    for (int k = 0; k < AHEAD; ++k)
-      if (k < joined) add(k, ahead[k]);
-#pragma unroll 4
-    for (int k = AHEAD; k < joined; ++k)
-      add(k, *reinterpret_cast<const float2*>(part + (int64_t)k * a.hkv *
-                                                         (TILE * HD)));
-    if (a.nsplit == 1) {
+    if (whole_row) {
       __hip_bfloat16* dst = out + row * HD + d;
       dst[0] = f2bf(acc.x);
       dst[1] = f2bf(acc.y);
@@ -458,10 +429,18 @@ __global__ __launch_bounds__(NW * WAVE, 4) void paged_decode_kernel(
 // Joins the partial slots of one (row, head): a wave each, 2 dims a lane.
 __global__ __launch_bounds__(4 * WAVE) void paged_join_kernel(
     const Paged a, __hip_bfloat16* __restrict__ out) {
-  const int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / WAVE;
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+  const int64_t row = (int64_t)blockIdx.x * 4 + wid;
   if (row >= (int64_t)a.B * a.hq) return;
   const int lane = threadIdx.x % WAVE;
   const int b = (int)(row / a.hq);  // one a wave: its branches are uniform
+  int4 at = make_int4(0, 0, 0, 0);
+  if (a.npre > 0) {
+    at = a.pre_at[b];  // not written where the row has none
+    if (a.pre_has[b] == 0) at.y = 0;
+  }
+  const int joined = at.y;
+  if (a.nsplit == 1 && joined == 0) return;  // written whole
   const int own = a.nsplit;  // up to 32, as of prefixes
   // The first o's are on their way before their weights are known: what is
   // not written (an empty range) weighs nothing.
@@ -470,25 +449,22 @@ __global__ __launch_bounds__(4 * WAVE) void paged_join_kernel(
       reinterpret_cast<const float2*>(a.part_o + row * own * HD) + lane;
   float2 x[AHEAD], y[AHEAD];
 #pragma unroll
-  for (int k = 0; k < AHEAD; ++k) x[k] = part[min(k, own - 1) * (HD / 2)];
+  for (int k = 0; k < AHEAD; ++k)
+    if (k < own) x[k] = part[k * (HD / 2)];
   float2 ml = make_float2(-INFINITY, 0.f);
   if (lane < own)
     ml = reinterpret_cast<const float2*>(a.part_ml)[row * own + lane];
-  int joined = 0;
-  const float2* pre = nullptr;
+  const int head = (int)(row - (int64_t)b * a.hq);
+  const int64_t first = prefix_row(a, at, head / a.G) + head % a.G;
   const int64_t step = (int64_t)a.hkv * TILE * (HD / 2);
-  if (prefix_len(a, b, row_len(a, b)) > 0) {
-    const int4 at = a.pre_at[b];
-    const int head = (int)(row % a.hq);
-    const int64_t r = prefix_row(a, at, head / a.G) + head % a.G;
-    joined = at.y;
-    pre = reinterpret_cast<const float2*>(a.pre_o + r * HD) + lane;
+  const float2* pre =
+      reinterpret_cast<const float2*>(a.pre_o + first * HD) + lane;
 #pragma unroll
-    for (int k = 0; k < AHEAD; ++k) y[k] = pre[min(k, joined - 1) * step];
-    if (lane >= own && lane - own < joined)
-      ml = reinterpret_cast<const float2*>(
-          a.pre_ml)[r + (int64_t)(lane - own) * a.hkv * TILE];
-  }
+  for (int k = 0; k < AHEAD; ++k)
+    if (k < joined) y[k] = pre[k * step];
+  if (lane >= own && lane - own < joined)
+    ml = reinterpret_cast<const float2*>(
+        a.pre_ml)[first + (int64_t)(lane - own) * a.hkv * TILE];
   float M, L;
   const float w = join_weight(ml.x, ml.y, M, L);
   float2 acc = make_float2(0.f, 0.f);
@@ -526,29 +502,29 @@ __global__ __launch_bounds__(4 * WAVE) void paged_join_kernel(
 // page's loads in flight under this page's products.  Bound: the matrix
 // instructions and, at 32 rows a wave, LDS reads at the same rate (each 1 KB
 // fragment feeds one 32x32x16 product of 32 cycles, four SIMDs to 128 B a
-// cycle); of 2 waves a SIMD neither is kept busy alone.  Measured: 512 rows
-// (32/8 heads) in 3 groups of 8192 e4m3 tokens 102 us, 670 TFLOP/s, of a CU's
-// busy cycles the matrix units 35 %, vector units 40 %, LDS 37 %; 256 rows of 2048
-// bf16 tokens 25.7 us.  blockIdx.x is the KV head, so that with 8 of them each
-// XCD's L2 holds one head's prefixes for every tile.
-template <bool FP8>
-__global__ __launch_bounds__(4 * WAVE, 2) void paged_shared_kernel(
-    const Paged a) {
+// cycle).  Measured by itself with two blocks a CU: 512 rows (32/8 heads) in 3
+// groups of 8192 e4m3 tokens 102 us, 670 TFLOP/s, of a CU's busy cycles the
+// matrix units 35 %, vector units 40 %, LDS 37 %; 256 rows of 2048 bf16 tokens
+// 25.7 us.  blockIdx.x % hkv is the KV head, so that with 8 of them each XCD's
+// L2 holds one head's prefixes for every tile.
+struct PrefixLds {
   // two pages of K, then two of V
-  __shared__ __attribute__((aligned(16)))
-  __hip_bfloat16 lds[2 * KVPAGE * (K_PITCH + V_PITCH32)];
-  __hip_bfloat16* const k_lds = lds;
-  __hip_bfloat16* const v_lds = lds + 2 * KVPAGE * K_PITCH;
+  __hip_bfloat16 pages[2 * KVPAGE * (K_PITCH + V_PITCH32)];
+  unsigned long long longest;  // length of a tile's row << 32 | row
+  int2 all_work;  // pages of all tiles, of the longest prefix
   // of each group: rows, prefix, its pages, tiles before it, work before and
   // up to its end
-  __shared__ int counts[MAXGROUPS], g_len[MAXGROUPS], g_pages[MAXGROUPS],
-      g_tile0[MAXGROUPS], g_work0[MAXGROUPS], g_work1[MAXGROUPS];
-  __shared__ int2 all_work;  // pages of all tiles, of the longest prefix
-  __shared__ int tile_rows[TILE];
-  __shared__ int tile_count;
-  __shared__ unsigned long long longest;  // length of a tile's row << 32 | row
+  int counts[MAXGROUPS], len[MAXGROUPS], pages_of[MAXGROUPS], tile0[MAXGROUPS],
+      work0[MAXGROUPS], work1[MAXGROUPS];
+  int tile_rows[TILE];
+  int tile_count;
+};
 
-  const int kvh = blockIdx.x, block = blockIdx.y;
+template <bool FP8>
+__device__ __forceinline__ void prefix_pieces(const Paged& a, const int kvh,
+                                              const int block, PrefixLds& L) {
+  __hip_bfloat16* const k_lds = L.pages;
+  __hip_bfloat16* const v_lds = L.pages + 2 * KVPAGE * K_PITCH;
   const int tid = threadIdx.x;
   const int wid = __builtin_amdgcn_readfirstlane(tid / WAVE);
   const int lane = tid % WAVE;
@@ -556,18 +532,18 @@ __global__ __launch_bounds__(4 * WAVE, 2) void paged_shared_kernel(
   const int per_tile = TILE / a.G;
 
   // ---- the groups' tiles and work, one group a lane
-  if (tid < MAXGROUPS) counts[tid] = 0;
+  if (tid < MAXGROUPS) L.counts[tid] = 0;
   __syncthreads();
   const int len = lane < a.ngroups ? max(a.group_lens[lane], 0) : 0;
   const int first = tid < a.B ? a.group[tid] : -1;
   for (int b = tid; b < a.B; b += 4 * WAVE) {
     const int g = b == tid ? first : a.group[b];
-    if (g >= 0 && g < a.ngroups) atomicAdd(&counts[g], 1);
+    if (g >= 0 && g < a.ngroups) atomicAdd(&L.counts[g], 1);
   }
   __syncthreads();
   if (wid == 0) {
     const int pages = min((len + KVPAGE - 1) / KVPAGE, a.max_pages);
-    const int tiles = (counts[lane] + per_tile - 1) / per_tile;
+    const int tiles = (L.counts[lane] + per_tile - 1) / per_tile;
     int tiles_to = tiles, work = tiles * pages;
     int most = tiles > 0 ? pages : 0;
 #pragma unroll
@@ -580,42 +556,42 @@ __global__ __launch_bounds__(4 * WAVE, 2) void paged_shared_kernel(
       }
       most = max(most, __shfl_xor(most, off, WAVE));
     }
-    g_len[lane] = len;
-    g_pages[lane] = pages;
-    g_tile0[lane] = tiles_to - tiles;
-    g_work0[lane] = work - tiles * pages;
-    g_work1[lane] = work;
-    if (lane == WAVE - 1) all_work = make_int2(work, most);
+    L.len[lane] = len;
+    L.pages_of[lane] = pages;
+    L.tile0[lane] = tiles_to - tiles;
+    L.work0[lane] = work - tiles * pages;
+    L.work1[lane] = work;
+    if (lane == WAVE - 1) L.all_work = make_int2(work, most);
   }
   __syncthreads();
-  const int work = __builtin_amdgcn_readfirstlane(all_work.x);
+  const int work = __builtin_amdgcn_readfirstlane(L.all_work.x);
   // a tile ends in up to one piece more than its pages fill
   const int each =
       max(max((work + a.npre - 1) / a.npre, LEAST),
-          (__builtin_amdgcn_readfirstlane(all_work.y) + MAXPARTS - 2) /
+          (__builtin_amdgcn_readfirstlane(L.all_work.y) + MAXPARTS - 2) /
               (MAXPARTS - 1));
   const int work_end = min(work, (block + 1) * each);
   int at = block * each;
   while (at < work_end) {
     // ---- this piece's group, tile, pages and rows: each row's group goes to
     // LDS (a byte, in what the pages take later), one wave walks the members
-    const int grp = __ffsll((long long)__ballot(at < g_work1[lane])) - 1;
-    const int pages = __builtin_amdgcn_readfirstlane(g_pages[grp]);
-    const int into = at - __builtin_amdgcn_readfirstlane(g_work0[grp]);
+    const int grp = __ffsll((long long)__ballot(at < L.work1[lane])) - 1;
+    const int pages = __builtin_amdgcn_readfirstlane(L.pages_of[grp]);
+    const int into = at - __builtin_amdgcn_readfirstlane(L.work0[grp]);
     const int tile = into / pages;  // of the group's
     const int pbegin = into % pages;
     const int piece =
-        block + tile + __builtin_amdgcn_readfirstlane(g_tile0[grp]);
+        block + tile + __builtin_amdgcn_readfirstlane(L.tile0[grp]);
     const int taken = min(pages - pbegin, work_end - at);
     const int tile_end = at - pbegin + pages;  // in the head's work
     at += taken;
 
-    unsigned char* groups = reinterpret_cast<unsigned char*>(lds);
-    static_assert(MAXB <= sizeof(lds), "a byte a row");
+    unsigned char* groups = reinterpret_cast<unsigned char*>(L.pages);
+    static_assert(MAXB <= sizeof(L.pages), "a byte a row");
     __syncthreads();  // nothing reads the last piece's pages or rows
     for (int b = tid; b < a.B; b += 4 * WAVE)
       groups[b] = (b == tid ? first : a.group[b]) == grp;
-    if (tid == 0) longest = 0;
+    if (tid == 0) L.longest = 0;
     __syncthreads();
     if (wid == 0) {
       const int skip = tile * per_tile;
@@ -624,21 +600,21 @@ __global__ __launch_bounds__(4 * WAVE, 2) void paged_shared_kernel(
         const bool in = b0 + lane < a.B && groups[b0 + lane];
         const unsigned long long bal = __ballot(in);
         const int rank = seen + __popcll(bal & ((1ull << lane) - 1)) - skip;
-        if (in && rank >= 0 && rank < per_tile) tile_rows[rank] = b0 + lane;
+        if (in && rank >= 0 && rank < per_tile) L.tile_rows[rank] = b0 + lane;
         seen += __popcll(bal);
       }
-      if (lane == 0) tile_count = min(seen - skip, per_tile);
+      if (lane == 0) L.tile_count = min(seen - skip, per_tile);
     }
     __syncthreads();
-    const int nrows = tile_count * a.G;
-    if (pbegin == 0 && kvh == 0 && tid < tile_count)
-      a.pre_at[tile_rows[tid]] =
+    const int nrows = L.tile_count * a.G;
+    if (pbegin == 0 && kvh == 0 && tid < L.tile_count)
+      a.pre_at[L.tile_rows[tid]] =
           make_int4(piece, (tile_end - 1) / each - block + 1, tid, 0);
 
     // ---- this wave's 32 query rows: one a lane, halves h of the MFMA's K
     const int i = wid * 32 + r32;
     const bool live = i < nrows;
-    const int b = tile_rows[live ? i / a.G : 0];
+    const int b = L.tile_rows[live ? i / a.G : 0];
     const int head = kvh * a.G + (live ? i % a.G : 0);
     const bool wave_live = wid * 32 < nrows;
     bf16x8v qf[8];
@@ -647,15 +623,15 @@ __global__ __launch_bounds__(4 * WAVE, 2) void paged_shared_kernel(
       qf[k] = load_q(a, a.q + b * a.q_stride + head * HD + k * 16 + h * 8);
     // (a lane without a row computes row 0 again and writes nothing)
     if (live)
-      atomicMax(&longest,
+      atomicMax(&L.longest,
                 (unsigned long long)row_len(a, b) << 32 | (unsigned)b);
     __syncthreads();
     // the longest row's pages (a shorter one's table may end before), none if
     // it ends inside the prefix
-    const int glen = __builtin_amdgcn_readfirstlane(g_len[grp]);
+    const int glen = __builtin_amdgcn_readfirstlane(L.len[grp]);
     const int32_t* table =
-        a.page_table + (int64_t)(unsigned)longest * a.max_pages;
-    const int pend = glen <= (int)(longest >> 32) ? pbegin + taken : pbegin;
+        a.page_table + (int64_t)(unsigned)L.longest * a.max_pages;
+    const int pend = glen <= (int)(L.longest >> 32) ? pbegin + taken : pbegin;
 
     float m = -INFINITY, l = 0.f;
     f32x16 o[4];
@@ -748,8 +724,8 @@ __global__ __launch_bounds__(4 * WAVE, 2) void paged_shared_kernel(
                               kt + t * 32 * K_PITCH + k * 16),
                           qf[k], s[t]);
         // six fragments ahead of the products (the compiler's own order has
-        // two, each product waits for LDS: 27.4 us against 25.7 at 256 rows of
-        // 2048 shared tokens, bf16)
+        // two, each product waits for LDS: 27.4 us against 25.7 for the
+        // prefixes of 256 rows with 2048 shared tokens, bf16)
         SCHED(DS_READ, 6);
 #pragma unroll
         for (int k = 0; k < 10; ++k) {
@@ -827,6 +803,34 @@ __global__ __launch_bounds__(4 * WAVE, 2) void paged_shared_kernel(
   }
 }
 
+// Both in one launch: a KV head's first npre blocks are the prefixes', bound by
+// products, the others its rows' own tokens, bound by bytes, and each covers
+// the other's waits: 512 rows in 3 groups of 8192 + 300 tokens 134 us where the
+// two one after the other took 142, 256 rows of 2048 + 300 67 / 71, 4 rows of
+// 1024 + 90 13.1 / 18.0.  Two blocks a CU cost the own tokens nothing (256 rows
+// of 700, cold: 125.1 us at four, 126.5 at two).
+template <bool FP8>
+__global__ __launch_bounds__(NW * WAVE, 2) void paged_shared_kernel(
+    const Paged a, __hip_bfloat16* __restrict__ out) {
+  __shared__ __attribute__((aligned(16))) union {
+    PrefixLds prefix;
+    OwnLds own;
+  } L;
+  const int kvh = blockIdx.x % a.hkv, i = blockIdx.x / a.hkv;
+  if (i < a.npre)
+    prefix_pieces<FP8>(a, kvh, i, L.prefix);
+  else
+    own_tokens<FP8>(a, out, kvh, (i - a.npre) / a.nsplit,
+                    (i - a.npre) % a.nsplit, L.own);
+}
+
+template <bool FP8>
+__global__ __launch_bounds__(NW * WAVE, 4) void paged_decode_kernel(
+    const Paged a, __hip_bfloat16* __restrict__ out) {
+  __shared__ __attribute__((aligned(16))) OwnLds L;
+  own_tokens<FP8>(a, out, blockIdx.x, blockIdx.y, blockIdx.z, L);
+}
+
 #include <torch/extension.h>
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
@@ -897,29 +901,37 @@ int splits_for(int64_t blocks, int pages) {
 }
 
 template <bool FP8>
-void launch_decode(const Paged& a, torch::Tensor& out, hipStream_t s) {
-  const dim3 grid(a.hkv, a.B, a.nsplit);
-  hipLaunchKernelGGL((paged_decode_kernel<FP8>), grid, dim3(NW * WAVE), 0, s,
-                     a, (__hip_bfloat16*)out.data_ptr());
-  if (a.nsplit > 1)
+void launch(const Paged& a, torch::Tensor& out, hipStream_t s) {
+  auto* o = (__hip_bfloat16*)out.data_ptr();
+  if (a.npre > 0) {
+    const int64_t blocks = (int64_t)a.hkv * (a.npre + a.B * a.nsplit);
+    TORCH_CHECK(blocks < (1 << 24), "too many rows and heads");
+    hipLaunchKernelGGL((paged_shared_kernel<FP8>), dim3((unsigned)blocks),
+                       dim3(NW * WAVE), 0, s, a, o);
+  } else {
+    hipLaunchKernelGGL((paged_decode_kernel<FP8>), dim3(a.hkv, a.B, a.nsplit),
+                       dim3(NW * WAVE), 0, s, a, o);
+  }
+  if (a.npre > 0 || a.nsplit > 1)
     hipLaunchKernelGGL(paged_join_kernel,
                        dim3((unsigned)(((int64_t)a.B * a.hq + 3) / 4)),
-                       dim3(4 * WAVE), 0, s, a,
-                       (__hip_bfloat16*)out.data_ptr());
+                       dim3(4 * WAVE), 0, s, a, o);
 }
 
 // The partial results, pieces of them the prefixes': of this call alone (the
 // allocator orders its reuse on the stream, and a captured graph keeps its own).
 torch::Tensor partials(Paged& a, const torch::Tensor& q, int64_t pieces) {
-  const int64_t own = a.nsplit > 1 ? (int64_t)a.B * a.hq * a.nsplit : 0;
+  const int64_t own =
+      a.nsplit > 1 || pieces > 0 ? (int64_t)a.B * a.hq * a.nsplit : 0;
   const int64_t pre = pieces * a.hkv * TILE;
   if (own + pre == 0) return torch::Tensor();
-  const int64_t at = pieces > 0 ? (int64_t)a.B * 4 : 0;
+  const int64_t at = pieces > 0 ? (int64_t)a.B * 6 : 0;  // whole 8 B
   auto work = torch::empty({(own + pre) * (HD + 2) + at},
                            q.options().dtype(torch::kFloat32));
   a.part_o = (float*)work.data_ptr();
   a.pre_o = a.part_o + own * HD;
   a.pre_at = (int4*)(a.pre_o + pre * HD);
+  a.pre_has = (int32_t*)(a.pre_at + a.B);
   a.part_ml = (float*)a.pre_at + at;
   a.pre_ml = a.part_ml + own * 2;
   return work;
@@ -940,7 +952,7 @@ void attn_decode_fp8(torch::Tensor out, torch::Tensor q, torch::Tensor kcache,
   c10::DeviceGuard guard(dev);
   a.nsplit = splits_for((int64_t)a.B * a.hkv, a.max_pages);
   const auto work = partials(a, q, 0);
-  launch_decode<true>(a, out, at::hip::getCurrentHIPStream().stream());
+  launch<true>(a, out, at::hip::getCurrentHIPStream().stream());
   HIP_CHECK_LAST();
 }
 
@@ -997,22 +1009,13 @@ void attn_decode_shared(torch::Tensor out, torch::Tensor q,
     a.group = (const int32_t*)group.data_ptr();
     a.group_lens = (const int32_t*)group_lens.data_ptr();
     a.npre = (int)std::max<int64_t>(
-        1, std::min<int64_t>(ROOM / a.hkv,
+        1, std::min<int64_t>(PRE_ROOM / a.hkv,
                              tiles * ((a.max_pages + LEAST - 1) / LEAST)));
   }
   const auto work = partials(a, q, a.npre > 0 ? a.npre + tiles : 0);
-  if (a.npre > 0) {
-    const dim3 grid(a.hkv, a.npre);
-    if (fp8)
-      hipLaunchKernelGGL((paged_shared_kernel<true>), grid, dim3(4 * WAVE), 0,
-                         s, a);
-    else
-      hipLaunchKernelGGL((paged_shared_kernel<false>), grid, dim3(4 * WAVE), 0,
-                         s, a);
-  }
   if (fp8)
-    launch_decode<true>(a, out, s);
+    launch<true>(a, out, s);
   else
-    launch_decode<false>(a, out, s);
+    launch<false>(a, out, s);
   HIP_CHECK_LAST();
 }
