@@ -196,8 +196,8 @@ __device__ __forceinline__ float join_weight(const float m, const float l,
 // a kernel that only loads them, cold, reaches 3.5 to 3.9 TB/s where a plain
 // read of one block of memory reaches 6.1.  Measured, e4m3, 32/8 heads: 256
 // rows of up to 700 tokens 49 us, 4.2 TB/s; 8 rows of up to 32768 tokens (64/8
-// heads) 92 us, 5.0 TB/s; one row of 777 tokens (8/2 heads) 9.6 us, of which the
-// join is 4.  The matrix instructions run mostly empty (G of 16 columns) and
+// heads) 92 us, 5.0 TB/s; one row of 777 tokens (8/2 heads) 9.7 us, of which
+// the join is 3.  The matrix instructions run mostly empty (G of 16 columns) and
 // still take a tenth of the vector instructions that dot products would.
 #define UNIT 32  // tokens of one step
 
@@ -887,7 +887,8 @@ Paged paged_args(const torch::Tensor& out, const torch::Tensor& q,
   a.num_pages = (int)kcache.size(0);
   // above 0, so that a masked score stays -inf: at a scale of 0 every weight
   // comes out as 2^(1e-37 * score) = 1
-  a.scale_log2 = std::max((float)(std::fabs(scale) * 1.4426950408889634), 1e-37f);
+  a.scale_log2 =
+      std::max((float)(std::fabs(scale) * 1.4426950408889634), 1e-37f);
   a.flip = scale < 0 ? 0x80008000u : 0u;
   return a;
 }
@@ -919,7 +920,7 @@ void launch(const Paged& a, torch::Tensor& out, hipStream_t s) {
 }
 
 // The partial results, pieces of them the prefixes': of this call alone (the
-// allocator orders its reuse on the stream, and a captured graph keeps its own).
+// allocator orders their reuse on the stream, and a captured graph keeps its).
 torch::Tensor partials(Paged& a, const torch::Tensor& q, int64_t pieces) {
   const int64_t own =
       a.nsplit > 1 || pieces > 0 ? (int64_t)a.B * a.hq * a.nsplit : 0;
