@@ -498,6 +498,72 @@ def test_attn_decode_shared_most_rows(B):
     _close(_shared(s, "cuda")[:, 0], want, tol)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("fp8", [False, True])
+def test_cache_beyond_32_bit_offsets(fp8):
+    """The last pages of a cache of more than 2^32 bytes (and elements of
+    codes): written, read back, attended alone and with a shared prefix."""
+    hkv = 8
+    s = _shared_batch([0, 0, -1], [128], [30, 70, 100], 16, hkv, fp8=fp8)
+    small = s["k"].shape[0]
+    P = 66000 if fp8 else 33000
+    assert P * hkv * PAGE * HD * s["k"].element_size() > 1 << 32
+    d = _to(s, "cuda")
+    for name in ("k", "v", "ks", "vs"):
+        if d[name] is not None:
+            t = torch.empty((P,) + s[name].shape[1:], dtype=s[name].dtype,
+                            device="cuda")
+            t[P - small:] = d[name]
+            d[name] = t
+    d["table"] += P - small
+    want = _expect(s, HD ** -0.5)
+    out = torch.full(s["q"].shape, 5.0, dtype=torch.bfloat16, device="cuda")
+    ops.attn_decode_shared(out, d["q"], d["k"], d["v"], d["table"], d["lens"],
+                           d["group"], d["glens"], HD ** -0.5, kscale=d["ks"],
+                           vscale=d["vs"])
+    _close(out, *want)
+    if not fp8:
+        return
+    out.fill_(5.0)
+    cache = (d["k"], d["v"], d["ks"], d["vs"])
+    ops.attn_decode_fp8(out, d["q"], *cache, d["table"], d["lens"],
+                        HD ** -0.5)
+    _close(out, *want)
+    g = torch.Generator().manual_seed(0)
+    x = [torch.randn(5, hkv, HD, generator=g).to(torch.bfloat16)
+         for _ in range(2)]
+    slots = (P * PAGE - 1 - torch.arange(5)).to(torch.int32).cuda()
+    ops.kv_write_fp8(*cache, x[0].cuda(), x[1].cuda(), slots)
+    back = [torch.zeros_like(t, device="cuda") for t in x]
+    ops.kv_read_fp8(*back, *cache, slots)
+    for t, b in zip(x, back):
+        assert torch.equal(b.cpu().double(), _quantised64(t)[0])
+
+
+@pytest.mark.gpu
+def test_attention_on_two_streams_at_once():
+    """Calls in flight together have workspaces of their own."""
+    batches = [_shared_batch([0, 0, 0, -1] * 4, [640], list(range(60, 76)), 32,
+                             8, seed=i) for i in range(2)]
+    moved = [_to(s, "cuda") for s in batches]
+    streams = [torch.cuda.Stream() for _ in batches]
+    outs = [[torch.empty(s["q"].shape, dtype=torch.bfloat16, device="cuda")
+             for _ in range(8)] for s in batches]
+    torch.cuda.synchronize()
+    for i in range(8):
+        for d, stream, out in zip(moved, streams, outs):
+            with torch.cuda.stream(stream):
+                ops.attn_decode_shared(out[i], d["q"], d["k"], d["v"],
+                                       d["table"], d["lens"], d["group"],
+                                       d["glens"], HD ** -0.5,
+                                       kscale=d["ks"], vscale=d["vs"])
+    torch.cuda.synchronize()
+    for s, out in zip(batches, outs):
+        _close(out[0], *_expect(s, HD ** -0.5))
+        for o in out[1:]:
+            assert torch.equal(o, out[0])
+
+
 def test_build_prefix_groups():
     table = np.array([[3, 4, 5, 6], [3, 4, 9, 0], [8, 1, 2, 0], [3, 4, 5, 7],
                       [8, 1, 2, 0], [11, 0, 0, 0], [3, 0, 0, 0]], np.int32)

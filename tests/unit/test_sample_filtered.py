@@ -196,6 +196,31 @@ def test_general_search_rows():
 
 
 @pytest.mark.gpu
+def test_rows_beyond_32_bit_offsets():
+    """The last rows of logits of more than 2^32 bytes; the others, not drawn,
+    keep their outputs."""
+    B, V = 17000, 128256
+    assert B * V * 2 > 1 << 32
+    g = torch.Generator().manual_seed(1)
+    last = (torch.randn(2, V, generator=g) * 3).to(torch.bfloat16)
+    logits = torch.empty(B, V, dtype=torch.bfloat16, device="cuda")
+    logits[-2:] = last.cuda()
+    f = [torch.full((B,), v, dtype=d, device="cuda")
+         for v, d in ((0.8, torch.float32), (500, torch.int32),
+                      (0.9, torch.float32), (0.001, torch.float32),
+                      (-1.0, torch.float32))]
+    f[4][-2:] = torch.tensor([0.3, 0.8])
+    out, kept = (torch.full((B,), -7, dtype=torch.int32, device="cuda")
+                 for _ in range(2))
+    ops.sample_filtered(out, logits, *f, kept=kept)
+    want, n = (torch.zeros(2, dtype=torch.int32) for _ in range(2))
+    ops.sample_filtered(want, last, *[t[-2:].cpu() for t in f], kept=n)
+    assert torch.equal(out[-2:].cpu(), want)
+    assert torch.equal(kept[-2:].cpu(), n)
+    assert (out[:-2] == -7).all() and (kept[:-2] == -7).all()
+
+
+@pytest.mark.gpu
 def test_view_off_alignment():
     """Logits that start off 16 bytes."""
     for dtype in (torch.bfloat16, torch.float32):
