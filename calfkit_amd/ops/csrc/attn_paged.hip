@@ -44,12 +44,11 @@
 // 66.8, 72.6, 77.3.
 #define PRE_ROOM 256
 // Pages of a split or of a prefix's piece, at least.  One row of 777 tokens:
-// 12.1 us at 1, 10.1 at 2, 11.9 at 4; 4 rows of 1024 shared tokens 22.4, 21.0,
-// 23.9.
+// 12.1 us at 1, 10.2 at 2, 11.8 at 4; 4 rows of 1024 shared tokens 22.4, 21.0,
+// 23.9 (cold).
 #define LEAST 2
-// Splits of a row and pieces of a tile's prefix, at most: each one's o is read
-// again.  One row of 8192 tokens: 20.5 us at 32, 28.0 at 64.  Both together are
-// joined by one wave.
+// Splits of a row and pieces of a tile's prefix, at most: both together are
+// joined by one wave.  One row of 32768 tokens 57 us at 8, 35 at 16, 33 at 32.
 #define MAXPARTS 32
 #define SLACK 8.f      // log2 by which a weight may pass 1
 
@@ -426,7 +425,11 @@ __device__ __forceinline__ void own_tokens(const Paged& a,
   }
 }
 
-// Joins the partial slots of one (row, head): a wave each, 2 dims a lane.
+// Joins the partial slots of one (row, head): a wave each, 2 dims a lane.  The
+// first AHEAD o's of the row's own splits are read before their weights are
+// known: room for 32 where there are many (one row of 4096 tokens 12.2 us, with
+// room for 8 17.7), for 8 where there are not, and many rows take the registers.
+template <int AHEAD>
 __global__ __launch_bounds__(4 * WAVE) void paged_join_kernel(
     const Paged a, __hip_bfloat16* __restrict__ out) {
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
@@ -442,12 +445,11 @@ __global__ __launch_bounds__(4 * WAVE) void paged_join_kernel(
   const int joined = at.y;
   if (a.nsplit == 1 && joined == 0) return;  // written whole
   const int own = a.nsplit;  // up to 32, as of prefixes
-  // The first o's are on their way before their weights are known: what is
-  // not written (an empty range) weighs nothing.
-  constexpr int AHEAD = 8;
+  // what is not written (an empty range) weighs nothing
+  constexpr int PRE_AHEAD = 8;
   const float2* part =
       reinterpret_cast<const float2*>(a.part_o + row * own * HD) + lane;
-  float2 x[AHEAD], y[AHEAD];
+  float2 x[AHEAD], y[PRE_AHEAD];
 #pragma unroll
   for (int k = 0; k < AHEAD; ++k)
     if (k < own) x[k] = part[k * (HD / 2)];
@@ -460,7 +462,7 @@ __global__ __launch_bounds__(4 * WAVE) void paged_join_kernel(
   const float2* pre =
       reinterpret_cast<const float2*>(a.pre_o + first * HD) + lane;
 #pragma unroll
-  for (int k = 0; k < AHEAD; ++k)
+  for (int k = 0; k < PRE_AHEAD; ++k)
     if (k < joined) y[k] = pre[k * step];
   if (lane >= own && lane - own < joined)
     ml = reinterpret_cast<const float2*>(
@@ -478,13 +480,11 @@ __global__ __launch_bounds__(4 * WAVE) void paged_join_kernel(
 #pragma unroll
   for (int k = 0; k < AHEAD; ++k)
     if (k < own) add(k, x[k]);
-#pragma unroll 8
-  for (int k = AHEAD; k < own; ++k) add(k, part[k * (HD / 2)]);
 #pragma unroll
-  for (int k = 0; k < AHEAD; ++k)
+  for (int k = 0; k < PRE_AHEAD; ++k)
     if (k < joined) add(own + k, y[k]);
 #pragma unroll 8
-  for (int k = AHEAD; k < joined; ++k) add(own + k, pre[k * step]);
+  for (int k = PRE_AHEAD; k < joined; ++k) add(own + k, pre[k * step]);
   const float inv = (L == 0.f) ? 0.f : 1.f / L;
   __hip_bfloat16* dst = out + row * HD + lane * 2;
   dst[0] = f2bf(L == 0.f ? 0.f : acc.x * inv);
@@ -913,10 +913,13 @@ void launch(const Paged& a, torch::Tensor& out, hipStream_t s) {
     hipLaunchKernelGGL((paged_decode_kernel<FP8>), dim3(a.hkv, a.B, a.nsplit),
                        dim3(NW * WAVE), 0, s, a, o);
   }
-  if (a.npre > 0 || a.nsplit > 1)
-    hipLaunchKernelGGL(paged_join_kernel,
-                       dim3((unsigned)(((int64_t)a.B * a.hq + 3) / 4)),
-                       dim3(4 * WAVE), 0, s, a, o);
+  const dim3 joins((unsigned)(((int64_t)a.B * a.hq + 3) / 4));
+  if (a.nsplit > 8)
+    hipLaunchKernelGGL((paged_join_kernel<MAXPARTS>), joins, dim3(4 * WAVE), 0,
+                       s, a, o);
+  else if (a.npre > 0 || a.nsplit > 1)
+    hipLaunchKernelGGL((paged_join_kernel<8>), joins, dim3(4 * WAVE), 0, s, a,
+                       o);
 }
 
 // The partial results, pieces of them the prefixes': of this call alone (the
