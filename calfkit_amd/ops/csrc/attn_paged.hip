@@ -215,6 +215,13 @@ __device__ __forceinline__ void own_tokens(const Paged& a,
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
   const int lane = threadIdx.x % WAVE;
   const int l16 = lane & 15, g4 = lane >> 4;
+  const int32_t* table = a.page_table + (int64_t)b * a.max_pages;
+  // the first page ids of a row's start, before its length is known (256 rows
+  // of 2048 + 300 tokens 66.8 -> 64.4 us)
+  int ids = a.max_pages > 0
+                ? table[min((wid + lane * NW) / (KVPAGE / UNIT),
+                            a.max_pages - 1)]
+                : -1;
   const int n = row_len(a, b);
   const int first = prefix_len(a, b, n);
   const int unit0 = first / UNIT;
@@ -244,7 +251,6 @@ __device__ __forceinline__ void own_tokens(const Paged& a,
   __hip_bfloat16* vt = L.v[wid];
   const __hip_bfloat16* vt_read =
       vt + (g4 * 4 + (l16 >> 2)) * V_PITCH + (l16 & 3) * 4;
-  const int32_t* table = a.page_table + (int64_t)b * a.max_pages;
 
   constexpr int ROWB = FP8 ? HD : 2 * HD;  // bytes of a cache row
   constexpr int KLD = FP8 ? 2 : 4;    // 16 B loads of a lane, a 16-token tile
@@ -252,10 +258,9 @@ __device__ __forceinline__ void own_tokens(const Paged& a,
   constexpr int VLD = UNIT * VROW / WAVE;
   const int koff = l16 * ROWB + g4 * 16, voff = lane * 16;
 
-  int ids = 0;
   for (int i = 0; i < steps; ++i) {
     const int u = ubegin + i * NW;
-    if (i % WAVE == 0) {
+    if (i % WAVE == 0 && (i > 0 || ubegin != wid)) {
       const int mine = u + lane * NW;
       ids = mine < uend ? table[mine / (KVPAGE / UNIT)] : -1;
     }
