@@ -29,7 +29,7 @@
 // registers (128256 bf16 are 64 registers a thread).  Bound: the histogram, one LDS
 // add an entry: 13 to 18 cycles an instruction of 64 lanes (LDS itself is busy
 // for 8, half of them bank conflicts), up to 37000 of the 62000 cycles of a bf16
-// row of 128256; then the row's bytes.  Measured: one bf16 row of 128256 16 to 20 us, 512 of them 67.5 us (1.9 TB/s;
+// row of 128256; then the row's bytes.  Measured: one bf16 row of 128256 15 to 24 us, 512 of them 67.5 us (1.9 TB/s;
 // a CU takes two, the histograms 31 us of it), 64 fp32 rows of 32000 45 us
 // (64-bit exponentials and two histograms).  Sorting the 512 rows with library
 // calls takes 11.7 ms.
