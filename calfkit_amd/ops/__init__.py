@@ -499,9 +499,10 @@ def attn_decode_shared(out: torch.Tensor, q: torch.Tensor,
     the same pages: each prefix is attended once for all its rows, the rest
     row by row, and the two are joined.  ``build_prefix_groups`` finds the
     groups.  The result is that of ``attn_decode`` (or, with the scales of
-    an e4m3 cache, ``attn_decode_fp8``) up to the order of its sums, whatever
-    the grouping; a row that ends inside its group's prefix is attended by
-    itself.
+    an e4m3 cache, ``attn_decode_fp8``) whatever the grouping, up to the order
+    of its sums and 2^-15 of each weight, which pass through the products as
+    two bf16 terms (in ``attn_decode_fp8`` too); a row that ends inside its
+    group's prefix is attended by itself.
     """
     if _native(q):
         _K.attn_decode_shared(out, q, kcache, vcache, page_table, seq_lens,

@@ -18,9 +18,13 @@
 // so B's slots m = 0..7 are read as {4 tokens of one half, 4 of the other}
 // and V^T is read in the same order: P never leaves its registers.
 //
-// P is rounded to bf16 for the matrix instruction (at most 2^-8 of each weight,
-// with independent signs: the size of the output's own rounding); its sum l is
-// the rounded weights', so that they sum to 1.
+// The matrix instruction takes bf16, so each weight of P goes through it as two
+// terms: its upper bits, and what they leave out, rounded, which loses at most
+// 2^-15 of it (one term alone would lose 2^-8, as much as the output's own
+// rounding).  The sum l is the terms', so that the weights sum to 1.  Beside
+// own tokens the second term costs nothing (256 rows of 700 tokens 49 us either
+// way), in the shared pass its products and splits take 512 rows with 3 prefixes
+// of 8192 tokens from 134 to 157 us, 256 rows of 2048 from 64 to 67.
 //
 // e4m3 rows become bf16 on the way in (scale times code is exact in bf16), so
 // both caches share one arithmetic.
@@ -111,6 +115,26 @@ __device__ __forceinline__ float add8(const bf16x8v p, float l) {
     l = __builtin_amdgcn_fdot2_f32_bf16((bf16x2){p[2 * j], p[2 * j + 1]}, ones,
                                         l, false);
   return l;
+}
+
+// Weights (0 and up) as two bf16 terms each: the first is the number next below
+// cut to bf16, so that both are above 0 where the weight is, and an infinite
+// value of V stays one (0 times it would be NaN).
+struct Terms {
+  u32x4 hi, lo;
+};
+__device__ __forceinline__ void split2(const float p, const float q, Terms& t,
+                                       const int at) {
+  using bf16x2 = __attribute__((ext_vector_type(2))) __bf16;
+  const unsigned u =
+      __builtin_elementwise_sub_sat(__float_as_uint(p), 1u) & 0xffff0000u;
+  const unsigned v =
+      __builtin_elementwise_sub_sat(__float_as_uint(q), 1u) & 0xffff0000u;
+  t.hi[at] = __builtin_amdgcn_perm(v, u, 0x07060302);
+  t.lo[at] = __builtin_bit_cast(
+      unsigned,
+      (bf16x2){(__bf16)(p - __uint_as_float(u)),
+               (__bf16)(q - __uint_as_float(v))});
 }
 
 struct Paged {
@@ -207,7 +231,7 @@ struct OwnLds {
   float ml[NW][MAXG][2];
 };
 
-template <bool FP8>
+template <bool FP8, bool WIDE>
 __device__ __forceinline__ void own_tokens(const Paged& a,
                                            __hip_bfloat16* __restrict__ out,
                                            const int kvh, const int b,
@@ -231,6 +255,11 @@ __device__ __forceinline__ void own_tokens(const Paged& a,
   const int uend = unit0 + min(nunits, (split + 1) * each);
   const int steps = uend > ubegin ? (uend - ubegin + NW - 1) / NW : 0;
 
+  // Columns: G query heads, and where 2G fit into 16, the same heads again,
+  // for their weights' second terms: the instructions are the same.
+  const int cols = WIDE ? a.G : 2 * a.G;
+  const bool second = !WIDE && l16 >= a.G;
+
   // fragment c of lane group g4 holds dims 32c + 8*g4 .. of a bf16 row, or of
   // an e4m3 row (whose 16 B are 16 dims) 64*(c/2) + 16*g4 + 8*(c%2) ..
   bf16x8v qf[4];
@@ -239,8 +268,9 @@ __device__ __forceinline__ void own_tokens(const Paged& a,
     const int d = FP8 ? (c / 2) * 64 + g4 * 16 + (c % 2) * 8 : c * 32 + g4 * 8;
     const u32x4 none = {0, 0, 0, 0};
     qf[c] = __builtin_bit_cast(bf16x8v, none);
-    if (l16 < a.G)
-      qf[c] = load_q(a, a.q + b * a.q_stride + (kvh * a.G + l16) * HD + d);
+    if (l16 < cols)
+      qf[c] = load_q(a, a.q + b * a.q_stride +
+                            (kvh * a.G + l16 - (second ? a.G : 0)) * HD + d);
   }
 
   float m = -INFINITY, l = 0.f;
@@ -329,11 +359,17 @@ __device__ __forceinline__ void own_tokens(const Paged& a,
       for (int d = 0; d < 8; ++d) o[d] *= keep;
     }
     m = mn;
-    bf16x8v pf;
+    Terms p2;
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      pf[j] = (__bf16)exp2_fast(fmaf(s[j / 4][j % 4], a.scale_log2, -mu));
+    for (int j = 0; j < 8; j += 2)
+      split2(exp2_fast(fmaf(s[j / 4][j % 4], a.scale_log2, -mu)),
+             exp2_fast(fmaf(s[j / 4][j % 4 + 1], a.scale_log2, -mu)), p2,
+             j / 2);
+    if constexpr (!WIDE) p2.hi = second ? p2.lo : p2.hi;
+    const bf16x8v pf = __builtin_bit_cast(bf16x8v, p2.hi);
+    const bf16x8v pl = __builtin_bit_cast(bf16x8v, p2.lo);
     l = add8(pf, l);
+    if constexpr (WIDE) l = add8(pl, l);
 
     // V to LDS as bf16; rows outside the sequence as zeros (weight 0 times
     // whatever a recycled page holds may be NaN)
@@ -359,10 +395,12 @@ __device__ __forceinline__ void own_tokens(const Paged& a,
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int d = 0; d < 8; ++d)
-      o[d] = MFMA16(join(read_tr(vt_read + d * 16),
-                         read_tr(vt_read + d * 16 + 16 * V_PITCH)),
-                    pf, o[d]);
+    for (int d = 0; d < 8; ++d) {
+      const bf16x8v v = join(read_tr(vt_read + d * 16),
+                             read_tr(vt_read + d * 16 + 16 * V_PITCH));
+      o[d] = MFMA16(v, pf, o[d]);
+      if constexpr (WIDE) o[d] = MFMA16(v, pl, o[d]);
+    }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
   }
@@ -380,7 +418,7 @@ __device__ __forceinline__ void own_tokens(const Paged& a,
   float* w_lds = o_lds + NW * MAXG * HD;                 // [16][NW]
   static_assert((NW * MAXG * HD + MAXG * NW) * 4 <= sizeof(L.v),
                 "O and the weights fit V's rows");
-  if (l16 < a.G) {
+  if (l16 < cols) {
 #pragma unroll
     for (int d = 0; d < 8; ++d)
       *reinterpret_cast<f32x4*>(
@@ -397,6 +435,7 @@ __device__ __forceinline__ void own_tokens(const Paged& a,
     if (lane < NW) {
       mk = L.ml[lane][g][0];
       lk = L.ml[lane][g][1];
+      if constexpr (!WIDE) lk += L.ml[lane][a.G + g][1];
     }
     const float w = join_weight(mk, lk, M, S);
     // no weight at all (an empty row): zeros
@@ -414,8 +453,14 @@ __device__ __forceinline__ void own_tokens(const Paged& a,
 #pragma unroll
     for (int k = 0; k < NW; ++k) {
       const float w = w_lds[g * NW + k];
-      const float2 x =
+      float2 x =
           *reinterpret_cast<const float2*>(&o_lds[(k * MAXG + g) * HD + d]);
+      if constexpr (!WIDE) {
+        const float2 y = *reinterpret_cast<const float2*>(
+            &o_lds[(k * MAXG + a.G + g) * HD + d]);
+        x.x += y.x;
+        x.y += y.y;
+      }
       acc.x = fmaf(w, x.x, acc.x);
       acc.y = fmaf(w, x.y, acc.y);
     }
@@ -762,31 +807,38 @@ __device__ __forceinline__ void prefix_pieces(const Paged& a, const int kvh,
           for (int d = 0; d < 4; ++d) o[d] *= keep;
         }
         const float mu = (m == -INFINITY) ? 0.f : m;
-        bf16x8v pf[4];
+        bf16x8v pf[4], pl[4];
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int u = 0; u < 4; ++u) {
+          Terms p2;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            pf[t * 2 + r / 8][r % 8] =
-                (__bf16)exp2_fast(fmaf(s[t][r], a.scale_log2, -mu));
+          for (int j = 0; j < 8; j += 2) {
+            const f32x16& x = s[u / 2];
+            const int r = u % 2 * 8 + j;
+            split2(exp2_fast(fmaf(x[r], a.scale_log2, -mu)),
+                   exp2_fast(fmaf(x[r + 1], a.scale_log2, -mu)), p2, j / 2);
           }
+          pf[u] = __builtin_bit_cast(bf16x8v, p2.hi);
+          pl[u] = __builtin_bit_cast(bf16x8v, p2.lo);
+        }
 #pragma unroll
-        for (int u = 0; u < 4; ++u) l = add8(pf[u], l);
+        for (int u = 0; u < 4; ++u) l = add8(pl[u], add8(pf[u], l));
 #pragma unroll
         for (int u = 0; u < 4; ++u)
 #pragma unroll
           for (int d = 0; d < 4; ++d) {
             const __hip_bfloat16* p = vt + u * 16 * V_PITCH32 + d * 32;
-            o[d] = MFMA32(join(read_tr(p), read_tr(p + 8 * V_PITCH32)), pf[u],
-                          o[d]);
+            const bf16x8v v = join(read_tr(p), read_tr(p + 8 * V_PITCH32));
+            o[d] = MFMA32(v, pf[u], o[d]);
+            o[d] = MFMA32(v, pl[u], o[d]);
           }
         SCHED(DS_READ, 8);
 #pragma unroll
         for (int k = 0; k < 12; ++k) {
-          SCHED(MFMA, 1);
+          SCHED(MFMA, 2);
           SCHED(DS_READ, 2);
         }
-        SCHED(MFMA, 4);
+        SCHED(MFMA, 8);
       }
       if (pi + 1 < pend) stage(buf ^ 1, pi + 1);
     }
@@ -814,7 +866,7 @@ __device__ __forceinline__ void prefix_pieces(const Paged& a, const int kvh,
 // two one after the other took 142, 256 rows of 2048 + 300 67 / 71, 4 rows of
 // 1024 + 90 13.1 / 18.0.  Two blocks a CU cost the own tokens nothing (256 rows
 // of 700, cold: 125.1 us at four, 126.5 at two).
-template <bool FP8>
+template <bool FP8, bool WIDE>
 __global__ __launch_bounds__(NW * WAVE, 2) void paged_shared_kernel(
     const Paged a, __hip_bfloat16* __restrict__ out) {
   __shared__ __attribute__((aligned(16))) union {
@@ -825,15 +877,15 @@ __global__ __launch_bounds__(NW * WAVE, 2) void paged_shared_kernel(
   if (i < a.npre)
     prefix_pieces<FP8>(a, kvh, i, L.prefix);
   else
-    own_tokens<FP8>(a, out, kvh, (i - a.npre) / a.nsplit,
+    own_tokens<FP8, WIDE>(a, out, kvh, (i - a.npre) / a.nsplit,
                     (i - a.npre) % a.nsplit, L.own);
 }
 
-template <bool FP8>
+template <bool FP8, bool WIDE>
 __global__ __launch_bounds__(NW * WAVE, 4) void paged_decode_kernel(
     const Paged a, __hip_bfloat16* __restrict__ out) {
   __shared__ __attribute__((aligned(16))) OwnLds L;
-  own_tokens<FP8>(a, out, blockIdx.x, blockIdx.y, blockIdx.z, L);
+  own_tokens<FP8, WIDE>(a, out, blockIdx.x, blockIdx.y, blockIdx.z, L);
 }
 
 #include <torch/extension.h>
@@ -906,16 +958,16 @@ int splits_for(int64_t blocks, int pages) {
       1, std::min<int64_t>({want, (pages + LEAST - 1) / LEAST, MAXPARTS}));
 }
 
-template <bool FP8>
+template <bool FP8, bool WIDE>
 void launch(const Paged& a, torch::Tensor& out, hipStream_t s) {
   auto* o = (__hip_bfloat16*)out.data_ptr();
   if (a.npre > 0) {
     const int64_t blocks = (int64_t)a.hkv * (a.npre + a.B * a.nsplit);
     TORCH_CHECK(blocks < (1 << 24), "too many rows and heads");
-    hipLaunchKernelGGL((paged_shared_kernel<FP8>), dim3((unsigned)blocks),
+    hipLaunchKernelGGL((paged_shared_kernel<FP8, WIDE>), dim3((unsigned)blocks),
                        dim3(NW * WAVE), 0, s, a, o);
   } else {
-    hipLaunchKernelGGL((paged_decode_kernel<FP8>), dim3(a.hkv, a.B, a.nsplit),
+    hipLaunchKernelGGL((paged_decode_kernel<FP8, WIDE>), dim3(a.hkv, a.B, a.nsplit),
                        dim3(NW * WAVE), 0, s, a, o);
   }
   const dim3 joins((unsigned)(((int64_t)a.B * a.hq + 3) / 4));
@@ -925,6 +977,15 @@ void launch(const Paged& a, torch::Tensor& out, hipStream_t s) {
   else if (a.npre > 0 || a.nsplit > 1)
     hipLaunchKernelGGL((paged_join_kernel<8>), joins, dim3(4 * WAVE), 0, s, a,
                        o);
+}
+
+template <bool FP8>
+void launch(const Paged& a, torch::Tensor& out) {
+  hipStream_t s = at::hip::getCurrentHIPStream().stream();
+  if (2 * a.G > MAXG)
+    launch<FP8, true>(a, out, s);
+  else
+    launch<FP8, false>(a, out, s);
 }
 
 // The partial results, pieces of them the prefixes': of this call alone (the
@@ -961,7 +1022,7 @@ void attn_decode_fp8(torch::Tensor out, torch::Tensor q, torch::Tensor kcache,
   c10::DeviceGuard guard(dev);
   a.nsplit = splits_for((int64_t)a.B * a.hkv, a.max_pages);
   const auto work = partials(a, q, 0);
-  launch<true>(a, out, at::hip::getCurrentHIPStream().stream());
+  launch<true>(a, out);
   HIP_CHECK_LAST();
 }
 
@@ -1007,7 +1068,6 @@ void attn_decode_shared(torch::Tensor out, torch::Tensor q,
   }
   a.ngroups = (int)group_lens.size(0);
   c10::DeviceGuard guard(dev);
-  hipStream_t s = at::hip::getCurrentHIPStream().stream();
   a.nsplit = splits_for((int64_t)a.B * a.hkv, a.max_pages);
   // each group may leave one tile part full; no more tiles than rows
   const int per_tile = TILE / a.G;
@@ -1023,8 +1083,8 @@ void attn_decode_shared(torch::Tensor out, torch::Tensor q,
   }
   const auto work = partials(a, q, a.npre > 0 ? a.npre + tiles : 0);
   if (fp8)
-    launch<true>(a, out, s);
+    launch<true>(a, out);
   else
-    launch<false>(a, out, s);
+    launch<false>(a, out);
   HIP_CHECK_LAST();
 }

@@ -564,6 +564,65 @@ def test_attention_on_two_streams_at_once():
             assert torch.equal(o, out[0])
 
 
+def _integers(s, scale):
+    """Small whole numbers for q and K, signs for V: scores are exact, so that
+    what is left of _expect's bound is the weights'."""
+    g = torch.Generator().manual_seed(7)
+    q = s["q"]
+    q.copy_(torch.randint(-1, 2, q.shape, generator=g).to(q.dtype))
+    q[..., 40:] = 0
+    for name, sc in (("k", "ks"), ("v", "vs")):
+        x = torch.randint(0, 2, s[name].shape, generator=g) * 2 - 1
+        if s[sc] is None:
+            s[name].copy_(x.to(torch.bfloat16))
+        else:
+            s[name] = x.float().to(torch.float8_e4m3fn)
+            s[sc].fill_(127)
+    out, _ = _expect(s, scale)
+    n = int(s["lens"].max())
+    # a weight as two bf16 terms: 2^-7 of it is left to the second, whose own
+    # rounding is 2^-8 of that.  Its exponent (up to 40 * scale * log2 e, below
+    # 2^5) has two roundings of 2^-24, the exponential and a join's factor one
+    # of 2^-23 each.  Twice, as the sum of weights is off by as much; sums of n
+    # in fp32.  (sum of p |v| is 1)
+    weight = 2 ** -15 + 2 ** -18 + 2 ** -22
+    return out, 2 ** -8 * out.abs() + 2 * (weight + n * 2 ** -24)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("hq,hkv", [(2, 1), (32, 8), (24, 3), (9, 1), (16, 1)])
+def test_attention_weights_are_not_cut_to_bf16(device, hq, hkv):
+    """Values of both signs that nearly cancel: a weight's error shows."""
+    scale = 0.37
+    s = _batch([260, 64, 1, 333], hq, hkv, seed=hq)
+    want = _integers(s, scale)
+    _close(_decode(s, scale, device=device), *want)
+    for fp8 in (False, True):
+        s = _shared_batch([0, 0, 1, -1, 0], [192, 320], [70, 1, 64, 300, 0],
+                          hq, hkv, seed=hq, fp8=fp8)
+        want = _integers(s, scale)
+        _close(_shared(s, device, scale), *want)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("hq,hkv", [(8, 2), (16, 1)])
+def test_attn_decode_shared_infinite_values_stay_infinite(device, hq, hkv):
+    """An infinity in V is its row's output in that place, as the formula has
+    it, in a prefix and among a row's own tokens."""
+    s = _shared_batch([0, 0, -1], [128], [30, 70, 100], hq, hkv)
+    want, tol = _expect(s, HD ** -0.5)
+    first, own = int(s["table"][0, 1]), int(s["table"][2, 1])
+    s["v"][first, 0, 5, 9] = math.inf
+    s["v"][own, 0, 5, 77] = -math.inf
+    got = _shared(s, device).cpu()
+    heads = slice(0, hq // hkv)
+    assert (got[:2, heads, 9] == math.inf).all()
+    assert (got[2, heads, 77] == -math.inf).all()
+    got[:2, heads, 9] = want[:2, heads, 9].to(got.dtype)
+    got[2, heads, 77] = want[2, heads, 77].to(got.dtype)
+    _close(got, want, tol)
+
+
 def test_build_prefix_groups():
     table = np.array([[3, 4, 5, 6], [3, 4, 9, 0], [8, 1, 2, 0], [3, 4, 5, 7],
                       [8, 1, 2, 0], [11, 0, 0, 0], [3, 0, 0, 0]], np.int32)
