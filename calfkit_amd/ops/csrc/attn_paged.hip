@@ -592,7 +592,8 @@ __device__ __forceinline__ void prefix_pieces(const Paged& a, const int kvh,
   }
   __syncthreads();
   if (wid == 0) {
-    const int pages = min((len + KVPAGE - 1) / KVPAGE, a.max_pages);
+    // (any int32 may be a length: no sum that passes 2^31)
+    const int pages = min(len / KVPAGE + (len % KVPAGE != 0), a.max_pages);
     const int tiles = (L.counts[lane] + per_tile - 1) / per_tile;
     int tiles_to = tiles, work = tiles * pages;
     int most = tiles > 0 ? pages : 0;

@@ -445,6 +445,18 @@ def test_attn_decode_shared_any_prefix_length(device, fp8):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("most", [2 ** 31 - 1, 2 ** 31 - 63, 2 ** 31 - 64])
+def test_attn_decode_shared_longest_prefix_lengths(device, most):
+    """The largest lengths an int32 holds: rows that end inside such a prefix
+    are attended by themselves, the other groups as ever."""
+    s = _shared_batch([0, 1, 0, 1, 1], [192, 128], [9, 40, 77, 3, 60], 8, 2)
+    want = _expect(s, HD ** -0.5)
+    for glens in ([most, 128], [192, most], [most, most]):
+        s["glens"] = torch.tensor(glens, dtype=torch.int32)
+        _close(_shared(s, device), *want)
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_attn_decode_shared_short_rows_first(device):
     """A group's first rows may have ended: the entries past a row's length
     name other pages, and none of them is read."""
