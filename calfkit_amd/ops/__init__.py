@@ -559,40 +559,100 @@ def build_prefix_groups(page_table: "np.ndarray", lengths: "np.ndarray",
                             "np.ndarray", "np.ndarray"]:
     """Host-side prefix groups of a batch for ``attn_decode_shared``.
 
-    page_table [B, max_pages] and lengths [B] as numpy arrays.  Rows with the
-    same first page form a group; its prefix is the run of whole pages that
-    all of them have in common.  Groups of fewer rows or pages than the
-    minimum are left out, and of more than ``max_groups`` those that save the
-    least reading; where all of them together save fewer than ``min_saved``
-    page reads, there are none.  Returns (group [B] i32, group_lens [max_groups] i32).
+    page_table [B, max_pages] and lengths [B] as numpy arrays.  Rows whose
+    first whole pages are the same can form a group, with those pages for its
+    prefix; where the runs that rows share branch (one system prompt, then
+    each kind's own), the groups are those that together save the most page
+    reads, taken one after the other: a row is in the longest of the runs
+    taken, a row too short for it in a shorter one or in none.  Groups of
+    fewer rows or pages than the minimum are left out, and there are at most
+    ``max_groups``; where all of them together save fewer than ``min_saved``
+    page reads, there are none.  Returns (group [B] i32,
+    group_lens [max_groups] i32).
     """
     import numpy as np
 
-    B = page_table.shape[0]
+    B, width = page_table.shape
     group = np.full(B, -1, dtype=np.int32)
     lens = np.zeros(max_groups, dtype=np.int32)
-    whole = np.minimum(np.asarray(lengths) // 64, page_table.shape[1])
+    least = max(2, min_rows)
+    whole = np.minimum(np.asarray(lengths) // 64, width)
     rows = np.flatnonzero(whole >= max(1, min_pages))
-    if rows.size == 0:
+    if rows.size:
+        # rows alone with their first page share nothing
+        _, where, count = np.unique(page_table[rows, 0], return_inverse=True,
+                                    return_counts=True)
+        rows = rows[count[where] >= least]
+    if rows.size == 0 or max_groups < 1:
         return group, lens
-    found = []
-    heads, where = np.unique(page_table[rows, 0], return_inverse=True)
-    for h in range(heads.size):
-        members = rows[where == h]
-        if members.size < max(2, min_rows):
-            continue
-        most = int(whole[members].min())
-        same = (page_table[members, :most]
-                == page_table[members[0], :most]).all(0)
-        pages = most if same.all() else int(np.argmin(same))
-        if pages >= max(1, min_pages):
-            found.append(((members.size - 1) * pages, pages, members))
-    found.sort(key=lambda f: -f[0])
-    if sum(f[0] for f in found[:max_groups]) < min_saved:
+
+    # rows in order of their page runs (an ended run is the largest of those
+    # that go on), and the pages each has in common with the next
+    n = whole[rows]
+    deep = int(n.max())
+    runs = np.where(np.arange(deep) < n[:, None], page_table[rows, :deep],
+                    np.int32(-1)).astype(np.int32, copy=False)
+    order = np.argsort(runs.view(f"V{4 * deep}").ravel(), kind="stable")
+    rows, n, runs = rows[order], n[order], runs[order]
+    same = runs[1:] == runs[:-1]
+    common = np.where(same.all(1), deep, same.argmin(1))
+    common = np.minimum(common, np.minimum(n[1:], n[:-1]))
+
+    # the tree of equal runs: rows lo..hi - 1 have d pages in common
+    found, open_ = [], []
+    for i, d in enumerate(common.tolist() + [0]):
+        lo = i
+        while open_ and open_[-1][0] > d:
+            depth, lo = open_.pop()
+            if depth >= min_pages and i + 1 - lo >= least:
+                found.append((depth, lo, i + 1))
+        if d and not (open_ and open_[-1][0] == d):
+            open_.append((d, lo))
+    if not found:
         return group, lens
-    for g, (_, pages, members) in enumerate(found[:max_groups]):
-        group[members] = g
-        lens[g] = pages * 64
+    d, lo, hi = np.array(found).T
+
+    # take the run that saves the most page reads next to those taken, until
+    # none does.  Its rows leave the longest shorter run taken around it (up:
+    # which, a: its depth), which may empty
+    rows_of = hi - lo          # not in a longer run taken
+    a, up = np.zeros_like(d), np.full_like(d, -1)
+    members = np.zeros_like(d)
+    taken = np.zeros(d.size, dtype=bool)
+    while taken.sum() < max_groups:
+        empties = (up >= 0) & (members[up] == rows_of)
+        gain = np.where(taken | (rows_of < least), 0,
+                        rows_of * (d - a) - d + np.where(empties, a, 0))
+        v = int(gain.argmax())
+        if gain[v] <= 0:
+            break
+        taken[v] = True
+        members[v] = rows_of[v]
+        if up[v] >= 0:
+            members[up[v]] -= rows_of[v]
+            taken[up[v]] = members[up[v]] > 0
+        around = (lo <= lo[v]) & (hi >= hi[v]) & (d < d[v])
+        rows_of[around & (d > a[v])] -= rows_of[v]
+        within = (lo >= lo[v]) & (hi <= hi[v]) & (d > d[v]) & (a < d[v])
+        a[within], up[within] = d[v], v
+
+    # the longest run taken that a row is in; runs left with too few: none
+    chosen = sorted(np.flatnonzero(taken).tolist(), key=lambda v: d[v])
+    while True:
+        owner = np.full(rows.size, -1)
+        for v in chosen:
+            owner[lo[v]:hi[v]] = v
+        sizes = {v: int((owner == v).sum()) for v in chosen}
+        kept = [v for v in chosen if sizes[v] >= least]
+        if len(kept) == len(chosen):
+            break
+        chosen = kept
+    saved = {v: (sizes[v] - 1) * int(d[v]) for v in chosen}
+    if not chosen or sum(saved.values()) < min_saved:
+        return group, lens
+    for g, v in enumerate(sorted(chosen, key=lambda v: -saved[v])):
+        group[rows[owner == v]] = g
+        lens[g] = d[v] * 64
     return group, lens
 
 

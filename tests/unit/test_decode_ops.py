@@ -658,6 +658,133 @@ def test_build_prefix_groups():
     assert none.shape == (0,)
 
 
+def _agent_rows(kinds, per, common, own, tail):
+    """Rows of several kinds: `common` pages for all, `own` pages of each
+    kind, `tail` of each row; in shuffled order."""
+    ids = iter(range(1 << 20))
+
+    def take(n):
+        return [next(ids) for _ in range(n)]
+
+    head, rows = take(common), []
+    for _ in range(kinds):
+        kind = head + take(own)
+        rows += [kind + take(tail) for _ in range(per)]
+    rows = np.array(rows, np.int32)
+    return rows[np.random.RandomState(kinds).permutation(len(rows))]
+
+
+def _pages_saved(table, lens, group, glens):
+    """After checking that every group is one."""
+    saved = 0
+    assert group.max(initial=-1) < len(glens)
+    for g, n in enumerate(glens):
+        rows = np.flatnonzero(group == g)
+        if rows.size == 0:
+            assert n == 0
+            continue
+        assert rows.size >= 2 and n > 0 and n % 64 == 0
+        assert (lens[rows] >= n).all()
+        assert (table[rows, :n // 64] == table[rows[0], :n // 64]).all()
+        saved += (rows.size - 1) * (n // 64)
+    return saved
+
+
+def test_prefix_groups_past_a_common_first_page():
+    """Three kinds with 8192 instructions each behind one page of preamble:
+    three groups, not one of the preamble."""
+    table = _agent_rows(3, 32, 1, 127, 3)
+    lens = np.full(96, 131 * 64 - 10)
+    group, glens = ops.build_prefix_groups(table, lens, max_groups=16)
+    assert sorted(glens[glens > 0]) == [8192] * 3
+    assert np.bincount(group).tolist() == [32] * 3
+    assert _pages_saved(table, lens, group, glens) == 3 * 31 * 128
+
+
+def test_prefix_groups_leave_a_short_row_out():
+    """One row that ends early does not cut the others' prefix."""
+    table = _agent_rows(1, 96, 0, 128, 1)
+    lens = np.full(96, 128 * 64 + 30)
+    for short in (70, 20):                 # one whole page, none
+        lens[17] = short
+        group, glens = ops.build_prefix_groups(table, lens, max_groups=16,
+                                               min_saved=94 * 128)
+        assert glens[glens > 0].tolist() == [8192]
+        assert np.flatnonzero(group < 0).tolist() == [17]
+    # two such rows are a group of their own
+    lens[17] = lens[40] = 70
+    group, glens = ops.build_prefix_groups(table, lens, max_groups=16)
+    assert glens[:3].tolist() == [8192, 64, 0]
+    assert np.flatnonzero(group == 1).tolist() == [17, 40]
+    group, glens = ops.build_prefix_groups(table, lens, min_rows=3)
+    assert np.flatnonzero(group < 0).tolist() == [17, 40]
+    group, glens = ops.build_prefix_groups(table, lens, min_pages=2)
+    assert np.flatnonzero(group < 0).tolist() == [17, 40]
+
+
+def test_prefix_groups_of_unrelated_rows_and_of_too_many_kinds():
+    rows = _agent_rows(40, 1, 0, 5, 1)
+    group, glens = ops.build_prefix_groups(rows, np.full(40, 380))
+    assert (group == -1).all() and (glens == 0).all()
+    table = _agent_rows(6, 4, 0, 9, 1)
+    lens = np.full(24, 9 * 64 + 5)
+    group, glens = ops.build_prefix_groups(table, lens, max_groups=4)
+    assert glens.tolist() == [9 * 64] * 4
+    assert np.bincount(group + 1).tolist() == [8, 4, 4, 4, 4]
+    none, glens = ops.build_prefix_groups(table, lens, max_groups=0)
+    assert (none == -1).all() and glens.size == 0
+
+
+def _most_saved(table, whole, rows, depth, given):
+    """The most page reads that groups of these rows can save, each row left
+    over worth `given` (its place in a group around): by trying both."""
+    if len(rows) == 1:
+        return given
+    while all(whole[r] > depth for r in rows) and len(
+            {table[r, depth] for r in rows}) == 1:
+        depth += 1
+    kinds = {}
+    for r in rows:
+        if whole[r] > depth:
+            kinds.setdefault(table[r, depth], []).append(r)
+    here = len(rows) - sum(map(len, kinds.values()))
+
+    def total(each):
+        return here * each + sum(_most_saved(table, whole, k, depth, each)
+                                 for k in kinds.values())
+
+    return max(total(given), total(depth) - depth if depth else 0)
+
+
+def test_prefix_groups_save_nearly_the_most():
+    """Random trees of runs: every group is one, and all together save what the
+    best one of them does or more (it is taken first, and each further one
+    adds), on average 99 % of what any choice can."""
+    rng = np.random.RandomState(0)
+    shares = []
+    for _ in range(400):
+        B, W, kinds = rng.randint(1, 14), rng.randint(1, 9), rng.randint(1, 4)
+        ids, table = {}, np.zeros((B, W), np.int32)
+        for b in range(B):
+            path = ()
+            for j in range(W):
+                path += (rng.randint(kinds) if rng.rand() < 0.5 else 0,)
+                table[b, j] = ids.setdefault(path, len(ids))
+        lens = rng.randint(0, W * 64 + 130, B)
+        saved = _pages_saved(table, lens, *ops.build_prefix_groups(table, lens))
+        whole = np.minimum(lens // 64, W)
+        runs = {}
+        for b in range(B):
+            for n in range(1, whole[b] + 1):
+                runs.setdefault(tuple(table[b, :n]), []).append(n)
+        one = max([(len(r) - 1) * r[0] for r in runs.values()], default=0)
+        most = _most_saved(table, whole, list(range(B)), 0, 0)
+        assert one <= saved <= most
+        if most:
+            shares.append(saved / most)
+    assert np.mean(shares) >= 0.99
+
+
 # --------------------------------------------------------------- refusals
 
 def _refusal_args(device):
