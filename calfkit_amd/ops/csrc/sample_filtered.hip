@@ -474,6 +474,7 @@ __device__ __forceinline__ Answer general(const Plain<T>& e, const Row& r,
     if (step == 1 && !(goal > 0.0)) {
       N = 0;
       ++step;
+      by_count = true;
       continue;
     }
     long long cnt = 0;

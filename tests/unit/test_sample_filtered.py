@@ -196,6 +196,24 @@ def test_general_search_rows():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("p", [0.0, -1.0])
+def test_general_search_of_rows_that_keep_one(p):
+    """top_p of 0 and less, over rows that no histogram holds."""
+    rng = torch.Generator().manual_seed(2)
+    x = (torch.randn(6, 5000, generator=rng)).to(torch.bfloat16)
+    x[:, 5] = 1e-30
+    x[3:] = x[3:, :1]                       # equal but for that one
+    x[3:, 5] = 1e-30
+    y = torch.zeros(6, 5000)
+    y[1:, 100:] = -7.0
+    y[3:, :2500] = torch.randn(2500, generator=rng) * 1e-6
+    y[3:, 2500:] = -10.0
+    for rows in (x, y):
+        _check(rows, [1.0, 0.9, 30.0] * 2, [0, 3, 4000] * 2, [p] * 6,
+               [0.0, 0.0, 0.5] * 2, [0.0, 0.6, 1 - 2.0 ** -24] * 2, "cuda")
+
+
+@pytest.mark.gpu
 def test_rows_beyond_32_bit_offsets():
     """The last rows of logits of more than 2^32 bytes; the others, not drawn,
     keep their outputs."""
