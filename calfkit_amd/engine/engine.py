@@ -84,7 +84,7 @@ def _encode_prefill(seqs) -> list[int]:
     for s in seqs:
         r = s.request
         names = r.tool_names or []
-        vals += [s.seq_id, r.max_new_tokens, int(r.temperature * 1e6),
+        vals += [s.seq_id, r.max_new_tokens, _float_bits(r.temperature),
                  r.top_k, _float_bits(r.top_p), _float_bits(r.min_p), r.seed,
                  int(r.ignore_eos),
                  r.tool_trigger if r.tool_names else -1, r.tool_ncalls,
@@ -99,7 +99,7 @@ def _decode_prefill(vals: list[int]) -> list["GenRequest"]:
     reqs = []
     i = 1
     for _ in range(vals[0]):
-        (sid, mx, temp_i, topk, topp, minp, seed, ig_eos, trig, ncalls,
+        (sid, mx, temp, topk, topp, minp, seed, ig_eos, trig, ncalls,
          n_names) = vals[i:i + 11]
         i += 11
         names = vals[i:i + n_names]
@@ -109,7 +109,7 @@ def _decode_prefill(vals: list[int]) -> list["GenRequest"]:
         ids = vals[i:i + n_ids]
         i += n_ids
         req = GenRequest(prompt_ids=list(ids), max_new_tokens=mx,
-                         temperature=temp_i / 1e6, top_k=topk,
+                         temperature=_bits_float(temp), top_k=topk,
                          top_p=_bits_float(topp), min_p=_bits_float(minp),
                          seed=seed,
                          ignore_eos=bool(ig_eos),

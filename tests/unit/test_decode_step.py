@@ -157,6 +157,15 @@ def test_lockstep_carries_the_filters():
     assert (got.top_k, got.seed, got.temperature) == (7, 9, 0.5)
 
 
+@pytest.mark.parametrize("temperature", [1e-7, 1 / 3, 0.7000004, 0.0, 2])
+def test_lockstep_carries_the_temperature_as_it_is(temperature):
+    """Every rank draws with the first one's temperature: one cut to 0 would
+    take the largest logit where the others draw."""
+    r = GenRequest(prompt_ids=[1, 2], temperature=temperature, top_p=0.9)
+    (_, got), = _decode_prefill(_encode_prefill([_Seq(4, r, None)]))
+    assert got.temperature == temperature and got.filtered == r.filtered
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("kv_dtype", ["bf16", "fp8"])
 def test_engine_graphs_match_eager(kv_dtype):
