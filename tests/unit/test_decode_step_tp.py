@@ -5,6 +5,7 @@ two-chunk decode pipeline against the plain forward."""
 import os
 from dataclasses import replace
 
+import numpy as np
 import pytest
 import torch
 import torch.multiprocessing as mp
@@ -141,3 +142,104 @@ def test_two_chunk_pipeline_matches_the_plain_forward():
     for plain, lap in (out[:2], out[2:]):
         # as for the pipeline over the bf16 cache: the same sums in chunks
         assert torch.allclose(plain, lap, atol=1e-3, rtol=1e-3)
+
+
+def _sliced(model, full, rank, world):
+    """The shard's weights from one whole model's."""
+    hq, hkv, dh, f = full.hq, full.hkv, full.dh, full.ffn_s
+
+    def part(t, dim=0):
+        return t.chunk(world, dim)[rank].contiguous()
+
+    model.embed, model.lm_head = full.embed, full.lm_head
+    for lw, fl in zip(model.layers, full.layers):
+        heads = fl.wqkv.split([hq * dh, hkv * dh, hkv * dh])
+        lw.wqkv = torch.cat([part(h) for h in heads])
+        lw.wo = part(fl.wo, 1)
+        lw.wgateup = torch.cat([part(h) for h in fl.wgateup.split([f, f])])
+        lw.wdown = part(fl.wdown, 1)
+    return model
+
+
+def _drive(model, filters):
+    """Prefill, prefill with prefix hits, decode to the end, in the same order
+    on every rank.  -> (logits of every draw, tokens of every request)"""
+    from concurrent.futures import Future
+
+    from calfkit_amd import ops
+    from calfkit_amd.engine.engine import GenRequest, InferenceEngine, _Seq
+
+    eng = InferenceEngine(model, max_batch=4, use_graphs=False,
+                          max_model_len=256, kv_dtype="fp8",
+                          shared_prefix=True)
+    prefix = [1] + [7 + (i * 37) % 400 for i in range(130)]
+    seqs = [_Seq(i + 1, GenRequest(prompt_ids=prefix + [20 + i],
+                                   max_new_tokens=9, ignore_eos=True,
+                                   seed=40 + i, **f), Future())
+            for i, f in enumerate(filters)]
+    logits, inner = [], ops.sample
+    # as arrays: a tensor in a queue belongs to the process that sent it
+    ops.sample = lambda out, x, *a, **k: (
+        logits.append(x.float().numpy().copy()), inner(out, x, *a, **k))[1]
+    try:
+        eng._prefill_batch(seqs[:1])
+        eng._prefill_batch(seqs[1:])
+        grouped = []
+        while eng._running:
+            eng._decode_step()
+            grouped.append(int((eng._group >= 0).sum()))
+    finally:
+        ops.sample = inner
+    assert max(grouped) == len(seqs)
+    return logits, [s.result.token_ids for s in seqs]
+
+
+def _values_worker(rank, world, port, q):
+    shard = _join(rank, world, port)
+    from calfkit_amd.engine import engine as engine_mod
+    from calfkit_amd.models.llama import LlamaShard
+
+    engine_mod.MIN_SHARED_BYTES = 0
+    full = LlamaShard(shard.cfg, device="cpu")
+    shard = _sliced(shard, full, rank, world)
+    out = []
+    for f in ([{}] * 3, [dict(temperature=0.8, top_p=0.9, min_p=0.01),
+                         dict(temperature=1.0, top_p=0.5, top_k=40),
+                         dict(temperature=0.7, min_p=0.02)]):
+        out.append(_drive(shard, f))
+    q.put((rank, out, _drive(full, [{}] * 3) if rank == 0 else None))
+    _leave()
+
+
+def test_sharded_engine_draws_the_tokens_of_every_rank_and_of_one():
+    """Greedy and filtered requests over an e4m3 cache with shared prefixes:
+    both ranks draw the same tokens, and the logits are those of the unsharded
+    model."""
+    (_, a, whole), (_, b, _) = _run(_values_worker, 29545)
+    for (la, ta), (lb, tb) in zip(a, b):
+        assert ta == tb and all(len(t) == 9 for t in ta)
+        assert all((x == y).all() for x, y in zip(la, lb))
+    # one rank rounds each of a layer's two projections once, two ranks round
+    # both parts and their sum: 4 roundings of 2^-8 between them, over two
+    # layers 16, 2^-4 if none cancels; rows stored in e4m3 that fall to another
+    # code (2^-4 and less, where such a rounding tips them) double that
+    bound = 2 ** -3
+    (got, tokens), (want, alone) = a[0], whole
+    assert len(got) == len(want)
+    # draws: the first request's, the others', then the steps of all three
+    rows = [[0], [1, 2]] + [[0, 1, 2]] * (len(got) - 2)
+    same, compared = [True] * 3, 0
+    step = [0, 0, 0]
+    for x, y, members in zip(got, want, rows):
+        for i, r in enumerate(members):
+            if not same[r] or step[r] >= 9:
+                continue
+            size = np.linalg.norm(y[i])
+            assert np.linalg.norm(x[i] - y[i]) <= bound * size
+            t = tokens[r][step[r]]
+            # the largest logit of one is within both errors of the other's
+            assert y[i].max() - y[i][t] <= 2 * bound * size
+            same[r] = t == alone[r][step[r]]
+            step[r] += 1
+            compared += 1
+    assert compared >= 3
