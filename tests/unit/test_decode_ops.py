@@ -337,6 +337,19 @@ def test_attn_decode_fp8_sharp_and_flat(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+def test_attention_with_a_negative_scale(device):
+    """The smallest product weighs most, in the own tokens, in a prefix and
+    where a row's end is masked."""
+    s = _batch([300, 77, 1, 64], 8, 2, seed=6)
+    _close(_decode(s, -0.3, device=device), *_expect(s, -0.3))
+    for fp8 in (False, True):
+        s = _shared_batch([0, 0, -1, 0], [128], [70, 1, 300, 33], 8, 2, seed=6,
+                          fp8=fp8)
+        s["glens"][0] = 100
+        _close(_shared(s, device, -0.3), *_expect(s, -0.3))
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_attn_decode_fp8_lengths_and_pages_out_of_range(device):
     """Lengths are taken to the table's width, negative ones are 0, and a page
     id outside the cache counts as a page without tokens."""
