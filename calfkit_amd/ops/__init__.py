@@ -780,7 +780,10 @@ def sample_filtered(out: torch.Tensor, logits: torch.Tensor,
     of the first's whole sum (1 or more: all); those whose weight is at least
     ``min_p`` (0 or less: all); never less than one.  The token is the first
     whose sum up to and with it passes ``uniform`` (in [0, 1)) times the kept
-    sum.  Sums are taken in 64 bits, so the token is the formula's.
+    sum.  Sums are taken in 64 bits, floating for bf16 and fixed point for most
+    f32 rows (a weight is off by 2^-47 of the largest at most with 128256
+    entries, 2^-49 with 32000, 2^-52 up to 4096), so the token is the formula's
+    where no border lies that near.
 
     A temperature that is not above 0 takes the largest logit.  A row without
     candidates gives token 0.  A row with a negative random number is not

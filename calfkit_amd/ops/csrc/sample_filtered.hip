@@ -20,8 +20,10 @@
 // counts are exact, and a row takes one exponential for each DISTINCT value
 // (about 1500) instead of one for each of 128256 entries.  fp32 logits take
 // linear bins of (m - x), with weights summed as 64-bit fixed point (integer
-// sums do not depend on the order of the atomics), and the bin that holds a
-// border is resolved by ranking its members.  Rows that fit neither (values
+// sums do not depend on the order of the atomics) in steps of 2^-51 of the
+// largest weight up to 4096 entries, 2^-48 at 32000, 2^-46 at 128256 and 2^-43
+// at 2^20, each weight rounded to half a step; the bin that holds a border is
+// resolved by ranking its members, whose weights are floating 64-bit ones.  Rows that fit neither (values
 // beyond 2^23, more distinct values than the list holds, a bin with too many
 // members) take a bisection over the keys, slow and general.
 //
@@ -54,7 +56,6 @@ constexpr int LISTED = BLOCK;  // equal values ranked one a thread
 // fp32
 constexpr int BINS32 = 8192;
 constexpr int MEMBERS = 2048;
-constexpr double FIXED = 8796093022208.0;  // 2^43: 2^20 entries sum below 2^63
 
 // 2^(j / 64), rounded to 64 bits.
 __constant__ const double POW2_64TH[64] = {
@@ -86,6 +87,9 @@ struct Args {
   const float* min_p;
   const float* uniform;
   int V;
+  // steps of 1 in the fixed point of fp32 rows: the finest whose V weights sum
+  // to 2^63 or less, 2^51 at most (a weight fits a double's 52 bits)
+  double steps, step;  // and 1 / steps
 };
 
 // What every path is asked: the row's filters.
@@ -789,7 +793,7 @@ struct Lds32 {
 
 template <int NC>
 __device__ __forceinline__ bool fp32_row(Entries<float, NC>& e, const Row& r,
-                                        Lds32& L, Answer& ans) {
+                                        const Args& a, Lds32& L, Answer& ans) {
   constexpr int PT = BINS32 / BLOCK;  // bins of a thread, in order
   Shared& s = L.s;
   const int tid = threadIdx.x;
@@ -825,7 +829,7 @@ __device__ __forceinline__ bool fp32_row(Entries<float, NC>& e, const Row& r,
     const int b = bin_of(x);
     // the sum with 2^52 has the rounded integer for its mantissa
     atomicAdd(&L.w[b], (unsigned long long)__double_as_longlong(
-                           fma(w, FIXED, 0x1p52)) &
+                           fma(w, a.steps, 0x1p52)) &
                            ((1ull << 52) - 1));
     atomicAdd(&L.n[b], 1u);
     nm += w >= s.min_p;
@@ -848,7 +852,7 @@ __device__ __forceinline__ bool fp32_row(Entries<float, NC>& e, const Row& r,
                                                                &w_fix);
   const unsigned long long bn = block_scan<unsigned long long>(tn, s.red_u,
                                                                &listed);
-  const double w_all = (double)w_fix * (1.0 / FIXED);
+  const double w_all = (double)w_fix * a.step;
 
   // ---- four questions, each to one bin: the sum of the first n_k, the rank
   // of the top-p border, the sum of the first N, the rank of the draw
@@ -883,8 +887,8 @@ __device__ __forceinline__ bool fp32_row(Entries<float, NC>& e, const Row& r,
       for (int j = 0; j < PT; ++j) {
         const unsigned n = binn[j];
         const unsigned long long ew = cw + binw[j], en = cn + n;
-        const double d0 = (double)cw * (1.0 / FIXED);
-        const double d1 = (double)ew * (1.0 / FIXED);
+        const double d0 = (double)cw * a.step;
+        const double d1 = (double)ew * a.step;
         if (n != 0 &&
             (by_count    ? ((long long)cn < rank && (long long)en >= rank)
              : step == 1 ? (d0 < goal && d1 >= goal)
@@ -1071,7 +1075,7 @@ __global__ __launch_bounds__(BLOCK) void sample_filtered_kernel(const Args a) {
       if constexpr (sizeof(T) == 2)
         done = bf16_row(e, r, L, ans);
       else
-        done = fp32_row(e, r, L, ans);
+        done = fp32_row(e, r, a, L, ans);
     }
   }
   // (known to be uniform, neither branch keeps the other's registers)
@@ -1089,6 +1093,7 @@ __global__ __launch_bounds__(BLOCK) void sample_filtered_kernel(const Args a) {
 #include <torch/extension.h>
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
+#include <cmath>
 
 void sample_filtered(torch::Tensor out, torch::Tensor logits,
                      torch::Tensor temperature, torch::Tensor top_k,
@@ -1119,6 +1124,8 @@ void sample_filtered(torch::Tensor out, torch::Tensor logits,
   if (B == 0) return;
   c10::DeviceGuard guard(dev);
   hipStream_t s = at::hip::getCurrentHIPStream().stream();
+  int bits = 51;
+  while (V > 1ll << (63 - bits)) --bits;
   const Args a{(int32_t*)out.data_ptr(),
                kept.has_value() ? (int32_t*)kept->data_ptr() : nullptr,
                logits.data_ptr(),
@@ -1127,7 +1134,9 @@ void sample_filtered(torch::Tensor out, torch::Tensor logits,
                (const float*)top_p.data_ptr(),
                (const float*)min_p.data_ptr(),
                (const float*)uniform.data_ptr(),
-               (int)V};
+               (int)V,
+               std::ldexp(1.0, bits),
+               std::ldexp(1.0, -bits)};
   // what a row has beyond the registers' 64 KB (bf16, short rows), 128 KB (f32)
   // or 256 KB is read again; 64 KB keep the instructions few: 256 rows of 8192
   // take 11.8 us against 14.9 with room for 256 KB, of 32000 19.8 against 23.3

@@ -213,6 +213,36 @@ def test_general_search_of_rows_that_keep_one(p):
                [0.0, 0.0, 0.5] * 2, [0.0, 0.6, 1 - 2.0 ** -24] * 2, "cuda")
 
 
+# one logit of 0 over 2000 of -c: with u these draw near a border, 2^-39 to
+# 2^-35 of the sum away from it.  A fixed point of 2^-43, whatever the row's
+# length, moves the sum of 2000 by up to 2^-33 and draws another token.
+NEAR_BORDERS = [(13.122835159301758, 0.9983434081077576),
+                (14.66104507446289, 0.9997100234031677),
+                (14.730710983276367, 0.9996070861816406),
+                (14.563593864440918, 0.9998524785041809),
+                (14.459906578063965, 0.9994561672210693),
+                (13.302825927734375, 0.9992644190788269)]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_fp32_draws_near_a_border(device):
+    V = 2001
+    x = torch.zeros(len(NEAR_BORDERS), V)
+    x[:, 1:] = -torch.tensor([c for c, _ in NEAR_BORDERS])[:, None]
+    u = [u for _, u in NEAR_BORDERS]
+    one = torch.ones(len(u), device=device)
+    none = torch.zeros(len(u), dtype=torch.int32, device=device)
+    out = none.clone()
+    ops.sample_filtered(out, x.to(device), one, none, one, 0 * one,
+                        torch.tensor(u, device=device))
+    for b, u in enumerate(u):
+        token, _, near = _formula(x[b], 1.0, 0, 1.0, 0.0, u)
+        # 2000 weights of 2^-18 and less and their sums in steps of 2^-51, each
+        # off by half of one, and a 64-bit sum to the border: 2^-40
+        assert 2.0 ** -39 < near < 2.0 ** -35
+        assert int(out[b]) == token
+
+
 @pytest.mark.gpu
 def test_rows_beyond_32_bit_offsets():
     """The last rows of logits of more than 2^32 bytes; the others, not drawn,
