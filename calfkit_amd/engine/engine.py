@@ -22,6 +22,7 @@ Decode runs (the hot loop):
 from __future__ import annotations
 
 import logging
+import numbers
 import queue
 import struct
 import threading
@@ -413,6 +414,10 @@ class InferenceEngine:
     # ---------------------------------------------------------------- submit
     def submit(self, request: GenRequest) -> Future:
         """Thread-safe; returns a Future[GenResult]."""
+        for name in ("top_p", "min_p"):  # here, where they end no one else's
+            v = getattr(request, name)
+            if not isinstance(v, numbers.Real):
+                raise TypeError(f"{name} must be a number: {v!r}")
         self.start()
         fut: Future = Future()
         with self._lock:

@@ -213,7 +213,7 @@ class LocalModelClient:
             max_new_tokens=max(1, s.max_tokens),
             temperature=s.temperature,
             top_k=s.top_k,
-            top_p=s.top_p,
+            top_p=1.0 if s.top_p is None else s.top_p,
             seed=s.seed or 0,
             ignore_eos=False,
             tool_names=tool_names,

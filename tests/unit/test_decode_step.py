@@ -1,10 +1,12 @@
 """The decode step's operators together: the engine with an e4m3 cache, shared
 prefixes and filtered draws, and a captured run of the three kernels."""
 
+import asyncio
 import threading
 import time
 import types
 
+import numpy as np
 import pytest
 import torch
 
@@ -13,8 +15,12 @@ from calfkit_amd.engine import engine as engine_mod
 from calfkit_amd.engine.engine import (GenRequest, InferenceEngine, _Seq,
                                        _decode_prefill, _encode_prefill)
 from calfkit_amd.engine.kvcache import KVCache
+from calfkit_amd.engine.local import LocalModelClient
+from calfkit_amd.engine.tokenizer import SyntheticTokenizer
+from calfkit_amd.messages import TextPart, UserMessage
 from calfkit_amd.models.config import TINY, get_config
 from calfkit_amd.models.llama import LlamaShard
+from calfkit_amd.schemas import EngineRequest, ModelSettings
 
 HD, PAGE = 128, 64
 
@@ -147,6 +153,41 @@ def test_filtered_rows_leave_the_others_alone_and_repeat():
     again = _agents(4, temperature=0.8, seed=5)
     again[1].top_p = 0.7
     assert _serve(_engine(), [again[1]]) == [a[1]]
+
+
+def test_a_filter_that_is_no_number_ends_its_own_request():
+    """It is refused where it is given; the requests beside it run on."""
+    eng = _engine()
+    try:
+        others = [eng.submit(r) for r in _agents(3, temperature=0.8, seed=5)]
+        for kw in (dict(top_p=None), dict(top_p="0.9"), dict(min_p=[0.1])):
+            with pytest.raises(TypeError):
+                eng.submit(_agents(1, temperature=0.8, **kw)[0])
+        others += [eng.submit(r) for r in _agents(1, temperature=0.8,
+                                                  top_p=np.float32(0.9))]
+        assert all(len(f.result(300).token_ids) == 9 for f in others)
+    finally:
+        eng.stop()
+
+
+def test_settings_without_a_top_p_are_unfiltered():
+    """A caller's settings may hold None for a value it leaves open."""
+    class Sink:
+        def emit(self, chunk):
+            pass
+
+    def answer(**kw):
+        client = LocalModelClient(TINY, device="cpu")
+        client._engine = _engine()
+        client._tokenizer = SyntheticTokenizer(TINY.vocab_size)
+        try:
+            return asyncio.run(client.complete(EngineRequest(
+                messages=(UserMessage((TextPart("hello"),)),), settings=ModelSettings(
+                    max_tokens=6, temperature=0.8, seed=4, **kw)), Sink())).text
+        finally:
+            client._engine.stop()
+
+    assert answer(top_p=None) == answer()
 
 
 def test_lockstep_carries_the_filters():
