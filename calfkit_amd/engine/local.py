@@ -214,6 +214,7 @@ class LocalModelClient:
             temperature=s.temperature,
             top_k=s.top_k,
             top_p=1.0 if s.top_p is None else s.top_p,
+            min_p=0.0 if s.min_p is None else s.min_p,
             seed=s.seed or 0,
             ignore_eos=False,
             tool_names=tool_names,

@@ -61,6 +61,9 @@ class ModelSettings:
     stop: tuple[str, ...] = ()
     #: parallel tool-call fan-out permitted
     parallel_tool_calls: bool = True
+    #: keep tokens of at least this part of the likeliest one's probability
+    #: (0 = off); of the in-process engine alone
+    min_p: float = 0.0
 
     def merged(self, other: "ModelSettings | None") -> "ModelSettings":
         """Overlay non-default fields of ``other`` on this instance."""
@@ -70,7 +73,7 @@ class ModelSettings:
         changes = {
             f: getattr(other, f)
             for f in ("max_tokens", "temperature", "top_p", "top_k", "seed", "stop",
-                       "parallel_tool_calls")
+                       "parallel_tool_calls", "min_p")
             if getattr(other, f) != getattr(base, f)
         }
         return replace(self, **changes) if changes else self

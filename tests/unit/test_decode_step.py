@@ -190,6 +190,29 @@ def test_settings_without_a_top_p_are_unfiltered():
     assert answer(top_p=None) == answer()
 
 
+def test_settings_reach_the_draw():
+    """An agent's top_p and min_p are its request's, its own over its model's."""
+    seen = []
+    client = LocalModelClient(TINY, device="cpu")
+    client._engine = eng = _engine()
+    client._tokenizer = SyntheticTokenizer(TINY.vocab_size)
+    inner = eng.submit
+    eng.submit = lambda r: (seen.append(r), inner(r))[1]
+
+    class Sink:
+        def emit(self, chunk):
+            pass
+
+    own = ModelSettings(max_tokens=3, temperature=0.5, min_p=0.05)
+    try:
+        asyncio.run(client.complete(EngineRequest(
+            messages=(UserMessage((TextPart("hello"),)),),
+            settings=ModelSettings(top_p=0.8, min_p=0.2).merged(own)), Sink()))
+    finally:
+        eng.stop()
+    assert (seen[0].top_p, seen[0].min_p, seen[0].filtered) == (0.8, 0.05, True)
+
+
 def test_lockstep_carries_the_filters():
     r = GenRequest(prompt_ids=[1, 2], temperature=0.5, top_k=7, seed=9,
                    top_p=0.9, min_p=0.05)
