@@ -59,11 +59,11 @@ RUN_STEPS = (8, 4, 2, 1)
 MAX_PREFIX_GROUPS = 16
 #: bytes of one layer's cache that groups save a step from being read, below
 #: which rows run without them: a pass over prefixes and its join cost up to
-#: 5 us.  Measured with cold caches, 32/8 heads, bf16, groups against none:
-#: 67 MB (256 rows of 64 shared tokens) 96.5 against 91.8 us, 66 MB (64 of 256)
-#: 32.2 / 31.1, 126 MB (16 of 2048) 25.2 / 25.1, 132 MB (64 of 512) 34.1 / 37.1,
-#: 134 MB (256 of 128) 95.0 / 93.8, 252 MB (16 of 4096) 28.9 / 36.2, 264 MB (64
-#: of 1024) 34.8 / 44.6
+#: 8 us.  Measured with cold caches, 32/8 heads, bf16, groups against none:
+#: 67 MB (256 rows of 64 shared tokens) 97.9 against 90.0 us, 66 MB (64 of 256)
+#: 31.8 / 32.5, 126 MB (16 of 2048) 23.8 / 25.3, 132 MB (64 of 512) 33.1 / 35.6,
+#: 134 MB (256 of 128) 95.8 / 92.4, 252 MB (16 of 4096) 29.4 / 35.7, 264 MB (64
+#: of 1024) 34.7 / 44.8; 16 pairs of 1024 (67 MB) 36.3 / 39.4, of 8192 162 / 187
 MIN_SHARED_BYTES = 128 << 20
 
 #: lockstep op channel opcodes (tensor-coded: the
@@ -1024,7 +1024,7 @@ class InferenceEngine:
                        self._temperature[:pad], self._seeds[i],
                        self._topk[:pad], row_seeds=self._row_seeds[i, :pad])
             # rows that filter by top-p or min-p are drawn again from their
-            # own logits; without any, every block leaves at once
+            # own logits; without any, every block leaves at once (2.4 us)
             ops.sample_filtered(self._sampled[i, :pad], logits,
                                 self._temperature[:pad], self._ftopk[:pad],
                                 self._topp[:pad], self._minp[:pad],

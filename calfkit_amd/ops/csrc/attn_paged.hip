@@ -21,10 +21,10 @@
 // The matrix instruction takes bf16, so each weight of P goes through it as two
 // terms: its upper bits, and what they leave out, rounded, which loses at most
 // 2^-15 of it (one term alone would lose 2^-8, as much as the output's own
-// rounding).  The sum l is the terms', so that the weights sum to 1.  Beside
-// own tokens the second term costs nothing (256 rows of 700 tokens 49 us either
+// rounding).  The sum l is the terms', so that the weights sum to 1.  Among own
+// tokens the second term costs nothing (256 rows of 700 tokens 49 us either
 // way), in the shared pass its products and splits take 512 rows with 3 prefixes
-// of 8192 tokens from 134 to 157 us, 256 rows of 2048 from 64 to 67.
+// of 8192 tokens from 134 to 156 us, 256 rows of 2048 from 64 to 67.
 //
 // e4m3 rows become bf16 on the way in (scale times code is exact in bf16), so
 // both caches share one arithmetic.
@@ -43,13 +43,17 @@
 // 52.9, 52.2, 56.4.
 #define ROOM 512
 // Blocks of its prefixes, one a CU, beside which one of own tokens runs.  512
-// rows in 3 groups of 8192 tokens (300 of their own, e4m3): 155 us at 192, 134
-// at 256, 143 at 384, 159 at 512; 256 rows of 2048 tokens (300, bf16): 65.1,
-// 66.8, 72.6, 77.3.
+// rows in 3 groups of 8192 tokens (300 of their own, e4m3): 186 us at 192, 156
+// at 256, 163 at 384, 172 at 512; 256 rows of 2048 tokens (300, bf16): 64.7,
+// 67.2, 71.7, 77.4.
 #define PRE_ROOM 256
-// Pages of a split or of a prefix's piece, at least.  One row of 777 tokens:
-// 12.1 us at 1, 10.2 at 2, 11.8 at 4; 4 rows of 1024 shared tokens 22.4, 21.0,
-// 23.9 (cold).
+// Pages of a prefix's piece, at least, and of a split where the row fills its
+// table.  One row of 777 tokens in 13 pages 9.0 us at 1, 8.3 at 2, 9.2 at 4; 4
+// rows of 1024 shared tokens 15.0, 14.2, 16.5.  The number of splits follows from
+// the table's width, so that a short row in a wide table is cut finer, down to
+// half pages.  The same bound on the device, for the row's length, takes one row
+// of 100 tokens in 129 pages from 9.2 to 9.5 us and 32 of them from 9.5 to 8.7:
+// not taken.  (3.3 of that is the join; in 2 pages, unsplit, 5.5 and 5.7.)
 #define LEAST 2
 // Splits of a row and pieces of a tile's prefix, at most: both together are
 // joined by one wave.  One row of 32768 tokens 57 us at 8, 35 at 16, 33 at 32.
@@ -215,13 +219,15 @@ __device__ __forceinline__ float join_weight(const float m, const float l,
 // the next half page's loads under this one's products gained nothing).  Page
 // ids come 64 at a time, one a lane.
 //
-// Bound: the bytes of the cache, in random panels of 4 KB (bf16: 8 KB) halves:
-// a kernel that only loads them, cold, reaches 3.5 to 3.9 TB/s where a plain
-// read of one block of memory reaches 6.1.  Measured, e4m3, 32/8 heads: 256
-// rows of up to 700 tokens 49 us, 4.2 TB/s; 8 rows of up to 32768 tokens (64/8
-// heads) 92 us, 5.0 TB/s; one row of 777 tokens (8/2 heads) 9.7 us, of which
-// the join is 3.  The matrix instructions run mostly empty (G of 16 columns) and
-// still take a tenth of the vector instructions that dot products would.
+// Bound: the bytes of the cache, in random panels of 4 KB (bf16: 8 KB) halves.
+// e4m3, 256 rows of 700 tokens, again and again / with other memory read between:
+// 71 / 126 us, a kernel that loads their pages and does nothing else 61 / 123; 8
+// rows of 32768 tokens 102 / 160, the loads 92 / 156.  Measured on changing
+// inputs, 32/8 heads: 256 rows of up to 700 tokens 49 us, 4.2 TB/s; 8 rows of up
+// to 32768 tokens (64/8 heads) 93 us, 5.0 TB/s; one row of 777 tokens 9.6 us, of
+// which the join is 3.3.  The matrix instructions run mostly empty (2G of 16
+// columns) and still take a tenth of the vector instructions that dot products
+// would.
 #define UNIT 32  // tokens of one step
 
 #define NW 4  // waves of a block
@@ -552,11 +558,13 @@ __global__ __launch_bounds__(4 * WAVE) void paged_join_kernel(
 // page's loads in flight under this page's products.  Bound: the matrix
 // instructions and, at 32 rows a wave, LDS reads at the same rate (each 1 KB
 // fragment feeds one 32x32x16 product of 32 cycles, four SIMDs to 128 B a
-// cycle).  Measured by itself with two blocks a CU: 512 rows (32/8 heads) in 3
-// groups of 8192 e4m3 tokens 102 us, 670 TFLOP/s, of a CU's busy cycles the
-// matrix units 35 %, vector units 40 %, LDS 37 %; 256 rows of 2048 bf16 tokens
-// 25.7 us.  blockIdx.x % hkv is the KV head, so that with 8 of them each XCD's
-// L2 holds one head's prefixes for every tile.
+// cycle; V's feed two, a weight's terms).  Measured without own tokens, with the
+// join: 512 rows (32/8 heads) in 3 groups of 8192 e4m3 tokens 147 us (125 with
+// one term a weight), 470 TFLOP/s without the second terms' products; 256 rows
+// of 2048 bf16 tokens 38 us.  With own tokens, of a CU's busy cycles the matrix
+// units work 31 %, the vector units 44 %, LDS 33 %: one wave a SIMD alternates
+// between exponentials and products.  blockIdx.x % hkv is the KV head, so that
+// with 8 of them each XCD's L2 holds one head's prefixes for every tile.
 struct PrefixLds {
   // two pages of K, then two of V
   __hip_bfloat16 pages[2 * KVPAGE * (K_PITCH + V_PITCH32)];
@@ -863,10 +871,10 @@ __device__ __forceinline__ void prefix_pieces(const Paged& a, const int kvh,
 
 // Both in one launch: a KV head's first npre blocks are the prefixes', bound by
 // products, the others its rows' own tokens, bound by bytes, and each covers
-// the other's waits: 512 rows in 3 groups of 8192 + 300 tokens 134 us where the
-// two one after the other took 142, 256 rows of 2048 + 300 67 / 71, 4 rows of
-// 1024 + 90 13.1 / 18.0.  Two blocks a CU cost the own tokens nothing (256 rows
-// of 700, cold: 125.1 us at four, 126.5 at two).
+// the other's waits: with one term a weight 512 rows in 3 groups of 8192 + 300
+// tokens took 134 us where the two one after the other took 142, 256 rows of
+// 2048 + 300 67 / 71, 4 rows of 1024 + 90 13.1 / 18.0.  Two blocks a CU cost the
+// own tokens nothing (256 rows of 700, cold: 125.1 us at four, 126.5 at two).
 template <bool FP8, bool WIDE>
 __global__ __launch_bounds__(NW * WAVE, 2) void paged_shared_kernel(
     const Paged a, __hip_bfloat16* __restrict__ out) {

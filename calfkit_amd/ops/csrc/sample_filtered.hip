@@ -23,18 +23,26 @@
 // sums do not depend on the order of the atomics) in steps of 2^-51 of the
 // largest weight up to 4096 entries, 2^-48 at 32000, 2^-46 at 128256 and 2^-43
 // at 2^20, each weight rounded to half a step; the bin that holds a border is
-// resolved by ranking its members, whose weights are floating 64-bit ones.  Rows that fit neither (values
-// beyond 2^23, more distinct values than the list holds, a bin with too many
-// members) take a bisection over the keys, slow and general.
+// resolved by ranking its members, whose weights are floating 64-bit ones.
+//
+// Rows that fit neither take a bisection over the keys, general and slow: 69
+// passes over the row in memory with an exponential an entry, 137 under a top-p,
+// 2.8 and 5.6 ms for 128256 bf16 entries, 1.9 and 3.4 ms for as many equal fp32
+// ones, 0.3 and 0.5 ms for 12000.  They are, bf16: a magnitude of 2^23 or more
+// (or below 2^-41, but 0) among values that count, over 4096 distinct values;
+// fp32: an infinity, a range beyond the type's, over 2048 entries in the bin of a
+// border (equal logits; 128256 random ones take 80 to 110 us by bins).
 //
 // One block of 1024 threads is one row; it reads the row once and holds it in
-// registers (128256 bf16 are 64 registers a thread).  Bound: the histogram, one LDS
-// add an entry: 13 to 18 cycles an instruction of 64 lanes (LDS itself is busy
-// for 8, half of them bank conflicts), up to 37000 of the 62000 cycles of a bf16
-// row of 128256; then the row's bytes.  Measured: one bf16 row of 128256 15 to 24 us, 512 of them 67.5 us (1.9 TB/s;
-// a CU takes two, the histograms 31 us of it), 64 fp32 rows of 32000 45 us
-// (64-bit exponentials and two histograms).  Sorting the 512 rows with library
-// calls takes 11.7 ms.
+// registers (128256 bf16 are 64 registers a thread).  Bound: the histogram, one
+// LDS add an entry: 13 to 18 cycles an instruction of 64 lanes (LDS itself is
+// busy for 8, half of them bank conflicts), up to 37000 of the 62000 cycles of a
+// bf16 row of 128256; then the row's bytes.  Measured: one bf16 row of 128256 24
+// to 28 us whatever its filters (the later its rank, the longer), 11 us at
+// temperature 0; 512 of them 68 us (1.9 TB/s; a CU takes two, one after the
+// other, the histograms 31 us of it), 64 fp32 rows of 32000 45 us (64-bit
+// exponentials and two histograms); rows that are not drawn 2.3 us for 1 and 2.4
+// for 512, as any launch.  Sorting the 512 rows with library calls takes 11.7 ms.
 
 #include "common.h"
 
